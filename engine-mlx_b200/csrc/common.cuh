@@ -26,6 +26,8 @@ enum : int {
   kDevTimeoutPeer = 2,  // a peer flag wait exceeded its spin limit
   kDevBadToken = 3,     // a token id outside [0, vocab)
   kDevKvOverflow = 4,   // position >= KV capacity
+  kDevBadPage = 5,      // a page table entry outside [0, n_pages)
+  kDevBadBatch = 6,     // rows or lengths that do not describe a batch
 };
 
 // Upper bound on the polls of any spin-wait before it reports and returns.

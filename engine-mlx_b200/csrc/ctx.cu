@@ -106,8 +106,9 @@ int ctx_sync_check(emx_ctx* c, const char* what) {
   EMX_CHECK_CUDA(cudaMemcpy(&st, c->status, sizeof(int), cudaMemcpyDeviceToHost), "status read");
   if (st != 0) {
     static const char* names[] = {"ok", "shared-memory barrier wait timed out", "peer flag wait timed out",
-                                  "token id out of range", "KV capacity exceeded"};
-    const char* nm = (st > 0 && st < 5) ? names[st] : "unknown";
+                                  "token id out of range", "KV capacity exceeded", "page outside the cache",
+                                  "rows or lengths that do not describe a batch"};
+    const char* nm = (st > 0 && st < 7) ? names[st] : "unknown";
     return fail(EMX_ERR_DEVICE, "%s: device status %d (%s)", what, st, nm);
   }
   return EMX_OK;

@@ -1,0 +1,575 @@
+// paged_attn.cu — attention of a batch's new rows over a paged K/V cache
+// whose first positions all sequences share.
+//
+// Row r of sequence i (q head g of KV head h) at position p:
+//   o = sum_j e^{s_j} v_j / sum_j e^{s_j},  s_j = scale q . k_j,  j <= p.
+// The positions fall in two parts, the common prefix [0, S) and the
+// sequence's own [S, p], and each part in pieces; a piece gives
+//   m = max s_j, l = sum e^{s_j - m}, O = sum e^{s_j - m} v_j   (base 2, fp32)
+// and pieces join as O = sum_x 2^{m_x - m} O_x, l likewise, o = O / l.  So the
+// prefix is read once for all rows of the batch, as one sequence whose rows
+// are every row, and the own parts once for their few rows.
+//
+// Workers.  A warp is a worker: it takes an even share of the key tiles (16
+// keys) of all segments — (sequence, KV head, tile of 16 or 32 rows) — in one
+// line (paged_plan.h), so lengths from one to the longest balance to within a
+// tile, without the host knowing them.  A share's pieces: a segment's first
+// tiles go to the piece slot of its rows, a share that begins inside a segment
+// to the slot of its worker; a second kernel joins the pieces of each row
+// (and a segment that one worker has whole is written by it).
+#include "paged_dev.cuh"
+
+namespace emx {
+
+namespace {
+
+constexpr int kKT = 16;       // keys of a tile
+constexpr int kWarps = 4;     // workers of a CTA
+constexpr int kStages = 3;    // tiles in flight a worker
+constexpr int kMaxSeqs = 1024;
+constexpr int kCtasPerSm = 2;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+  const int n = on ? 16 : 0;  // 0: the 16 bytes become zeros, nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+// Pieces of one part (own or shared): first[] by row and q head, more[] by worker.
+struct Pieces {
+  float* first_o;    // [n_rows * n_q][HD]
+  float2* first_ml;  // [n_rows * n_q]
+  float* more_o;     // [workers][rows of a tile][HD]
+  float2* more_ml;   // [workers][rows of a tile]
+};
+
+struct Work {
+  PagedAttnArgs a;
+  Pieces own, shared;
+  int64_t* starts;  // [n_seqs + 1] tiles before each sequence (own part)
+  int own_workers, shared_workers;
+  int own_mt, shared_mt;  // rows of a tile
+};
+
+// starts[0..n_seqs] of all sequences into shared memory, by the whole CTA.
+template <int THREADS>
+__device__ __forceinline__ void plan_starts(const PagedAttnArgs& a, const Line& line, int64_t* starts, bool report) {
+  __shared__ int64_t wsum[THREADS / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (a.p.n_seqs + THREADS - 1) / THREADS;  // consecutive sequences of a thread
+  const int i0 = min(a.p.n_seqs, tid * per), i1 = min(a.p.n_seqs, i0 + per);
+  int64_t sum = 0;
+  for (int i = i0; i < i1; ++i) {
+    const SeqInfo s = line.seq(i);
+    if (!s.ok && report) report_status(a.p.status, seq_status(a.p, i));
+    const int64_t t = line.tiles(s);
+    starts[i] = t;
+    sum += t;
+  }
+  int64_t incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) wsum[warp] = incl;
+  __syncthreads();
+  int64_t run = incl - sum;
+  for (int w = 0; w < warp; ++w) run += wsum[w];
+  for (int i = i0; i < i1; ++i) {
+    const int64_t t = starts[i];
+    starts[i] = run;
+    run += t;
+  }
+  if (tid == THREADS - 1) {  // its run ends the line
+    starts[a.p.n_seqs] = run;
+  }
+  __syncthreads();
+}
+
+template <int HD, int NT, bool SHARED>
+struct Worker {
+  static constexpr int MT = 16 * NT;
+  static constexpr int kRowB = HD * 2;             // bytes of a cached row
+  static constexpr int kTileB = kKT * kRowB;       // one tile of K (or V)
+  static constexpr int kStageB = 2 * kTileB;
+  static constexpr int kChunks = HD / 8;           // 16-byte chunks of a row
+  static constexpr int kCopies = kKT * kChunks / 32;
+
+  const Work& w;
+  Line line;
+  int lane;
+  uint32_t ring;       // this warp's stages
+  uint32_t* valid;     // [kStages] bit j: key j of the tile is there
+
+  // 16-byte chunk c of row r: rows of a tile hit all banks of ldmatrix
+  static __device__ __forceinline__ uint32_t at(int r, int c) {
+    return (uint32_t)(r * kRowB + ((c ^ (r & 7)) << 4));
+  }
+
+  // Cache row of key `lane` (< 16) of the cursor's tile, ~0 where there is none.
+  __device__ __forceinline__ uint32_t key_row(const Cursor& c) const {
+    const PagedAttnArgs& a = w.a;
+    const int pos = (SHARED ? 0 : a.shared_len) + c.k * kKT + (lane & 15);
+    uint32_t row = ~0u;
+    if (pos < c.s.len) {
+      const int pg = pos / a.p.page_size;
+      const int page = SHARED ? a.shared_pages[pg] : a.p.table[(size_t)c.seq * a.p.max_pages + pg];
+      if (page >= 0 && page < a.p.n_pages)
+        row = cache_row(page, a.p.n_kv, c.head(), a.p.page_size, pos - pg * a.p.page_size);
+      else
+        report_status(a.p.status, kDevBadPage);
+    }
+    return row;
+  }
+
+  __device__ __forceinline__ void issue(int stage, uint32_t row) const {
+    const uint32_t base = ring + stage * kStageB;
+    const unsigned there = __ballot_sync(0xffffffffu, row != ~0u) & 0xffffu;
+    if (lane == 0) valid[stage] = there;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int r = (i * 32 + lane) / kChunks, c = lane % kChunks;
+      const uint32_t src = __shfl_sync(0xffffffffu, row, r);
+      const bool on = src != ~0u;
+      const size_t off = on ? (size_t)src * HD + c * 8 : 0;
+      cp_async16(base + at(r, c), w.a.p.k + off, on);
+      cp_async16(base + kTileB + at(r, c), w.a.p.v + off, on);
+    }
+  }
+
+  __device__ __forceinline__ void run(int64_t total, int worker, int workers) const;
+};
+
+// The share of `worker` of `workers` in the line's `total` tiles.
+template <int HD, int NT, bool SHARED>
+__device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int64_t total, int worker, int workers) const {
+  const PagedAttnArgs& a = w.a;
+  const Pieces& pc = SHARED ? w.shared : w.own;
+  const int64_t x0 = share_begin(total, worker, workers), x1 = share_begin(total, worker + 1, workers);
+  const int n = (int)(x1 - x0);
+  if (n <= 0) return;
+  Cursor ld, cc;
+  const int hpg = line.hpg;
+  cc.seek(line, x0);
+  ld = cc;
+  uint32_t row = key_row(ld);
+  int loaded = 0;
+  for (; loaded < kStages - 1; ++loaded) {
+    if (loaded < n) {
+      issue(loaded, row);
+      if (loaded + 1 < n) {
+        ld.next(line);
+        row = key_row(ld);
+      }
+    }
+    cp_commit();
+  }
+  const float sl2 = a.scale * kLog2e;
+  const int quad = lane >> 2, col = (lane & 3) * 2;
+
+  uint32_t qf[NT][HD / 16][4];
+  float o[NT][HD / 8][4];
+  float m[NT][2], l[NT][2];
+  int vis[NT][2];  // keys of this part that the row sees
+  int least = 0;   // fewest of them over the tile's rows
+  bool fresh = true, whole = false;
+  int R = 0, row_base = 0, h = 0;
+  for (int t = 0; t < n; ++t) {
+    if (fresh) {
+      // a segment begins for this worker: its rows of q, and how far they see
+      fresh = false;
+      whole = cc.k == 0;
+      h = cc.seg / cc.mt;
+      row_base = (cc.seg - h * cc.mt) * MT;
+      R = cc.s.rows * hpg;
+      least = 0x7fffffff;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int r = row_base + nt * 16 + quad + b * 8;
+          const bool on = r < R;
+          const int tok = r / hpg;
+          vis[nt][b] = !on ? 0 : SHARED ? a.shared_len : cc.s.len - cc.s.rows + tok + 1 - a.shared_len;
+          if (on) least = min(least, vis[nt][b]);
+          m[nt][b] = -INFINITY;
+          l[nt][b] = 0.f;
+          const bf16* qr = a.q + ((size_t)(cc.s.row0 + (on ? tok : 0)) * a.p.n_q + h * hpg + (on ? r - tok * hpg : 0)) * HD;
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            qf[nt][ks][b] = on ? *reinterpret_cast<const uint32_t*>(qr + ks * 16 + col) : 0u;
+            qf[nt][ks][b + 2] = on ? *reinterpret_cast<const uint32_t*>(qr + ks * 16 + col + 8) : 0u;
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < HD / 8; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][d][e] = 0.f;
+      }
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, x));
+    }
+    // ---- the next load, then this tile
+    if (loaded < n) {
+      issue(loaded % kStages, row);
+      ++loaded;
+      if (loaded < n) {
+        ld.next(line);
+        row = key_row(ld);
+      }
+    }
+    cp_commit();
+    cp_wait<kStages - 1>();
+    __syncwarp();
+    const int stage = t % kStages;
+    const uint32_t K = ring + stage * kStageB, V = K + kTileB;
+    const uint32_t there = valid[stage];
+    const int key0 = cc.k * kKT;  // within the part
+
+    float s[NT][2][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][j][e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      uint32_t kf[4];  // keys 0-7 (dims lo, hi), keys 8-15 (dims lo, hi)
+      ldsm4(kf, K + at((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mma_bf16_16816(s[nt][0], qf[nt][ks][0], qf[nt][ks][1], qf[nt][ks][2], qf[nt][ks][3], kf[0], kf[1]);
+        mma_bf16_16816(s[nt][1], qf[nt][ks][0], qf[nt][ks][1], qf[nt][ks][2], qf[nt][ks][3], kf[2], kf[3]);
+      }
+    }
+    uint32_t pf[NT][4];
+    bool moved = false;
+    float alpha[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int key = j * 8 + col + e;
+            const bool on = key0 + key < vis[nt][b] && ((there >> key) & 1u);
+            float& v = s[nt][j][2 * b + e];
+            v = on ? v * sl2 : -INFINITY;
+            mx = fmaxf(mx, v);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float to = fmaxf(m[nt][b], mx);
+        const float base = to == -INFINITY ? 0.f : to;  // nothing seen yet: weights 2^-inf = 0
+        alpha[nt][b] = ex2f(m[nt][b] - base);
+        moved |= to > m[nt][b];
+        m[nt][b] = to;
+        float sum = 0.f;
+        float pv[2][2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            pv[j][e] = ex2f(s[nt][j][2 * b + e] - base);
+          }
+        // weights go to the products in bf16: each is off by at most 2^-9 of
+        // itself, and l sums the rounded ones, so a constant V comes out exact
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const __nv_bfloat162 two = __floats2bfloat162_rn(pv[j][0], pv[j][1]);
+          const uint32_t u = *reinterpret_cast<const uint32_t*>(&two);
+          pf[nt][b + 2 * j] = u;
+          sum += __uint_as_float(u << 16) + __uint_as_float(u & 0xffff0000u);
+        }
+        l[nt][b] = l[nt][b] * alpha[nt][b] + sum;
+      }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int d = 0; d < HD / 8; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][d][e] *= alpha[nt][e >> 1];
+    }
+    // A row that does not see a key gives it weight 0, and 0 * inf is NaN: a
+    // tile that some rows see further into than others and whose V holds
+    // something not finite takes its products one visible key at a time.
+    bool odd = false;
+    if (!SHARED && key0 + kKT > least) {
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const uint4 u = *reinterpret_cast<const uint4*>(__cvta_shared_to_generic(V + (i * 32 + lane) * 16));
+        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= (x[e] & 0x7f80u) == 0x7f80u || (x[e] & 0x7f800000u) == 0x7f800000u;
+      }
+      odd = __any_sync(0xffffffffu, odd);
+    }
+    if (!odd) {
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) {
+        uint32_t vf[4];  // dims lo (keys lo, hi), dims hi (keys lo, hi)
+        ldsm4t(vf, V + at((lane & 7) + (((lane >> 3) & 1) << 3), d * 2 + (lane >> 4)));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma_bf16_16816(o[nt][2 * d], pf[nt][0], pf[nt][1], pf[nt][2], pf[nt][3], vf[0], vf[1]);
+          mma_bf16_16816(o[nt][2 * d + 1], pf[nt][0], pf[nt][1], pf[nt][2], pf[nt][3], vf[2], vf[3]);
+        }
+      }
+    } else {
+      for (int key = 0; key < kKT; ++key) {
+        const int from = (lane & ~3) | ((key & 7) >> 1);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const uint32_t u = __shfl_sync(0xffffffffu, key < 8 ? pf[nt][b] : pf[nt][b + 2], from);
+            const float pw = (key & 1) ? __uint_as_float(u & 0xffff0000u) : __uint_as_float(u << 16);
+            const bool on = key0 + key < vis[nt][b] && ((there >> key) & 1u);
+#pragma unroll
+            for (int d = 0; d < HD / 8; ++d) {
+              const uint32_t x =
+                  *reinterpret_cast<const uint32_t*>(__cvta_shared_to_generic(V + at(key, d) + (lane & 3) * 4));
+              if (on) {
+                o[nt][d][2 * b] = fmaf(pw, __uint_as_float(x << 16), o[nt][d][2 * b]);
+                o[nt][d][2 * b + 1] = fmaf(pw, __uint_as_float(x & 0xffff0000u), o[nt][d][2 * b + 1]);
+              }
+            }
+          }
+      }
+    }
+    __syncwarp();  // the stage may be filled again
+
+    const bool last = cc.k + 1 == cc.kt;
+    if (last || t + 1 == n) {
+      // ---- this worker's piece of the segment
+      const bool direct = whole && last && !SHARED && a.shared_len == 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          float ls = l[nt][b];
+          ls += __shfl_xor_sync(0xffffffffu, ls, 1);
+          ls += __shfl_xor_sync(0xffffffffu, ls, 2);
+          const int r = row_base + nt * 16 + quad + b * 8;
+          if (r >= R) continue;
+          const int tok = r / hpg;
+          const size_t head = (size_t)(cc.s.row0 + tok) * a.p.n_q + h * hpg + (r - tok * hpg);
+          if (direct) {
+            const float inv = ls > 0.f ? 1.f / ls : ls == 0.f ? 0.f : ls;  // no key seen: zeros; NaN stays
+#pragma unroll
+            for (int d = 0; d < HD / 8; ++d) {
+              const __nv_bfloat162 two = __floats2bfloat162_rn(o[nt][d][2 * b] * inv, o[nt][d][2 * b + 1] * inv);
+              *reinterpret_cast<__nv_bfloat162*>(a.out + head * HD + d * 8 + col) = two;
+            }
+          } else {
+            const size_t slot = whole ? head : (size_t)worker * MT + (r - row_base);
+            float* dst = (whole ? pc.first_o : pc.more_o) + slot * HD;
+#pragma unroll
+            for (int d = 0; d < HD / 8; ++d)
+              *reinterpret_cast<float2*>(dst + d * 8 + col) = make_float2(o[nt][d][2 * b], o[nt][d][2 * b + 1]);
+            if ((lane & 3) == 0) (whole ? pc.first_ml : pc.more_ml)[slot] = make_float2(m[nt][b], ls);
+          }
+        }
+      fresh = true;
+    }
+    if (t + 1 < n) cc.next(line);
+  }
+  cp_wait<0>();
+}
+
+template <int HD, int NT, bool SHARED>
+__global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const __grid_constant__ Work w) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int64_t starts[SHARED ? 1 : kMaxSeqs + 1];
+  __shared__ uint32_t valid[kWarps][kStages];
+  using Wk = Worker<HD, NT, SHARED>;
+  const int warp = threadIdx.x >> 5;
+  const Line line = make_line(w.a.p, w.a.shared_len, !SHARED, Wk::MT, kKT, starts);
+  int64_t total;
+  if (SHARED) {
+    total = line.tiles(line.seq(0));
+  } else {
+    plan_starts<kWarps * 32>(w.a, line, starts, blockIdx.x == 0);
+    total = starts[w.a.p.n_seqs];
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.x; i <= w.a.p.n_seqs; i += kWarps * 32) w.starts[i] = starts[i];
+  }
+  pdl_trigger();
+  if (total == 0) return;
+  Wk k{w, line, (int)(threadIdx.x & 31), smem_u32(smem) + warp * (uint32_t)(kStages * Wk::kStageB), valid[warp]};
+  k.run(total, blockIdx.x * kWarps + warp, gridDim.x * kWarps);
+}
+
+// One warp a (row, q head): joins its pieces.
+template <int HD>
+__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ Work w) {
+  const PagedAttnArgs& a = w.a;
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  pdl_wait();
+  if (item >= (int64_t)a.p.n_rows * a.p.n_q) return;
+  const int row = (int)(item / a.p.n_q), hq = (int)(item - (int64_t)row * a.p.n_q);
+  const int hpg = a.p.n_q / a.p.n_kv, h = hq / hpg;
+  const int i = warp_find_seq(a.p.indptr, a.p.n_seqs, row);
+  if (i >= a.p.n_seqs || row < a.p.indptr[i]) return;  // behind the last sequence: left as it was
+  const SeqInfo s = load_seq(a.p, i, a.shared_len);
+  constexpr int E = HD / 32;
+  bf16* dst = a.out + (size_t)item * HD + lane * E;
+  float o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  auto take = [&](const float* src, float2 ml) {
+    float v[E];
+    if constexpr (E == 4) {
+      const float4 f = *reinterpret_cast<const float4*>(src + lane * E);
+      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    } else {
+      const float2 f = *reinterpret_cast<const float2*>(src + lane * E);
+      v[0] = f.x, v[1] = f.y;
+    }
+    const float to = fmaxf(m, ml.x), base = to == -INFINITY ? 0.f : to;
+    const float x = ex2f(m - base), y = ex2f(ml.x - base);
+    l = l * x + ml.y * y;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = o[e] * x + v[e] * y;
+    m = to;
+  };
+  // the pieces of row r (of its sequence) in one part; x0: the tiles before the sequence, T all
+  auto part = [&](const Pieces& pc, const Line& line, const SeqInfo& s, int workers, int64_t T, int64_t x0, int r) {
+    const int kt = line.key_tiles(s);
+    x0 += ((int64_t)h * line.row_tiles(s) + r / line.mt) * kt;
+    const int c0 = share_of(T, x0, workers), c1 = share_of(T, x0 + kt - 1, workers);
+    if (c0 == c1 && a.shared_len == 0) return false;  // one worker had the segment whole and wrote it
+    take(pc.first_o + item * HD, pc.first_ml[item]);
+    for (int c = c0 + 1; c <= c1; ++c) {
+      if (share_begin(T, c, workers) == share_begin(T, c + 1, workers)) continue;
+      const size_t slot = (size_t)c * line.mt + r % line.mt;
+      take(pc.more_o + slot * HD, pc.more_ml[slot]);
+    }
+    return true;
+  };
+  if (s.ok) {
+    const int g = hq - h * hpg;
+    const Line own = make_line(a.p, a.shared_len, true, w.own_mt, kKT, w.starts);
+    if (!part(w.own, own, s, w.own_workers, w.starts[a.p.n_seqs], w.starts[i], (row - s.row0) * hpg + g)) return;
+    if (a.shared_len > 0) {
+      const Line all = make_line(a.p, a.shared_len, false, w.shared_mt, kKT, nullptr);
+      part(w.shared, all, all.seq(0), w.shared_workers, all.tiles(all.seq(0)), 0, row * hpg + g);
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+  uint32_t u[E / 2];
+#pragma unroll
+  for (int e = 0; e < E / 2; ++e) {
+    const __nv_bfloat162 two = __floats2bfloat162_rn(o[2 * e] * inv, o[2 * e + 1] * inv);
+    u[e] = *reinterpret_cast<const uint32_t*>(&two);
+  }
+  if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(u[0], u[1]);
+  else *reinterpret_cast<uint32_t*>(dst) = u[0];
+}
+
+size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// The workspace's parts; returns its size (base may be null).
+size_t lay_out(Work& w, int num_sms, unsigned char* base) {
+  const PagedArgs& p = w.a.p;
+  const size_t heads = (size_t)p.n_rows * p.n_q;
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    void* q = base ? base + off : nullptr;
+    off += up(bytes);
+    return q;
+  };
+  w.starts = static_cast<int64_t*>(take(sizeof(int64_t) * (kMaxSeqs + 1)));
+  w.own_workers = w.shared_workers = num_sms * kCtasPerSm * kWarps;
+  auto pieces = [&](Pieces& pc) {
+    pc.first_o = static_cast<float*>(take(heads * p.head_dim * sizeof(float)));
+    pc.first_ml = static_cast<float2*>(take(heads * sizeof(float2)));
+    pc.more_o = static_cast<float*>(take((size_t)w.own_workers * 32 * p.head_dim * sizeof(float)));
+    pc.more_ml = static_cast<float2*>(take((size_t)w.own_workers * 32 * sizeof(float2)));
+  };
+  pieces(w.own);
+  if (w.a.shared_len > 0) pieces(w.shared);
+  return off;
+}
+
+template <int HD, int NT, bool SHARED>
+cudaError_t launch_part(const Work& w, int workers, cudaStream_t st) {
+  const int smem = kWarps * kStages * Worker<HD, NT, SHARED>::kStageB;
+  static cudaError_t once = cudaFuncSetAttribute(paged_attn_kernel<HD, NT, SHARED>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (once != cudaSuccess) return once;
+  paged_attn_kernel<HD, NT, SHARED><<<workers / kWarps, kWarps * 32, smem, st>>>(w);
+  return cudaGetLastError();
+}
+
+template <int HD>
+cudaError_t launch(Work& w, cudaStream_t st) {
+  const PagedArgs& p = w.a.p;
+  const int hpg = p.n_q / p.n_kv;
+  w.own_mt = (int64_t)p.n_rows * hpg > 16 * (int64_t)p.n_seqs ? 32 : 16;
+  w.shared_mt = (int64_t)p.n_rows * hpg > 16 ? 32 : 16;
+  cudaError_t e = cudaSuccess;
+  if (w.a.shared_len > 0) {
+    e = w.shared_mt == 32 ? launch_part<HD, 2, true>(w, w.shared_workers, st)
+                          : launch_part<HD, 1, true>(w, w.shared_workers, st);
+    if (e != cudaSuccess) return e;
+  }
+  e = w.own_mt == 32 ? launch_part<HD, 2, false>(w, w.own_workers, st)
+                     : launch_part<HD, 1, false>(w, w.own_workers, st);
+  if (e != cudaSuccess) return e;
+  const int64_t items = (int64_t)p.n_rows * p.n_q;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((items + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<HD>, static_cast<const Work>(w));
+}
+
+}  // namespace
+
+size_t paged_attn_workspace(int n_rows, int n_q, int n_kv, int head_dim, int shared_len, int num_sms) {
+  Work w = {};
+  w.a.p.n_rows = n_rows;
+  w.a.p.n_q = n_q;
+  w.a.p.n_kv = n_kv;
+  w.a.p.head_dim = head_dim;
+  w.a.shared_len = shared_len;
+  return lay_out(w, num_sms, nullptr);
+}
+
+cudaError_t paged_attn_launch(const PagedAttnArgs& a, int num_sms, cudaStream_t st) {
+  Work w = {};
+  w.a = a;
+  lay_out(w, num_sms, static_cast<unsigned char*>(a.workspace));
+  return a.p.head_dim == 128 ? launch<128>(w, st) : launch<64>(w, st);
+}
+
+}  // namespace emx

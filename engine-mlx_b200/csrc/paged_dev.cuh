@@ -1,0 +1,42 @@
+// paged_dev.cuh — device helpers of the paged-cache kernels.
+#pragma once
+#include "paged.cuh"
+
+namespace emx {
+
+__device__ __forceinline__ SeqInfo load_seq(const PagedArgs& p, int i, int shared) {
+  return seq_info(p.indptr[i], p.indptr[i + 1], p.lengths[i], p.n_rows, shared, (int64_t)p.max_pages * p.page_size);
+}
+
+__device__ __forceinline__ Line make_line(const PagedArgs& p, int shared_len, bool own, int mt, int keys,
+                                          const int64_t* starts) {
+  return Line{own, p.n_seqs, p.n_rows, p.n_kv, p.n_q / p.n_kv, shared_len, mt, keys, (int64_t)p.max_pages * p.page_size,
+              p.indptr, p.lengths, starts};
+}
+
+// The status a sequence that is not in order reports.
+__device__ __forceinline__ int seq_status(const PagedArgs& p, int i) {
+  return (int64_t)p.lengths[i] > (int64_t)p.max_pages * p.page_size ? kDevKvOverflow : kDevBadBatch;
+}
+
+// The sequence that batch row `row` belongs to: the first i with
+// indptr[i + 1] > row, by all 32 lanes of a warp, or n_seqs.  Every read is
+// inside indptr whatever it holds; the caller checks indptr[i] <= row, which
+// an indptr that does not ascend may break.
+__device__ __forceinline__ int warp_find_seq(const int* indptr, int n_seqs, int row) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = n_seqs;  // the answer is in [lo, lo + n]
+  while (n > 0) {
+    const int stride = (n + 31) / 32;
+    const int at = min(lo + (lane + 1) * stride, lo + n);  // lane's block of sequences ends before `at`
+    const unsigned hit = __ballot_sync(0xffffffffu, indptr[at] > row);
+    if (!hit) return lo + n;
+    const int first = __ffs(hit) - 1;
+    const int b = lo + first * stride, e = min(b + stride, lo + n);
+    lo = b;
+    n = e - b - 1;  // the answer is one of [b, e): e - 1 if no earlier one has it
+  }
+  return lo;
+}
+
+}  // namespace emx

@@ -1,0 +1,130 @@
+// paged_plan.h — the index arithmetic of the batched operators over a paged
+// K/V cache: which rows, positions and pages belong to a sequence, and how
+// the key tiles of all (sequence, KV head, row tile) segments are dealt out
+// to a fixed grid.  Plain integer functions, shared by the kernels and by a
+// host test that walks every index for whole batches.
+#pragma once
+#include <stdint.h>
+
+#ifdef __CUDACC__
+#define EMX_HD __host__ __device__ __forceinline__
+#else
+#define EMX_HD inline
+#endif
+
+namespace emx {
+
+// One sequence of a batch: rows [row0, row0 + rows) of the batch are its last
+// `rows` positions, of `len` in all.  !ok: the batch names rows, or a length,
+// that cannot be (see seq_info).
+struct SeqInfo {
+  int row0, rows, len;
+  bool ok;
+};
+
+// rows [a, b) of a batch of n_rows, `len` positions of which the first
+// `shared` belong to the common prefix, `room` positions in the page table.
+// A sequence without rows is always in order (nothing of it is looked at).
+EMX_HD SeqInfo seq_info(int a, int b, int len, int n_rows, int shared, int64_t room) {
+  SeqInfo s;
+  s.ok = true;
+  if (a < 0 || b < a || b > n_rows) {
+    s.row0 = s.rows = s.len = 0;
+    s.ok = false;
+    return s;
+  }
+  s.row0 = a;
+  s.rows = b - a;
+  s.len = len;
+  if (s.rows > 0 && (len < 0 || (int64_t)len < (int64_t)shared + s.rows || (int64_t)len > room)) s.ok = false;
+  return s;
+}
+
+EMX_HD int ceil_div(int a, int b) { return (int)(((int64_t)a + b - 1) / b); }
+
+// Row (in units of head_dim elements) of the cache [n_pages, n_kv, page_size]
+// that holds position `off` of page `page` for KV head h.  A pool of
+// 64-element bf16 rows with more than 2^32 of them would not fit the device.
+EMX_HD uint32_t cache_row(int page, int n_kv, int h, int page_size, int off) {
+  return ((uint32_t)page * (uint32_t)n_kv + (uint32_t)h) * (uint32_t)page_size + (uint32_t)off;
+}
+
+// Segments: (KV head, row tile) pairs of one sequence, row tiles innermost,
+// each of `kt` key tiles.  Tiles of sequence i are [start_i, start_{i+1}) of
+// the batch's T; worker c of G takes [c T / G, (c + 1) T / G).
+EMX_HD int64_t share_begin(int64_t T, int c, int G) { return T * c / G; }
+// The worker that has tile x: the largest c whose share begins at or before x
+// (shares may be empty when T < G, and an empty share is never the answer).
+EMX_HD int share_of(int64_t T, int64_t x, int G) { return (int)(((x + 1) * G - 1) / T); }
+
+// The line of key tiles of one part of a batch's positions: the common prefix
+// [0, shared_len), as one sequence with every row of the batch, or (own) each
+// sequence's positions from shared_len on.  Row tiles hold `mt` rows (a row
+// being one q head of one new token), key tiles `keys` positions.
+struct Line {
+  bool own;
+  int n_seqs, n_rows, n_kv, hpg, shared_len, mt, keys;
+  int64_t room;          // positions of a page table
+  const int* indptr;
+  const int* lengths;
+  const int64_t* starts;  // own: tiles before each sequence
+
+  EMX_HD SeqInfo seq(int i) const {
+    if (own) return seq_info(indptr[i], indptr[i + 1], lengths[i], n_rows, shared_len, room);
+    SeqInfo s;
+    s.row0 = 0;
+    s.rows = n_rows;
+    s.len = shared_len;
+    s.ok = true;
+    return s;
+  }
+  EMX_HD int row_tiles(const SeqInfo& s) const { return (int)(((int64_t)s.rows * hpg + mt - 1) / mt); }
+  EMX_HD int key_tiles(const SeqInfo& s) const { return ceil_div(own ? s.len - shared_len : s.len, keys); }
+  EMX_HD int64_t tiles(const SeqInfo& s) const {
+    if (!s.ok || s.rows == 0) return 0;
+    return (int64_t)n_kv * row_tiles(s) * key_tiles(s);
+  }
+};
+
+// Where a worker stands in a line.
+struct Cursor {
+  int seq, seg, k;  // sequence, segment within it, key tile within that
+  int mt, kt;       // row tiles a KV head, key tiles a segment
+  SeqInfo s;
+
+  EMX_HD void enter(const Line& line) {
+    s = line.seq(seq);
+    mt = line.row_tiles(s);
+    kt = line.key_tiles(s);
+  }
+  // To tile x < T.
+  EMX_HD void seek(const Line& line, int64_t x) {
+    seq = 0;
+    if (line.own) {
+      int lo = 0, hi = line.n_seqs - 1;  // the last sequence that begins at or before x
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (line.starts[mid] <= x) lo = mid;
+        else hi = mid - 1;
+      }
+      seq = lo;
+      x -= line.starts[lo];
+    }
+    enter(line);
+    seg = (int)(x / kt);
+    k = (int)(x - (int64_t)seg * kt);
+  }
+  // To the next tile; the caller does not go past the last one.
+  EMX_HD void next(const Line& line) {
+    if (++k < kt) return;
+    k = 0;
+    if (++seg < mt * line.n_kv || !line.own) return;
+    seg = 0;
+    do ++seq;
+    while (seq < line.n_seqs - 1 && line.starts[seq + 1] == line.starts[seq]);
+    if (seq < line.n_seqs) enter(line);
+  }
+  EMX_HD int head() const { return seg / mt; }
+};
+
+}  // namespace emx

@@ -41,6 +41,18 @@ class QwenConfig(C.Structure):
             "expert_bits", "expert_group", "kv_cap", "max_prefill")]
 
 
+class PagedKVStruct(C.Structure):
+    """emx_paged_kv"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_int) for n in ("n_pages", "page_size", "n_kv",
+                                                                               "head_dim")]
+
+
+class PagedBatchStruct(C.Structure):
+    """emx_paged_batch"""
+    _fields_ = [(n, C.c_int) for n in ("n_seqs", "n_rows", "max_pages")] + [
+        (n, C.c_void_p) for n in ("indptr", "lengths", "table")]
+
+
 _SIGS = {
     "emx_last_error": (C.c_char_p, []),
     "emx_version": (C.c_char_p, []),
@@ -84,6 +96,13 @@ _SIGS = {
     "emx_moe_route": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),
     "emx_gather_qmm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int] + [C.c_void_p] * 4 + [C.c_int, C.c_void_p] +
                        [C.c_int] * 5),
+    "emx_paged_append": (C.c_int, [C.c_void_p] * 4 + [C.c_float, C.c_float, C.c_int, C.POINTER(PagedKVStruct),
+                                                      C.POINTER(PagedBatchStruct), C.c_void_p]),
+    "emx_sdpa_paged_workspace": (C.c_int, [C.c_void_p, C.POINTER(PagedKVStruct), C.POINTER(PagedBatchStruct), C.c_int,
+                                           C.c_int, C.POINTER(C.c_size_t)]),
+    "emx_sdpa_paged": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(PagedKVStruct), C.POINTER(PagedBatchStruct), C.c_int,
+                                 C.c_float, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]),
+    "emx_verify_draft": (C.c_int, [C.c_void_p] * 3 + [C.c_int] + [C.c_void_p] * 3 + [C.c_int] * 3 + [C.c_void_p] * 2),
     "emx_comm_unique_id": (C.c_int, [C.c_void_p]),
     "emx_comm_init": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_void_p)]),
     "emx_comm_destroy": (C.c_int, [C.c_void_p]),
@@ -197,6 +216,32 @@ class Buffer:
         return out
 
 
+def _ptr(x) -> Optional[int]:
+    """Device address of a Buffer, or of anything with data_ptr() (a torch tensor); None for None."""
+    if x is None:
+        return None
+    return x.ptr if isinstance(x, Buffer) else x.data_ptr()
+
+
+class PagedKV:
+    """The paged K/V cache of one layer (emx_paged_kv): device arrays bf16
+    [n_pages, n_kv, page_size, head_dim].  Keeps the arrays alive."""
+
+    def __init__(self, k, v, n_pages: int, page_size: int, n_kv: int, head_dim: int):
+        self.k, self.v = k, v
+        self.c = PagedKVStruct(_ptr(k), _ptr(v), n_pages, page_size, n_kv, head_dim)
+
+
+class PagedBatch:
+    """A batch over a paged cache (emx_paged_batch): device int32 arrays indptr
+    [n_seqs + 1], lengths [n_seqs] and table [n_seqs, max_pages], whose
+    contents may change from call to call.  Keeps the arrays alive."""
+
+    def __init__(self, indptr, lengths, table, n_seqs: int, n_rows: int, max_pages: int):
+        self.indptr, self.lengths, self.table = indptr, lengths, table
+        self.c = PagedBatchStruct(n_seqs, n_rows, max_pages, _ptr(indptr), _ptr(lengths), _ptr(table))
+
+
 class Ctx:
     """MlxCtx equivalent: one device and one stream (crates/mlx-ffi/src/ops/real/mod.rs:4-41)."""
 
@@ -205,6 +250,7 @@ class Ctx:
         _check(lib().emx_ctx_create(int(device), C.byref(h)))
         self.h = h.value
         self.device = device
+        self._workspace = None  # sdpa_paged's, where the caller brings none
 
     def close(self):
         if self.h:
@@ -378,6 +424,51 @@ class Ctx:
         _check(lib().emx_gather_qmm(self.h, x.ptr, int(x_per_slot), w.ptr, s.ptr, b.ptr, idx.ptr, n_slots, out.ptr,
                                     n_experts, N, K, group_size, bits))
         return out
+
+    # --- a batch of sequences over a paged cache; device arrays are Buffers or
+    # torch tensors, whose contents must be complete before the call: it runs
+    # on this context's stream
+    def paged_append(self, qkv, kv, batch, n_q, q_norm=None, k_norm=None, eps=1e-6, theta=1e6, out=None):
+        """Per-head norm and rotation of q and k, k and v to their pages; returns q bf16 [n_rows, n_q, head_dim]."""
+        if out is None:
+            out = self.alloc(batch.c.n_rows * n_q * kv.c.head_dim * 2)
+        _check(lib().emx_paged_append(self.h, _ptr(qkv), _ptr(q_norm), _ptr(k_norm), eps, theta, n_q, kv.c, batch.c,
+                                      _ptr(out)))
+        return out
+
+    def sdpa_paged_workspace(self, kv, batch, n_q, shared_len=0) -> int:
+        """Bytes of workspace that sdpa_paged needs."""
+        n = C.c_size_t()
+        _check(lib().emx_sdpa_paged_workspace(self.h, kv.c, batch.c, n_q, shared_len, C.byref(n)))
+        return n.value
+
+    def sdpa_paged(self, q, kv, batch, n_q, scale, shared_len=0, shared_pages=None, out=None, workspace=None):
+        """Attention of the batch's rows, the first shared_len positions read once for all; `workspace` is a
+        Buffer of sdpa_paged_workspace bytes (by default one that the context keeps and grows)."""
+        if out is None:
+            out = self.alloc(batch.c.n_rows * n_q * kv.c.head_dim * 2)
+        if workspace is None:
+            need = self.sdpa_paged_workspace(kv, batch, n_q, shared_len)
+            if self._workspace is None or self._workspace.nbytes < need:
+                if self._workspace is not None:
+                    self._workspace.free()
+                    self._workspace = None
+                self._workspace = self.alloc(need)
+            workspace = self._workspace
+        _check(lib().emx_sdpa_paged(self.h, _ptr(q), kv.c, batch.c, n_q, scale, shared_len, _ptr(shared_pages), _ptr(out),
+                                    workspace.ptr, workspace.nbytes))
+        return out
+
+    def verify_draft(self, target, draft, tokens, uniforms, n_seqs, n_draft, vocab, dtype=F32, counts=None, out=None,
+                     accepted=None):
+        """Speculative sampling's acceptance: (tokens int32 [n_seqs, n_draft + 1], accepted int32 [n_seqs])."""
+        if out is None:
+            out = self.alloc(n_seqs * (n_draft + 1) * 4)
+        if accepted is None:
+            accepted = self.alloc(n_seqs * 4)
+        _check(lib().emx_verify_draft(self.h, _ptr(target), _ptr(draft), dtype, _ptr(tokens), _ptr(counts),
+                                      _ptr(uniforms), n_seqs, n_draft, vocab, _ptr(out), _ptr(accepted)))
+        return out, accepted
 
 
 # --------------------------------------------------------------------- comm

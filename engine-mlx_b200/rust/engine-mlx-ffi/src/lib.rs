@@ -194,6 +194,57 @@ impl MlxCtx {
     pub fn argmax(&self, x: &DeviceBuffer, rows: i32, n: i32, out: &mut DeviceBuffer) -> Result<()> {
         check(unsafe { sys::emx_argmax(self.raw, x.as_ptr(), rows, n, out.as_mut_ptr() as *mut i32) }, "argmax")
     }
+
+    // ---- a batch of sequences over a paged cache (emx.h describes the two
+    // structs; their device arrays must outlive the enqueued work, and what
+    // they hold is read on the device)
+    /// Per-head norm and rotation of q and k, k and v to their pages of the cache.
+    ///
+    /// # Safety
+    /// The pointers in `kv` and `batch` must be device arrays of the sizes they state.
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn paged_append(&self, qkv: &DeviceBuffer, q_norm: Option<&DeviceBuffer>,
+                               k_norm: Option<&DeviceBuffer>, eps: f32, rope_theta: f32, n_q: i32,
+                               kv: &sys::emx_paged_kv, batch: &sys::emx_paged_batch, q_out: &mut DeviceBuffer)
+                               -> Result<()> {
+        let opt = |b: Option<&DeviceBuffer>| b.map_or(std::ptr::null(), |b| b.as_ptr());
+        check(sys::emx_paged_append(self.raw, qkv.as_ptr(), opt(q_norm), opt(k_norm), eps, rope_theta, n_q, kv, batch,
+                                    q_out.as_mut_ptr()), "paged_append")
+    }
+    /// Bytes of workspace that `sdpa_paged` needs.
+    pub fn sdpa_paged_workspace(&self, kv: &sys::emx_paged_kv, batch: &sys::emx_paged_batch, n_q: i32,
+                                shared_len: i32) -> Result<usize> {
+        let mut n = 0usize;
+        check(unsafe { sys::emx_sdpa_paged_workspace(self.raw, kv, batch, n_q, shared_len, &mut n) },
+              "sdpa_paged_workspace")?;
+        Ok(n)
+    }
+    /// Attention of a batch's rows over the cache, the pages `shared_pages` of
+    /// the first `shared_len` positions read once for all sequences.
+    ///
+    /// # Safety
+    /// As `paged_append`.
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn sdpa_paged(&self, q: &DeviceBuffer, kv: &sys::emx_paged_kv, batch: &sys::emx_paged_batch, n_q: i32,
+                             scale: f32, shared_len: i32, shared_pages: Option<&DeviceBuffer>,
+                             out: &mut DeviceBuffer, workspace: &mut DeviceBuffer) -> Result<()> {
+        let pages = shared_pages.map_or(std::ptr::null(), |b| b.as_ptr() as *const i32);
+        let bytes = workspace.len();
+        check(sys::emx_sdpa_paged(self.raw, q.as_ptr(), kv, batch, n_q, scale, shared_len, pages, out.as_mut_ptr(),
+                                  workspace.as_mut_ptr(), bytes), "sdpa_paged")
+    }
+    /// Speculative sampling's acceptance of drafted tokens (`dtype`: sys::EMX_F32 or sys::EMX_BF16).
+    #[allow(clippy::too_many_arguments)]
+    pub fn verify_draft(&self, target: &DeviceBuffer, draft: Option<&DeviceBuffer>, dtype: i32, tokens: &DeviceBuffer,
+                        counts: Option<&DeviceBuffer>, uniforms: &DeviceBuffer, n_seqs: i32, n_draft: i32, vocab: i32,
+                        out: &mut DeviceBuffer, accepted: &mut DeviceBuffer) -> Result<()> {
+        let opt = |b: Option<&DeviceBuffer>| b.map_or(std::ptr::null(), |b| b.as_ptr());
+        check(unsafe {
+            sys::emx_verify_draft(self.raw, target.as_ptr(), opt(draft), dtype, tokens.as_ptr() as *const i32,
+                                  opt(counts) as *const i32, uniforms.as_ptr() as *const f32, n_seqs, n_draft, vocab,
+                                  out.as_mut_ptr() as *mut i32, accepted.as_mut_ptr() as *mut i32)
+        }, "verify_draft")
+    }
 }
 
 impl Drop for MlxCtx {

@@ -15,6 +15,8 @@ pub const EMX_DEV_TIMEOUT_MBAR: c_int = 1;
 pub const EMX_DEV_TIMEOUT_PEER: c_int = 2;
 pub const EMX_DEV_BAD_TOKEN: c_int = 3;
 pub const EMX_DEV_KV_OVERFLOW: c_int = 4;
+pub const EMX_DEV_BAD_PAGE: c_int = 5;
+pub const EMX_DEV_BAD_BATCH: c_int = 6;
 pub const EMX_UNIQUE_ID_BYTES: c_int = 128;
 
 pub const EMX_BF16: c_int = 0;
@@ -83,6 +85,28 @@ pub struct emx_st_tensor {
     pub bytes: u64,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct emx_paged_kv {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub n_pages: c_int,
+    pub page_size: c_int,
+    pub n_kv: c_int,
+    pub head_dim: c_int,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct emx_paged_batch {
+    pub n_seqs: c_int,
+    pub n_rows: c_int,
+    pub max_pages: c_int,
+    pub indptr: *const i32,
+    pub lengths: *const i32,
+    pub table: *const i32,
+}
+
 extern "C" {
     pub fn emx_set_error_handler(handler: emx_error_handler, data: *mut c_void);
     pub fn emx_last_error() -> *const c_char;
@@ -125,6 +149,10 @@ extern "C" {
     pub fn emx_scatter_single(ctx: *mut emx_ctx, cache: *mut c_void, offset: *const i32, upd: *const c_void, nkv: c_int, cap: c_int, head_dim: c_int) -> c_int;
     pub fn emx_moe_route(ctx: *mut emx_ctx, router_logits: *const c_void, n_experts: c_int, top_k: c_int, normalize: c_int, idx: *mut i32, weights: *mut f32) -> c_int;
     pub fn emx_gather_qmm(ctx: *mut emx_ctx, x: *const c_void, x_per_slot: c_int, w: *const c_void, scales: *const c_void, biases: *const c_void, idx: *const i32, n_slots: c_int, y: *mut c_void, n_experts: c_int, N: c_int, K: c_int, group_size: c_int, bits: c_int) -> c_int;
+    pub fn emx_paged_append(ctx: *mut emx_ctx, qkv: *const c_void, q_norm: *const c_void, k_norm: *const c_void, eps: f32, rope_theta: f32, n_q: c_int, kv: *const emx_paged_kv, batch: *const emx_paged_batch, q_out: *mut c_void) -> c_int;
+    pub fn emx_sdpa_paged_workspace(ctx: *mut emx_ctx, kv: *const emx_paged_kv, batch: *const emx_paged_batch, n_q: c_int, shared_len: c_int, bytes: *mut usize) -> c_int;
+    pub fn emx_sdpa_paged(ctx: *mut emx_ctx, q: *const c_void, kv: *const emx_paged_kv, batch: *const emx_paged_batch, n_q: c_int, scale: f32, shared_len: c_int, shared_pages: *const i32, out: *mut c_void, workspace: *mut c_void, workspace_bytes: usize) -> c_int;
+    pub fn emx_verify_draft(ctx: *mut emx_ctx, target: *const c_void, draft: *const c_void, dtype: c_int, tokens: *const i32, counts: *const i32, uniforms: *const f32, n_seqs: c_int, n_draft: c_int, vocab: c_int, out: *mut i32, accepted: *mut i32) -> c_int;
     pub fn emx_comm_unique_id(id_out: *mut c_void) -> c_int;
     pub fn emx_comm_init(ctx: *mut emx_ctx, unique_id: *const c_void, nranks: c_int, rank: c_int, out: *mut *mut emx_comm) -> c_int;
     pub fn emx_comm_destroy(comm: *mut emx_comm) -> c_int;

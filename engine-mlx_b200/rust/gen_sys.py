@@ -19,7 +19,7 @@ SCALAR = {"int": "c_int", "float": "f32", "int32_t": "i32", "int64_t": "i64", "u
           "size_t": "usize", "char": "c_char", "void": "c_void", "emx_dtype": "c_int",
           "emx_error_handler": "emx_error_handler", "emx_token_cb": "emx_token_cb"}
 OPAQUE = ["emx_ctx", "emx_comm", "emx_qwen3"]
-STRUCTS = ["emx_qwen3_config", "emx_st_tensor"]
+STRUCTS = ["emx_qwen3_config", "emx_st_tensor", "emx_paged_kv", "emx_paged_batch"]
 RUST_KEYWORDS = {"type", "ref", "mut", "fn", "in", "loop", "match", "move", "self", "use", "where"}
 
 

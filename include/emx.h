@@ -46,6 +46,8 @@ extern "C" {
 #define EMX_DEV_TIMEOUT_PEER 2 /* a bounded peer-flag wait gave up */
 #define EMX_DEV_BAD_TOKEN 3    /* token id outside [0, vocab) */
 #define EMX_DEV_KV_OVERFLOW 4  /* position >= KV capacity */
+#define EMX_DEV_BAD_PAGE 5     /* page table entry outside [0, n_pages) */
+#define EMX_DEV_BAD_BATCH 6    /* rows or lengths that do not describe a batch */
 
 typedef enum { EMX_BF16 = 0, EMX_F32 = 1, EMX_U32 = 2, EMX_I32 = 3 } emx_dtype;
 
@@ -191,6 +193,90 @@ int emx_moe_route(emx_ctx* ctx, const void* router_logits, int n_experts, int to
 int emx_gather_qmm(emx_ctx* ctx, const void* x, int x_per_slot, const void* w, const void* scales,
                    const void* biases, const int32_t* idx, int n_slots, void* y, int n_experts, int N, int K,
                    int group_size, int bits);
+
+/* ------------------------------------------------- batches, paged cache
+ * One step of batched, speculative serving (no reference counterpart: its
+ * cache and decode step hold one sequence).  The new rows of all sequences
+ * leave the q|k|v projection together (emx_paged_append), attend
+ * (emx_sdpa_paged), and drafted tokens are kept or replaced
+ * (emx_verify_draft).  Everything that changes from step to step — lengths,
+ * rows, page tables — is read on the device, and no call allocates or waits,
+ * so a step may be captured into a graph and replayed. */
+
+/* The K/V cache of one layer: bf16 [n_pages, n_kv, page_size, head_dim] each
+ * (a page of one head is a small static cache), 16-byte aligned.  head_dim 64
+ * or 128; any page_size >= 1. */
+typedef struct {
+  void* k;
+  void* v;
+  int n_pages, page_size, n_kv, head_dim;
+} emx_paged_kv;
+
+/* A batch over such a cache; all three arrays int32 on the device.  Sequence i
+ * has rows [indptr[i], indptr[i+1]) of the batch (none: an idle slot, whose
+ * length and table are not read) and they are its last ones: row j of c
+ * stands at position lengths[i] - c + j.  Position p is in page
+ * table[i * max_pages + p / page_size], at row p % page_size of it.
+ * indptr[0] >= 0, ascending; rows from indptr[n_seqs] to n_rows belong to
+ * nobody and what would be written for them stays as it was.  n_seqs <= 1024.
+ * A sequence whose rows or length cannot be (rows outside [0, n_rows), fewer
+ * positions than rows) reports EMX_DEV_BAD_BATCH, one longer than its table
+ * EMX_DEV_KV_OVERFLOW, a page outside [0, n_pages) EMX_DEV_BAD_PAGE; nothing
+ * outside the named buffers is touched then. */
+typedef struct {
+  int n_seqs, n_rows, max_pages;
+  const int32_t* indptr;  /* [n_seqs + 1] */
+  const int32_t* lengths; /* [n_seqs], new rows included */
+  const int32_t* table;   /* [n_seqs, max_pages] */
+} emx_paged_batch;
+
+/* rms_norm of q and k per head, rope of both to their rows' positions, and the
+ * slice_update of k and v, for all rows of a batch in one pass: qkv
+ * bf16[n_rows, (n_q + 2 n_kv) * head_dim] as q | k | v; q_norm / k_norm
+ * bf16[head_dim] or null (no norm); rope_theta 0: no rotation.  q_out
+ * bf16[n_rows, n_q, head_dim] (not overlapping qkv); k and v go to their
+ * pages.  fp32 throughout (angles as exact as fp64 gives them, at any
+ * position), rounded to bf16 once.  Positions of one batch must be in
+ * different cache rows.  A row of a sequence not in order is skipped; one
+ * whose page is outside the cache gets its q only. */
+int emx_paged_append(emx_ctx* ctx, const void* qkv, const void* q_norm, const void* k_norm, float eps, float rope_theta,
+                     int n_q, const emx_paged_kv* kv, const emx_paged_batch* batch, void* q_out);
+/* Bytes of workspace that emx_sdpa_paged needs for batches of at most this
+ * n_rows over this cache (lengths, indptr and tables are not looked at; k, v
+ * and the arrays may be null). */
+int emx_sdpa_paged_workspace(emx_ctx* ctx, const emx_paged_kv* kv, const emx_paged_batch* batch, int n_q, int shared_len,
+                             size_t* bytes);
+/* Attention of a batch's rows over the paged cache: q bf16[n_rows, n_q,
+ * head_dim], the row at position p attends positions 0..p of its sequence;
+ * out likewise.  The first shared_len positions of every sequence with rows
+ * are the pages shared_pages[shared_len / page_size] (device): they are read
+ * once for the whole batch, and the tables' entries for them are not read.
+ * shared_len: whole pages, 0 for none; a sequence with rows has at least
+ * shared_len + its rows positions.  Rows of a sequence not in order become
+ * zeros, as do rows that see no page inside the cache (such a page's positions
+ * are left out).  The workspace (256-byte aligned) belongs to this call until
+ * it has run: calls that can overlap, or graphs that do, take one each. */
+int emx_sdpa_paged(emx_ctx* ctx, const void* q, const emx_paged_kv* kv, const emx_paged_batch* batch, int n_q, float scale,
+                   int shared_len, const int32_t* shared_pages, void* out, void* workspace, size_t workspace_bytes);
+/* Speculative sampling's acceptance for a batch of sequences, from given
+ * uniform numbers in [0, 1): target [n_seqs, n_draft + 1, vocab] and draft
+ * [n_seqs, n_draft, vocab] probabilities (dtype EMX_F32 or EMX_BF16; draft
+ * null: every draft was certain), tokens int32[n_seqs, n_draft], counts
+ * int32[n_seqs] drafts of each sequence (null: n_draft; more count as
+ * n_draft), uniforms f32[n_seqs, n_draft + 1].  Draft j is accepted while
+ * u_j q_j(x_j) < p_j(x_j); then one more token is drawn with the last uniform
+ * (index n_draft): from max(p - q, 0) of the first refused draft's row (p
+ * itself where that has no mass), or from the row behind the last draft — the
+ * first index whose running sum exceeds u times the total.  out int32[n_seqs,
+ * n_draft + 1]: the accepted drafts, that token, then -1; accepted
+ * int32[n_seqs]: how many drafts.  Comparisons and sums are in fp64; the rows
+ * need not sum to 1, and entries that are negative or not finite carry no
+ * mass.  No mass at all: -1 in the token's place.  counts[i] < 0: an empty
+ * slot, all -1 and 0 accepted.  A draft outside [0, vocab) is refused
+ * and reports EMX_DEV_BAD_TOKEN. */
+int emx_verify_draft(emx_ctx* ctx, const void* target, const void* draft, emx_dtype dtype, const int32_t* tokens,
+                     const int32_t* counts, const float* uniforms, int n_seqs, int n_draft, int vocab, int32_t* out,
+                     int32_t* accepted);
 
 /* ------------------------------------------------------------ collectives */
 typedef struct emx_comm emx_comm;

@@ -1,0 +1,363 @@
+"""emx_paged_append and emx_sdpa_paged against their definitions in 64 bits, on an sm_100 GPU.  Rows of the cache that
+belong to no position, and pages that belong to nobody, hold NaN throughout."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import emx
+from paged_case import NAN, Case
+
+pytestmark = pytest.mark.gpu
+
+H = 2.0 ** -8  # half a step of bf16, relative
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = emx.Ctx(0)
+    yield c
+    c.close()
+
+
+def stream_of(ctx):
+    p = C.c_void_p()
+    assert emx.lib().emx_ctx_stream(ctx.h, C.byref(p)) == 0
+    return p.value
+
+
+def attend(ctx, c, fill=NAN, ws=None):
+    out = ctx.put(np.full((c.n_rows + 1, c.n_q, c.hd), fill, np.uint16))
+    ctx.sdpa_paged(c.dq, c.kv, c.batch, c.n_q, c.scale, c.shared, c.d_shared, out=out, workspace=ws)
+    c.status = ctx.device_status()  # read and cleared: a copy to the host would raise it
+    return out.read(np.uint16, (c.n_rows + 1, c.n_q, c.hd))
+
+
+def check_attend(c, got, fill=NAN):
+    """Bound: the output's rounding, H |o|; the weights' rounding to bf16, which moves o by at most H sum w |v - o| <=
+    H (mean |v| + |o|); and the scores' fp32 products and exponentials, whose errors (128 terms of 2^-24, a 2-ulp
+    exponential) stay below 2^-12 of a weight each: 2^-11 (mean |v| + |o|)."""
+    want, size = c.attend()
+    g = emx.f32(got[:c.n]).astype(np.float64)
+    tol = H * np.abs(want) + (H + 2.0 ** -11) * (size + np.abs(want))
+    bad = ~(np.abs(g - want) <= tol)
+    assert not bad.any(), (int(bad.sum()), float(np.nanmax(np.abs(g - want) / tol)), np.argwhere(bad)[:4].tolist())
+    assert (got[c.n:] == fill).all()  # rows behind the last sequence
+
+
+HEADS = [(4, 2), (8, 8), (16, 2), (5, 1), (32, 1)]
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("n_q,n_kv", HEADS)
+@pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 131])
+def test_one_sequence_one_row(ctx, length, n_q, n_kv, hd):
+    c = Case(length, [1], [length], n_q, n_kv, hd).device(ctx)
+    check_attend(c, attend(ctx, c))
+    assert c.status == 0
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("page", [1, 7, 16, 24, 64, 100])
+@pytest.mark.parametrize("pages_shared", [0, 1, 3])
+def test_pages_of_any_size(ctx, page, pages_shared, hd):
+    shared = page * pages_shared
+    rows = [1, 3, 0, 1, 2]
+    c = Case(page, rows, [shared + t for t in (1, 3, 0, 200, 77)], 4, 2, hd, page, shared, pad=2).device(ctx)
+    check_attend(c, attend(ctx, c))
+    assert c.status == 0
+
+
+@pytest.mark.parametrize("n_q,n_kv", HEADS)
+@pytest.mark.parametrize("rows", [1, 2, 5, 16, 33, 130])
+def test_several_rows_see_no_later_ones(ctx, rows, n_q, n_kv):
+    c = Case(rows, [rows, 0, rows, 1], [rows, 0, rows + 61, 150], n_q, n_kv, pad=1).device(ctx)
+    check_attend(c, attend(ctx, c))
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("n_q,n_kv", HEADS)
+@pytest.mark.parametrize("seqs,shared", [(1, 128), (3, 48), (9, 512), (40, 272), (140, 1040), (300, 144)])
+def test_a_shared_prefix(ctx, seqs, shared, n_q, n_kv, hd):
+    r = np.random.default_rng(seqs)
+    rows = r.choice([0, 1, 1, 1, 3], seqs)
+    rows[0] = 1
+    c = Case(seqs, rows, shared + rows + r.integers(0, 60, seqs), n_q, n_kv, hd, 16, shared, pad=3).device(ctx)
+    check_attend(c, attend(ctx, c))
+    assert c.status == 0
+
+
+def test_long_and_short_together(ctx):
+    lens = [9000, 1, 17, 5000, 64, 1, 3, 700]
+    c = Case(5, [1, 1, 2, 1, 8, 1, 3, 1], lens, 8, 2, page=32).device(ctx)
+    check_attend(c, attend(ctx, c))
+
+
+def test_a_long_prefix_and_far_pages(ctx):
+    c = Case(6, [1] * 20, [6000 + 64 + i for i in range(20)], 8, 2, page=48, shared=6000, spare=50).device(ctx)
+    check_attend(c, attend(ctx, c))
+
+
+def test_all_slots_idle(ctx):
+    c = Case(7, [0, 0, 0], [0, 5, 0], pad=4).device(ctx)
+    got = attend(ctx, c, fill=7)
+    assert (got == 7).all() and c.status == 0
+
+
+def test_what_a_row_does_not_see_may_be_anything(ctx):
+    """NaN and infinities in the K and V of later rows leave earlier rows as they are, and reach the rows that see
+    them; a row of q that is NaN spoils no other."""
+    c = Case(8, [6, 2, 1], [70, 40, 30], 4, 2)
+    at = c.table[0, 67 // 16], 67 % 16
+    for x, bad in ((c.v, 0x7F80), (c.k, 0x7FC0)):
+        d = Case(8, [6, 2, 1], [70, 40, 30], 4, 2)
+        (d.v if x is c.v else d.k)[at[0], :, at[1], 3] = bad  # seen by rows 3, 4, 5 (positions 67, 68, 69)
+        d.device(ctx)
+        got = attend(ctx, d)
+        g = emx.f32(got[:d.n])
+        assert not np.isfinite(g[3:6, :, 3]).any()
+        want, size = c.attend()
+        ok = [0, 1, 2, 6, 7, 8]
+        assert (np.abs(g[ok] - want[ok]) <= (2 * H + 2.0 ** -11) * (size[ok] + np.abs(want[ok]))).all()
+        if x is c.v:  # only that dimension
+            rest = np.delete(np.arange(128), 3)
+            assert np.isfinite(g[3:6][..., rest]).all()
+    d = Case(8, [6, 2, 1], [70, 40, 30], 4, 2)
+    d.q[1, 2] = NAN
+    g = emx.f32(attend(ctx, d.device(ctx))[:d.n])
+    assert np.isnan(g[1, 2]).all() and np.isnan(g).sum() == 128
+
+
+def test_scores_of_any_size(ctx):
+    """Huge scores (weights of 0 and 1), and a maximum that keeps moving."""
+    c = Case(9, [2, 1], [300, 160], 4, 2, shared=0)
+    k = emx.f32(c.k)
+    c.k = emx.bf16(k * 60)
+    c.q = emx.bf16(emx.f32(c.q) * 30)
+    c.device(ctx)
+    want, size = c.attend()
+    g = emx.f32(attend(ctx, c)[:c.n]).astype(np.float64)
+    # scores of ~2e4 carry fp32 errors of 128 * 2^-24 * sum |q k| scale ~ 0.25 in the exponent at the worst; the two
+    # largest scores of a row are farther apart than 20 here for nearly all rows, so most rows equal one row of V
+    s = np.abs(g - want)
+    assert np.isfinite(g).all() and np.median(s) <= 2 * H * np.median(size) and (s <= 2 * size.max()).all()
+
+
+def test_bad_pages_are_left_out_and_reported(ctx):
+    c = Case(10, [1, 2], [100, 50], 4, 2)
+    c.table[0, 2] = c.n_pages  # positions 32..47
+    c.table[1, 1] = -1  # positions 16..31
+    c.device(ctx)
+    g = emx.f32(attend(ctx, c)[:c.n]).astype(np.float64)
+    assert c.status == 5
+    for i, hole in ((0, range(32, 48)), (1, range(16, 32))):
+        keep = np.array([p for p in range(c.lens[i]) if p not in hole])
+        k, v = (emx.f32(x[c.table[i, keep // 16], :, keep % 16]).astype(np.float64) for x in (c.k, c.v))
+        for j, p in enumerate(c.positions(i)):
+            row, m = c.indptr[i] + j, keep <= p
+            q = emx.f32(c.q[row]).astype(np.float64).reshape(2, 2, 128)
+            w = np.exp(np.einsum("hgd,shd->hgs", q, k[m]) * c.scale)
+            w /= w.sum(-1, keepdims=True)
+            want = np.einsum("hgs,shd->hgd", w, v[m]).reshape(4, 128)
+            size = np.einsum("hgs,shd->hgd", w, np.abs(v[m])).reshape(4, 128)
+            assert (np.abs(g[row] - want) <= (2 * H + 2.0 ** -11) * (size + np.abs(want))).all()
+    # no page at all: zeros
+    c = Case(11, [1, 1], [30, 30], 4, 2)
+    c.table[1] = 1 << 30
+    g = attend(ctx, c.device(ctx))
+    assert (g[1] == 0).all() and (g[0] != 0).any() and c.status == 5
+
+
+@pytest.mark.parametrize("shared", [0, 32])
+def test_sequences_out_of_order_give_zeros_and_a_status(ctx, shared):
+    c = Case(12, [1, 3, 1, 2], [shared + 40, shared + 60, shared + 50, shared + 8], 4, 2, shared=shared).device(ctx)
+    c.d_lens.write(np.array([shared + 40, shared + 2, shared + 50, c.max_pages * 16 + 1], np.int32))
+    got = attend(ctx, c)
+    assert c.status in (4, 6)
+    assert (got[1:4] == 0).all() and (got[5:7] == 0).all()
+    want, size = c.attend()
+    g = emx.f32(got[:c.n])
+    for r in (0, 4):
+        assert (np.abs(g[r] - want[r]) <= (2 * H + 2.0 ** -11) * (size[r] + np.abs(want[r]))).all()
+    # rows that cannot be
+    for bad in ([0, 9, 5, 6, 7], [-2, 1, 2, 3, 4], [0, 1, 4, 5, 100]):
+        c.d_indptr.write(np.array(bad, np.int32))
+        attend(ctx, c)
+        assert c.status in (4, 6)
+    c.d_indptr.write(c.indptr)
+    c.d_lens.write(np.array(c.lens, np.int32))
+    check_attend(c, attend(ctx, c))
+    assert c.status == 0
+
+
+def test_the_same_call_gives_the_same_bits(ctx):
+    c = Case(13, [1, 2, 1, 1] * 8, [400 + 13 * i for i in range(32)], 8, 2, shared=256).device(ctx)
+    first = attend(ctx, c)
+    for _ in range(3):
+        assert (attend(ctx, c) == first).all()
+
+
+def test_one_sequence_equals_the_static_cache(ctx):
+    """The same rows through emx_sdpa_decode."""
+    c = Case(14, [1], [333], 16, 8).device(ctx)
+    k, v = (np.ascontiguousarray(x[c.table[0, np.arange(333) // 16], :, np.arange(333) % 16].transpose(1, 0, 2)) for x in (c.k, c.v))
+    ref = emx.f32(ctx.sdpa_decode(c.dq, ctx.put(k), ctx.put(v), 16, 8, 333, 128, 333, c.scale).read(np.uint16, (16, 128)))
+    g = emx.f32(attend(ctx, c)[0])
+    _, size = c.attend()
+    assert (np.abs(g - ref) <= 4 * H * (size[0] + np.abs(ref))).all()
+
+
+def test_workspace_is_checked_and_not_overrun(ctx):
+    c = Case(15, [1, 4, 1], [300, 200, 40], 8, 2, shared=32).device(ctx)
+    need = ctx.sdpa_paged_workspace(c.kv, c.batch, 8, 32)
+    ws = ctx.put(np.full(need + 4096, 0xA5, np.uint8))
+    whole = ws.nbytes
+    ws.nbytes = need - 1
+    with pytest.raises(emx.EmxError, match="workspace"):
+        attend(ctx, c, ws=ws)
+    ws.nbytes = need
+    check_attend(c, attend(ctx, c, ws=ws))
+    ws.nbytes = whole
+    assert (ws.read(np.uint8, whole)[need:] == 0xA5).all()
+
+
+def test_captured_and_replayed_as_the_batch_changes(ctx):
+    """One graph of append and attention, replayed with other lengths, rows and tables; a second one with a workspace of
+    its own runs at the same time on another stream."""
+    torch = pytest.importorskip("torch")
+    other = emx.Ctx(0)
+    a = Case(16, [1, 1, 2, 1], [100, 37, 90, 64], 8, 2, shared=32).device(ctx)
+    e = Case(18, [1] * 6, [900 + i for i in range(6)], 8, 2, shared=64).device(other)
+    graphs = []
+    for cx, c in ((ctx, a), (other, e)):
+        out = cx.put(np.zeros((c.n_rows, 8, 128), np.uint16))
+        ws = cx.alloc(cx.sdpa_paged_workspace(c.kv, c.batch, 8, c.shared))
+        cx.sdpa_paged(c.dq, c.kv, c.batch, 8, c.scale, c.shared, c.d_shared, out=out, workspace=ws)
+        cx.synchronize()
+        st, g = torch.cuda.ExternalStream(stream_of(cx)), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st, capture_error_mode="thread_local"):
+            cx.sdpa_paged(c.dq, c.kv, c.batch, 8, c.scale, c.shared, c.d_shared, out=out, workspace=ws)
+        graphs.append((g, st, out))
+
+    def replay():
+        for _ in range(5):
+            for g, st, _ in graphs:
+                with torch.cuda.stream(st):
+                    g.replay()
+        torch.cuda.synchronize()
+
+    replay()
+    check_attend(a, graphs[0][2].read(np.uint16, (a.n_rows, 8, 128)))
+    check_attend(e, graphs[1][2].read(np.uint16, (6, 8, 128)))
+    # lengths shorter by some positions, rows moved between sequences
+    a.lens, a.rows = [70, 36, 33, 64], [2, 1, 1, 1]
+    a.indptr = np.concatenate([[0], np.cumsum(a.rows)]).astype(np.int32)
+    a.d_lens.write(np.array(a.lens, np.int32))
+    a.d_indptr.write(a.indptr)
+    ctx.synchronize()
+    replay()
+    check_attend(a, graphs[0][2].read(np.uint16, (a.n_rows, 8, 128)))
+    del graphs
+    other.close()
+
+
+# ------------------------------------------------------------------------------------------------------------ append
+def check_append(ctx, c, norm=True, theta=1e6, eps=1e-6):
+    r = c.rng
+    wq, wk = (emx.bf16(1 + 0.2 * r.normal(size=c.hd)) if norm else None for _ in range(2))
+    out = ctx.put(np.full((c.n_rows + 1, c.n_q, c.hd), NAN, np.uint16))
+    ctx.paged_append(c.dqkv, c.kv, c.batch, c.n_q, None if wq is None else ctx.put(wq), None if wk is None else ctx.put(wk),
+                     eps, theta, out=out)
+    got = out.read(np.uint16, (c.n_rows + 1, c.n_q, c.hd))
+    k, v = (x.read(np.uint16, c.k.shape) for x in (c.dk, c.dv))
+    q_, k_, v_ = c.append(wq, wk, eps, theta)
+    half = c.hd // 2
+
+    def near(g, want):
+        # one rounding to bf16, and fp32 steps (a mean of squares, a root, two products) of the pair that is rotated:
+        # 16 of them at 2^-24 of its length
+        pair = np.sqrt(want[..., :half] ** 2 + want[..., half:] ** 2)
+        tol = H * np.abs(want) + 2.0 ** -20 * np.concatenate([pair, pair], -1)
+        err = np.abs(emx.f32(g).astype(np.float64) - want)
+        assert (err <= tol).all(), float((err / np.maximum(tol, 1e-30)).max())
+
+    near(got[:c.n], q_)
+    assert (got[c.n:] == NAN).all()
+    wk_, wv_ = c.k.copy(), c.v.copy()
+    for i in range(c.n_seqs):
+        p = c.positions(i)
+        at = c.table[i, p // c.page], slice(None), p % c.page
+        rows = slice(c.indptr[i], c.indptr[i + 1])
+        if c.rows[i]:
+            near(k[at], k_[rows])
+            assert (emx.f32(v[at]) == v_[rows]).all()
+            wk_[at], wv_[at] = k[at], v[at]
+    assert (k == wk_).all() and (v == wv_).all()  # and nothing else was written
+    return got
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("n_q,n_kv", HEADS + [(64, 8)])
+@pytest.mark.parametrize("rows", [[1], [1] * 70, [3, 0, 17, 1, 40], [300]])
+def test_append(ctx, rows, n_q, n_kv, hd):
+    r = np.random.default_rng(len(rows))
+    c = Case(len(rows), rows, [k + int(r.integers(0, 200)) for k in rows], n_q, n_kv, hd, pad=3).device(ctx)
+    check_append(ctx, c)
+    assert ctx.device_status() == 0
+
+
+@pytest.mark.parametrize("norm,theta", [(False, 1e6), (True, 0.0), (False, 0.0), (True, 1e4)])
+def test_append_without_norm_or_rotation(ctx, norm, theta):
+    check_append(ctx, Case(21, [2, 1, 5], [20, 1, 300], 8, 2, page=24).device(ctx), norm, theta)
+
+
+def test_append_far_positions(ctx):
+    """Angles of a million radians: the pages of the last positions alone are there."""
+    c = Case(22, [1, 2], [5, 9], 4, 2)
+    far = 1_000_003
+    c.max_pages = far // 16 + 1
+    c.lens = [far, far - 700]
+    table = np.full((2, c.max_pages), -1, np.int32)
+    for i, (n, t) in enumerate(zip(c.rows, c.lens)):
+        for p in range(t - n, t):
+            table[i, p // 16] = i
+    c.table = table
+    c.device(ctx)
+    check_append(ctx, c)
+    assert ctx.device_status() == 0
+
+
+def test_append_many_rows(ctx):
+    """More rows than the grid has warps."""
+    c = Case(23, [9000, 1, 2500], [9000, 50, 2600], 3, 1, 64, 32).device(ctx)
+    check_append(ctx, c)
+
+
+def test_append_skips_what_is_out_of_order(ctx):
+    c = Case(24, [1, 2, 1, 1], [10, 20, 30, 31], 4, 2)
+    c.table[2, 1] = c.n_pages + 3
+    c.device(ctx)
+    c.d_lens.write(np.array([10, 1, 30, c.max_pages * 16 + 1], np.int32))
+    out = ctx.put(np.full((c.n_rows, 4, 128), NAN, np.uint16))
+    ctx.paged_append(c.dqkv, c.kv, c.batch, 4, out=out)
+    assert ctx.device_status() in (4, 5, 6)
+    got = out.read(np.uint16, (c.n_rows, 4, 128))
+    q_, k_, v_ = c.append()
+    for r in (0, 3):  # rows of sequences 0 and 2: q is there
+        assert np.allclose(emx.f32(got[r]), q_[r], rtol=H, atol=1e-4)
+    assert (got[1:3] == NAN).all() and (got[4] == NAN).all()
+    k, v = (x.read(np.uint16, c.k.shape) for x in (c.dk, c.dv))
+    wv = c.v.copy()
+    p = c.positions(0)
+    wv[c.table[0, p // 16], :, p % 16] = v[c.table[0, p // 16], :, p % 16]
+    assert (v == wv).all()  # sequence 0's row alone was written
+    assert np.allclose(emx.f32(k[c.table[0, p // 16], :, p % 16]), k_[:1], rtol=H, atol=1e-4)
+
+
+def test_append_norm_of_large_and_zero_heads(ctx):
+    c = Case(25, [2, 1], [40, 9], 4, 2)
+    x = c.qkv.reshape(c.n_rows, 8, 128)
+    x[0, 0] = 0  # a head of zeros: eps keeps it
+    x[1, 1] = emx.bf16(np.full(128, 1e18, np.float32))  # squares near fp32's end
+    x[1, 4] = emx.bf16(np.full(128, 1e-18, np.float32))
+    check_append(ctx, c.device(ctx))
