@@ -17,7 +17,7 @@
 // tiles go to the piece slot of its rows, a share that begins inside a segment
 // to the slot of its worker; a second kernel joins the pieces of each row
 // (and a segment that one worker has whole is written by it).
-#include "paged_dev.cuh"
+#include "paged_attn.cuh"
 
 namespace emx {
 
@@ -28,7 +28,6 @@ constexpr int kWarps = 4;     // workers of a CTA
 constexpr int kStages = 3;    // tiles in flight a worker
 constexpr int kMaxSeqs = 1024;
 constexpr int kCtasPerSm = 2;
-constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;  // 0: the 16 bytes become zeros, nothing is read
@@ -49,22 +48,6 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
-
-// Pieces of one part (own or shared): first[] by row and q head, more[] by worker.
-struct Pieces {
-  float* first_o;    // [n_rows * n_q][HD]
-  float2* first_ml;  // [n_rows * n_q]
-  float* more_o;     // [workers][rows of a tile][HD]
-  float2* more_ml;   // [workers][rows of a tile]
-};
-
-struct Work {
-  PagedAttnArgs a;
-  Pieces own, shared;
-  int64_t* starts;  // [n_seqs + 1] tiles before each sequence (own part)
-  int own_workers, shared_workers;
-  int own_mt, shared_mt;  // rows of a tile
-};
 
 // starts[0..n_seqs] of all sequences into shared memory, by the whole CTA.
 template <int THREADS>
@@ -111,7 +94,7 @@ struct Worker {
   static constexpr int kChunks = HD / 8;           // 16-byte chunks of a row
   static constexpr int kCopies = kKT * kChunks / 32;
 
-  const Work& w;
+  const PagedWork& w;
   Line line;
   int lane;
   uint32_t ring;       // this warp's stages
@@ -153,17 +136,17 @@ struct Worker {
     }
   }
 
-  __device__ __forceinline__ void run(int64_t total, int worker, int workers) const;
+  __device__ __forceinline__ void run(int64_t total, int worker, int64_t per) const;
 };
 
-// The share of `worker` of `workers` in the line's `total` tiles.
+// The share of `worker`, `per` tiles of the line's `total`.
 template <int HD, int NT, bool SHARED>
-__device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int64_t total, int worker, int workers) const {
+__device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int64_t total, int worker, int64_t per) const {
   const PagedAttnArgs& a = w.a;
   const Pieces& pc = SHARED ? w.shared : w.own;
-  const int64_t x0 = share_begin(total, worker, workers), x1 = share_begin(total, worker + 1, workers);
-  const int n = (int)(x1 - x0);
-  if (n <= 0) return;
+  const int64_t x0 = worker * per;
+  if (x0 >= total) return;
+  const int n = (int)min(per, total - x0);
   Cursor ld, cc;
   const int hpg = line.hpg;
   cc.seek(line, x0);
@@ -399,7 +382,7 @@ __device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int64_t total, int w
 }
 
 template <int HD, int NT, bool SHARED>
-__global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const __grid_constant__ Work w) {
+__global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const __grid_constant__ PagedWork w) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int64_t starts[SHARED ? 1 : kMaxSeqs + 1];
   __shared__ uint32_t valid[kWarps][kStages];
@@ -418,12 +401,12 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const __grid_co
   pdl_trigger();
   if (total == 0) return;
   Wk k{w, line, (int)(threadIdx.x & 31), smem_u32(smem) + warp * (uint32_t)(kStages * Wk::kStageB), valid[warp]};
-  k.run(total, blockIdx.x * kWarps + warp, gridDim.x * kWarps);
+  k.run(total, blockIdx.x * kWarps + warp, share_size(total, gridDim.x * kWarps, 1));
 }
 
 // One warp a (row, q head): joins its pieces.
 template <int HD>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ Work w) {
+__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedWork w) {
   const PagedAttnArgs& a = w.a;
   const int lane = threadIdx.x & 31;
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -436,47 +419,83 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   const SeqInfo s = load_seq(a.p, i, a.shared_len);
   constexpr int E = HD / 32;
   bf16* dst = a.out + (size_t)item * HD + lane * E;
+  // the row's pieces: first slots, then the workers' slots of both parts
+  const float* src_o[2][2] = {};
+  const float2* src_ml[2][2] = {};
+  int more[2] = {0, 0}, step[2] = {0, 0}, parts = 0;
+  auto part = [&](const Pieces& pc, const Line& line, const SeqInfo& s, int workers, int64_t T, int64_t x0, int r, int x) {
+    const int kt = line.key_tiles(s);
+    x0 += ((int64_t)h * line.row_tiles(s) + r / line.mt) * kt;
+    const int64_t per = share_size(T, workers, 1);
+    const int c0 = (int)(x0 / per), c1 = (int)((x0 + kt - 1) / per);
+    const size_t slot = (size_t)(c0 + 1) * line.mt + r % line.mt;
+    src_o[x][0] = pc.first_o + item * HD;
+    src_ml[x][0] = pc.first_ml + item;
+    src_o[x][1] = pc.more_o + slot * HD;
+    src_ml[x][1] = pc.more_ml + slot;
+    more[x] = c1 - c0;
+    step[x] = line.mt;
+  };
+  if (s.ok) {
+    const int g = hq - h * hpg;
+    const Line own = make_line(a.p, a.shared_len, true, w.own_mt, w.own_keys, w.starts);
+    part(w.own, own, s, w.own_workers, w.starts[a.p.n_seqs], w.starts[i], (row - s.row0) * hpg + g, 0);
+    parts = 1;
+    if (a.shared_len > 0) {
+      const Line all = make_line(a.p, a.shared_len, false, w.shared_mt, w.shared_keys, nullptr);
+      part(w.shared, all, all.seq(0), w.shared_workers, all.tiles(all.seq(0)), 0, row * hpg + g, 1);
+      parts = 2;
+    } else if (more[0] == 0) {
+      return;  // one worker had the segment whole and wrote it
+    }
+  }
+  // piece x of the row: maxima and sums of 32 pieces in the lanes, then their O
+  const int n0 = parts > 0 ? 1 + more[0] : 0, n = n0 + (parts > 1 ? 1 + more[1] : 0);
   float o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
   float m = -INFINITY, l = 0.f;
-  auto take = [&](const float* src, float2 ml) {
-    float v[E];
-    if constexpr (E == 4) {
-      const float4 f = *reinterpret_cast<const float4*>(src + lane * E);
-      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-    } else {
-      const float2 f = *reinterpret_cast<const float2*>(src + lane * E);
-      v[0] = f.x, v[1] = f.y;
+  auto o_of = [&](int x) {
+    const int b = x >= n0, y = x - (b ? n0 : 0);
+    return y == 0 ? src_o[b][0] : src_o[b][1] + (size_t)(y - 1) * step[b] * HD;
+  };
+  for (int x0 = 0; x0 < n; x0 += 32) {
+    const int x = x0 + lane;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (x < n) {
+      const int b = x >= n0, y = x - (b ? n0 : 0);
+      ml = y == 0 ? *src_ml[b][0] : src_ml[b][1][(size_t)(y - 1) * step[b]];
     }
-    const float to = fmaxf(m, ml.x), base = to == -INFINITY ? 0.f : to;
-    const float x = ex2f(m - base), y = ex2f(ml.x - base);
-    l = l * x + ml.y * y;
+    // a NaN among the sums stays one, whatever its maximum
+    const float to = fmaxf(m, warp_max(ml.x)), base = to == -INFINITY ? 0.f : to;
+    const float was = ex2f(m - base), wx = ex2f(ml.x - base);
+    l = l * was + warp_sum(ml.y * wx);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * x + v[e] * y;
+    for (int e = 0; e < E; ++e) o[e] *= was;
     m = to;
-  };
-  // the pieces of row r (of its sequence) in one part; x0: the tiles before the sequence, T all
-  auto part = [&](const Pieces& pc, const Line& line, const SeqInfo& s, int workers, int64_t T, int64_t x0, int r) {
-    const int kt = line.key_tiles(s);
-    x0 += ((int64_t)h * line.row_tiles(s) + r / line.mt) * kt;
-    const int c0 = share_of(T, x0, workers), c1 = share_of(T, x0 + kt - 1, workers);
-    if (c0 == c1 && a.shared_len == 0) return false;  // one worker had the segment whole and wrote it
-    take(pc.first_o + item * HD, pc.first_ml[item]);
-    for (int c = c0 + 1; c <= c1; ++c) {
-      if (share_begin(T, c, workers) == share_begin(T, c + 1, workers)) continue;
-      const size_t slot = (size_t)c * line.mt + r % line.mt;
-      take(pc.more_o + slot * HD, pc.more_ml[slot]);
-    }
-    return true;
-  };
-  if (s.ok) {
-    const int g = hq - h * hpg;
-    const Line own = make_line(a.p, a.shared_len, true, w.own_mt, kKT, w.starts);
-    if (!part(w.own, own, s, w.own_workers, w.starts[a.p.n_seqs], w.starts[i], (row - s.row0) * hpg + g)) return;
-    if (a.shared_len > 0) {
-      const Line all = make_line(a.p, a.shared_len, false, w.shared_mt, kKT, nullptr);
-      part(w.shared, all, all.seq(0), w.shared_workers, all.tiles(all.seq(0)), 0, row * hpg + g);
+    const int many = min(32, n - x0);
+    constexpr int U = 8;  // pieces in flight
+    for (int y = 0; y < many; y += U) {
+      float v[U][E];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool on = y + u < many;
+        const float* p = o_of(x0 + (on ? y + u : 0)) + lane * E;
+        if constexpr (E == 4) {
+          const float4 f = on ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
+        } else {
+          const float2 f = on ? *reinterpret_cast<const float2*>(p) : make_float2(0.f, 0.f);
+          v[u][0] = f.x, v[u][1] = f.y;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float wu = __shfl_sync(0xffffffffu, wx, (y + u) & 31);
+        if (y + u < many)
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] = fmaf(v[u][e], wu, o[e]);
+      }
     }
   }
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
@@ -493,7 +512,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // The workspace's parts; returns its size (base may be null).
-size_t lay_out(Work& w, int num_sms, unsigned char* base) {
+size_t lay_out(PagedWork& w, int num_sms, unsigned char* base) {
   const PagedArgs& p = w.a.p;
   const size_t heads = (size_t)p.n_rows * p.n_q;
   size_t off = 0;
@@ -504,19 +523,20 @@ size_t lay_out(Work& w, int num_sms, unsigned char* base) {
   };
   w.starts = static_cast<int64_t*>(take(sizeof(int64_t) * (kMaxSeqs + 1)));
   w.own_workers = w.shared_workers = num_sms * kCtasPerSm * kWarps;
-  auto pieces = [&](Pieces& pc) {
+  auto pieces = [&](Pieces& pc, size_t rows) {
     pc.first_o = static_cast<float*>(take(heads * p.head_dim * sizeof(float)));
     pc.first_ml = static_cast<float2*>(take(heads * sizeof(float2)));
-    pc.more_o = static_cast<float*>(take((size_t)w.own_workers * 32 * p.head_dim * sizeof(float)));
-    pc.more_ml = static_cast<float2*>(take((size_t)w.own_workers * 32 * sizeof(float2)));
+    pc.more_o = static_cast<float*>(take(rows * p.head_dim * sizeof(float)));
+    pc.more_ml = static_cast<float2*>(take(rows * sizeof(float2)));
   };
-  pieces(w.own);
-  if (w.a.shared_len > 0) pieces(w.shared);
+  const size_t warps = (size_t)w.own_workers * 32, ctas = (size_t)num_sms * kTcRows;
+  pieces(w.own, warps);
+  if (w.a.shared_len > 0) pieces(w.shared, warps > ctas ? warps : ctas);
   return off;
 }
 
 template <int HD, int NT, bool SHARED>
-cudaError_t launch_part(const Work& w, int workers, cudaStream_t st) {
+cudaError_t launch_part(const PagedWork& w, int workers, cudaStream_t st) {
   const int smem = kWarps * kStages * Worker<HD, NT, SHARED>::kStageB;
   static cudaError_t once = cudaFuncSetAttribute(paged_attn_kernel<HD, NT, SHARED>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -526,15 +546,24 @@ cudaError_t launch_part(const Work& w, int workers, cudaStream_t st) {
 }
 
 template <int HD>
-cudaError_t launch(Work& w, cudaStream_t st) {
+cudaError_t launch(PagedWork& w, int num_sms, cudaStream_t st) {
   const PagedArgs& p = w.a.p;
   const int hpg = p.n_q / p.n_kv;
   w.own_mt = (int64_t)p.n_rows * hpg > 16 * (int64_t)p.n_seqs ? 32 : 16;
-  w.shared_mt = (int64_t)p.n_rows * hpg > 16 ? 32 : 16;
+  w.own_keys = kKT;
   cudaError_t e = cudaSuccess;
   if (w.a.shared_len > 0) {
-    e = w.shared_mt == 32 ? launch_part<HD, 2, true>(w, w.shared_workers, st)
-                          : launch_part<HD, 1, true>(w, w.shared_workers, st);
+    if ((int64_t)p.n_rows * hpg > 32) {
+      w.shared_mt = kTcRows;
+      w.shared_keys = kTcKeys;
+      w.shared_workers = num_sms;
+      e = paged_shared_tc_launch(w, num_sms, st);
+    } else {
+      w.shared_mt = (int64_t)p.n_rows * hpg > 16 ? 32 : 16;
+      w.shared_keys = kKT;
+      e = w.shared_mt == 32 ? launch_part<HD, 2, true>(w, w.shared_workers, st)
+                            : launch_part<HD, 1, true>(w, w.shared_workers, st);
+    }
     if (e != cudaSuccess) return e;
   }
   e = w.own_mt == 32 ? launch_part<HD, 2, false>(w, w.own_workers, st)
@@ -550,13 +579,13 @@ cudaError_t launch(Work& w, cudaStream_t st) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<HD>, static_cast<const Work>(w));
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<HD>, static_cast<const PagedWork>(w));
 }
 
 }  // namespace
 
 size_t paged_attn_workspace(int n_rows, int n_q, int n_kv, int head_dim, int shared_len, int num_sms) {
-  Work w = {};
+  PagedWork w = {};
   w.a.p.n_rows = n_rows;
   w.a.p.n_q = n_q;
   w.a.p.n_kv = n_kv;
@@ -566,10 +595,10 @@ size_t paged_attn_workspace(int n_rows, int n_q, int n_kv, int head_dim, int sha
 }
 
 cudaError_t paged_attn_launch(const PagedAttnArgs& a, int num_sms, cudaStream_t st) {
-  Work w = {};
+  PagedWork w = {};
   w.a = a;
   lay_out(w, num_sms, static_cast<unsigned char*>(a.workspace));
-  return a.p.head_dim == 128 ? launch<128>(w, st) : launch<64>(w, st);
+  return a.p.head_dim == 128 ? launch<128>(w, num_sms, st) : launch<64>(w, num_sms, st);
 }
 
 }  // namespace emx

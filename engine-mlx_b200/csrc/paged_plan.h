@@ -51,11 +51,12 @@ EMX_HD uint32_t cache_row(int page, int n_kv, int h, int page_size, int off) {
 
 // Segments: (KV head, row tile) pairs of one sequence, row tiles innermost,
 // each of `kt` key tiles.  Tiles of sequence i are [start_i, start_{i+1}) of
-// the batch's T; worker c of G takes [c T / G, (c + 1) T / G).
-EMX_HD int64_t share_begin(int64_t T, int c, int G) { return T * c / G; }
-// The worker that has tile x: the largest c whose share begins at or before x
-// (shares may be empty when T < G, and an empty share is never the answer).
-EMX_HD int share_of(int64_t T, int64_t x, int G) { return (int)(((x + 1) * G - 1) / T); }
+// the batch's T; worker c takes [c per, (c + 1) per) of them, so no worker of
+// the first ceil(T / per) is without work and tile x is worker x / per's.
+EMX_HD int64_t share_size(int64_t T, int workers, int least) {
+  const int64_t per = (T + workers - 1) / workers;
+  return per > least ? per : least;
+}
 
 // The line of key tiles of one part of a batch's positions: the common prefix
 // [0, shared_len), as one sequence with every row of the batch, or (own) each

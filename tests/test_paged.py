@@ -104,7 +104,7 @@ using namespace emx;
 // Walks every worker's share of the line the way the kernel does.  seen[x] counts tile x = (segment, key tile) in line
 // order; pieces[segment] gets the pieces written (first, more); returns 0, or where an index left its range.
 extern "C" int walk(int own, int n_seqs, int n_rows, int n_kv, int hpg, int shared, int mt, int keys, long room,
-                    const int* indptr, const int* lengths, int64_t* starts, int workers, int* seen, long n_seen, int* pieces) {
+                    const int* indptr, const int* lengths, int64_t* starts, int workers, int least, int* seen, long n_seen, int* pieces) {
   Line line{own != 0, n_seqs, n_rows, n_kv, hpg, shared, mt, keys, room, indptr, lengths, starts};
   int64_t T = 0;
   if (own) {
@@ -115,9 +115,10 @@ extern "C" int walk(int own, int n_seqs, int n_rows, int n_kv, int hpg, int shar
   }
   if (T != n_seen) return 1;
   if (T == 0) return 0;
-  int64_t segs_before = 0;
+  const int64_t per = share_size(T, workers, least);
+  if ((T + per - 1) / per > workers) return 13;
   for (int c = 0; c < workers; ++c) {
-    const int64_t x0 = share_begin(T, c, workers), x1 = share_begin(T, c + 1, workers);
+    const int64_t x0 = c * per, x1 = x0 + per < T ? x0 + per : T;
     if (x1 <= x0) continue;
     Cursor cur;
     cur.seek(line, x0);
@@ -139,7 +140,7 @@ extern "C" int walk(int own, int n_seqs, int n_rows, int n_kv, int hpg, int shar
       if (cur.k + 1 == cur.kt || x + 1 == x1) {
         // what the join will look for: the worker of the segment's first tile has the first piece
         const int64_t s0 = before + (int64_t)cur.seg * cur.kt;
-        const int c0 = share_of(T, s0, workers), c1 = share_of(T, s0 + cur.kt - 1, workers);
+        const int c0 = (int)(s0 / per), c1 = (int)((s0 + cur.kt - 1) / per);
         if (whole ? c != c0 : !(c > c0 && c <= c1)) return 9;
         if (!whole && ++more > 1) return 10;  // one slot a worker
         pieces[x - cur.k + 0] += 1;           // counted at the segment's tile that the piece ends in
@@ -148,15 +149,11 @@ extern "C" int walk(int own, int n_seqs, int n_rows, int n_kv, int hpg, int shar
       if (x + 1 < x1) cur.next(line);
     }
   }
-  // every non-empty share inside a segment wrote exactly one piece of it
+  // every share that reaches into a segment wrote exactly one piece of it
   Cursor cur;
   cur.seek(line, 0);
   for (int64_t x = 0; x < T;) {
-    const int c0 = share_of(T, x, workers), c1 = share_of(T, x + cur.kt - 1, workers);
-    int want = 0;
-    for (int c = c0; c <= c1; ++c) want += share_begin(T, c + 1, workers) > share_begin(T, c, workers);
-    if (share_begin(T, c0, workers) > x || share_begin(T, c0 + 1, workers) <= x) return 11;
-    if (pieces[x] != want) return 12;
+    if (pieces[x] != (x + cur.kt - 1) / per - x / per + 1) return 12;
     x += cur.kt;
     if (x < T) for (int k = cur.kt; k > 0; --k) cur.next(line);
   }
@@ -174,9 +171,9 @@ def walk(tmp_path_factory):
                     str(src), "-o", str(lib)], check=True)
     f = C.CDLL(str(lib)).walk
     f.restype = C.c_int
-    f.argtypes = [C.c_int] * 8 + [C.c_long] + [C.c_void_p] * 3 + [C.c_int, C.c_void_p, C.c_long, C.c_void_p]
+    f.argtypes = [C.c_int] * 8 + [C.c_long] + [C.c_void_p] * 3 + [C.c_int, C.c_int, C.c_void_p, C.c_long, C.c_void_p]
 
-    def run(own, indptr, lengths, n_rows, n_kv, hpg, shared, mt, keys, room, workers):
+    def run(own, indptr, lengths, n_rows, n_kv, hpg, shared, mt, keys, room, workers, least=1):
         indptr, lengths = np.asarray(indptr, np.int32), np.asarray(lengths, np.int32)
         n = len(lengths)
         total = 0
@@ -191,7 +188,7 @@ def walk(tmp_path_factory):
         seen, pieces = np.zeros(total + 1, np.int32), np.zeros(total + 1, np.int32)
         starts = np.zeros(n + 1, np.int64)
         rc = f(own, n, n_rows, n_kv, hpg, shared, mt, keys, room, indptr.ctypes.data, lengths.ctypes.data, starts.ctypes.data,
-               workers, seen.ctypes.data, total, pieces.ctypes.data)
+               workers, least, seen.ctypes.data, total, pieces.ctypes.data)
         assert rc == 0, rc
         assert (seen[:total] == 1).all()
         return total
@@ -211,7 +208,7 @@ def test_every_tile_has_one_worker_and_every_piece_is_joined(walk, seed):
     for own in (0, 1):
         if own or (shared and indptr[-1]):
             walk(own, indptr, lens, int(indptr[-1]) + 3, n_kv, hpg, shared, int(r.choice([16, 32, 128])),
-                 int(r.choice([16, 64, 128])), 8192, int(r.choice([1, 7, 148, 1184])))
+                 int(r.choice([16, 64, 128])), 8192, int(r.choice([1, 7, 148, 1184])), int(r.choice([1, 4])))
 
 
 @pytest.mark.parametrize("seed", range(40))
