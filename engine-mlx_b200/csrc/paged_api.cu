@@ -42,8 +42,8 @@ int check_shape(const char* op, const emx_paged_kv* kv, const emx_paged_batch* b
              kv->n_kv);
   PG_REQUIRE(n_q <= 1024, "%s: n_q %d exceeds 1024", op, n_q);
   PG_REQUIRE(kv->n_pages >= 0 && kv->page_size >= 1, "%s: bad cache: %d pages of %d", op, kv->n_pages, kv->page_size);
-  // 32-bit row numbers; with 64-element rows their cache would be 512 GB
-  PG_REQUIRE((double)kv->n_pages * kv->n_kv * kv->page_size < 4294967295.0, "%s: cache of %d x %d x %d rows is too large", op,
+  // row numbers are int32 coordinates of a tensor map; with 64-element rows that cache would be 256 GB
+  PG_REQUIRE((double)kv->n_pages * kv->n_kv * kv->page_size < 2147483647.0, "%s: cache of %d x %d x %d rows is too large", op,
              kv->n_pages, kv->n_kv, kv->page_size);
   PG_REQUIRE(b->n_seqs >= 0 && b->n_seqs <= kMaxSeqs, "%s: n_seqs %d outside [0, %d]", op, b->n_seqs, kMaxSeqs);
   PG_REQUIRE(b->n_rows >= 0 && (int64_t)b->n_rows * n_q <= 0x7fffffff, "%s: n_rows %d is negative or too large for %d heads",

@@ -389,6 +389,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const __grid_co
   using Wk = Worker<HD, NT, SHARED>;
   const int warp = threadIdx.x >> 5;
   const Line line = make_line(w.a.p, w.a.shared_len, !SHARED, Wk::MT, kKT, starts);
+  pdl_trigger();
   int64_t total;
   if (SHARED) {
     total = line.tiles(line.seq(0));
@@ -398,10 +399,13 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const __grid_co
     if (blockIdx.x == 0)
       for (int i = threadIdx.x; i <= w.a.p.n_seqs; i += kWarps * 32) w.starts[i] = starts[i];
   }
-  pdl_trigger();
-  if (total == 0) return;
-  Wk k{w, line, (int)(threadIdx.x & 31), smem_u32(smem) + warp * (uint32_t)(kStages * Wk::kStageB), valid[warp]};
-  k.run(total, blockIdx.x * kWarps + warp, share_size(total, gridDim.x * kWarps, 1));
+  if (total > 0) {
+    Wk k{w, line, (int)(threadIdx.x & 31), smem_u32(smem) + warp * (uint32_t)(kStages * Wk::kStageB), valid[warp]};
+    k.run(total, blockIdx.x * kWarps + warp, share_size(total, gridDim.x * kWarps, 1));
+  }
+  // The own part is launched while the shared one runs and needs nothing of
+  // it, but the join waits for this kernel alone: so it ends after the other.
+  if (!SHARED) pdl_wait();
 }
 
 // One warp a (row, q head): joins its pieces.
@@ -410,47 +414,47 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   const PagedAttnArgs& a = w.a;
   const int lane = threadIdx.x & 31;
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  pdl_wait();
   if (item >= (int64_t)a.p.n_rows * a.p.n_q) return;
+  // ---- before the pieces are there: whose row it is and where its pieces will be
   const int row = (int)(item / a.p.n_q), hq = (int)(item - (int64_t)row * a.p.n_q);
-  const int hpg = a.p.n_q / a.p.n_kv, h = hq / hpg;
+  const int hpg = a.p.n_q / a.p.n_kv, h = hq / hpg, g = hq - h * hpg;
   const int i = warp_find_seq(a.p.indptr, a.p.n_seqs, row);
   if (i >= a.p.n_seqs || row < a.p.indptr[i]) return;  // behind the last sequence: left as it was
   const SeqInfo s = load_seq(a.p, i, a.shared_len);
   constexpr int E = HD / 32;
   bf16* dst = a.out + (size_t)item * HD + lane * E;
-  // the row's pieces: first slots, then the workers' slots of both parts
+  // a part's first slot, then the slots of the workers after the first (`step` rows apart)
   const float* src_o[2][2] = {};
   const float2* src_ml[2][2] = {};
-  int more[2] = {0, 0}, step[2] = {0, 0}, parts = 0;
-  auto part = [&](const Pieces& pc, const Line& line, const SeqInfo& s, int workers, int64_t T, int64_t x0, int r, int x) {
-    const int kt = line.key_tiles(s);
-    x0 += ((int64_t)h * line.row_tiles(s) + r / line.mt) * kt;
+  int more[2] = {0, 0}, step[2] = {0, 0};
+  auto part = [&](const Pieces& pc, int mt, int kt, int workers, int64_t T, int64_t x0, int r, int x) {
     const int64_t per = share_size(T, workers, 1);
     const int c0 = (int)(x0 / per), c1 = (int)((x0 + kt - 1) / per);
-    const size_t slot = (size_t)(c0 + 1) * line.mt + r % line.mt;
+    const size_t slot = (size_t)(c0 + 1) * mt + r % mt;
     src_o[x][0] = pc.first_o + item * HD;
     src_ml[x][0] = pc.first_ml + item;
     src_o[x][1] = pc.more_o + slot * HD;
     src_ml[x][1] = pc.more_ml + slot;
     more[x] = c1 - c0;
-    step[x] = line.mt;
+    step[x] = mt;
   };
-  if (s.ok) {
-    const int g = hq - h * hpg;
-    const Line own = make_line(a.p, a.shared_len, true, w.own_mt, w.own_keys, w.starts);
-    part(w.own, own, s, w.own_workers, w.starts[a.p.n_seqs], w.starts[i], (row - s.row0) * hpg + g, 0);
-    parts = 1;
-    if (a.shared_len > 0) {
-      const Line all = make_line(a.p, a.shared_len, false, w.shared_mt, w.shared_keys, nullptr);
-      part(w.shared, all, all.seq(0), w.shared_workers, all.tiles(all.seq(0)), 0, row * hpg + g, 1);
-      parts = 2;
-    } else if (more[0] == 0) {
-      return;  // one worker had the segment whole and wrote it
-    }
+  if (s.ok && a.shared_len > 0) {
+    const Line all = make_line(a.p, a.shared_len, false, w.shared_mt, w.shared_keys, nullptr);
+    const SeqInfo every = all.seq(0);
+    const int r = row * hpg + g, kt = all.key_tiles(every);
+    part(w.shared, w.shared_mt, kt, w.shared_workers, all.tiles(every),
+         ((int64_t)h * all.row_tiles(every) + r / w.shared_mt) * kt, r, 1);
   }
-  // piece x of the row: maxima and sums of 32 pieces in the lanes, then their O
-  const int n0 = parts > 0 ? 1 + more[0] : 0, n = n0 + (parts > 1 ? 1 + more[1] : 0);
+  const Line own = make_line(a.p, a.shared_len, true, w.own_mt, w.own_keys, w.starts);
+  const int r_own = (row - s.row0) * hpg + g, kt_own = own.key_tiles(s);
+  const int64_t x_own = ((int64_t)h * own.row_tiles(s) + r_own / w.own_mt) * kt_own;
+  pdl_wait();
+  if (s.ok) {
+    part(w.own, w.own_mt, kt_own, w.own_workers, w.starts[a.p.n_seqs], w.starts[i] + x_own, r_own, 0);
+    if (a.shared_len == 0 && more[0] == 0) return;  // one worker had the segment whole and wrote it
+  }
+  const int n0 = s.ok ? 1 + more[0] : 0, n = n0 + (s.ok && a.shared_len > 0 ? 1 + more[1] : 0);
+  // maxima and sums of 32 pieces in the lanes, then their O
   float o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
@@ -535,14 +539,30 @@ size_t lay_out(PagedWork& w, int num_sms, unsigned char* base) {
   return off;
 }
 
+// `overlap`: the launch may begin while the kernel before it runs.
+void launch_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& at, unsigned grid, int threads, int smem, cudaStream_t st,
+                          bool overlap) {
+  cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = overlap ? 1 : 0;
+}
+
 template <int HD, int NT, bool SHARED>
-cudaError_t launch_part(const PagedWork& w, int workers, cudaStream_t st) {
+cudaError_t launch_part(const PagedWork& w, int workers, cudaStream_t st, bool overlap) {
   const int smem = kWarps * kStages * Worker<HD, NT, SHARED>::kStageB;
   static cudaError_t once = cudaFuncSetAttribute(paged_attn_kernel<HD, NT, SHARED>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (once != cudaSuccess) return once;
-  paged_attn_kernel<HD, NT, SHARED><<<workers / kWarps, kWarps * 32, smem, st>>>(w);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute at;
+  launch_config(cfg, at, workers / kWarps, kWarps * 32, smem, st, overlap);
+  return cudaLaunchKernelEx(&cfg, paged_attn_kernel<HD, NT, SHARED>, w);
 }
 
 template <int HD>
@@ -553,7 +573,7 @@ cudaError_t launch(PagedWork& w, int num_sms, cudaStream_t st) {
   w.own_keys = kKT;
   cudaError_t e = cudaSuccess;
   if (w.a.shared_len > 0) {
-    if ((int64_t)p.n_rows * hpg > 32) {
+    if ((int64_t)p.n_rows * hpg > 32 && paged_shared_tc_takes(p)) {
       w.shared_mt = kTcRows;
       w.shared_keys = kTcKeys;
       w.shared_workers = num_sms;
@@ -561,24 +581,19 @@ cudaError_t launch(PagedWork& w, int num_sms, cudaStream_t st) {
     } else {
       w.shared_mt = (int64_t)p.n_rows * hpg > 16 ? 32 : 16;
       w.shared_keys = kKT;
-      e = w.shared_mt == 32 ? launch_part<HD, 2, true>(w, w.shared_workers, st)
-                            : launch_part<HD, 1, true>(w, w.shared_workers, st);
+      e = w.shared_mt == 32 ? launch_part<HD, 2, true>(w, w.shared_workers, st, false)
+                            : launch_part<HD, 1, true>(w, w.shared_workers, st, false);
     }
     if (e != cudaSuccess) return e;
   }
-  e = w.own_mt == 32 ? launch_part<HD, 2, false>(w, w.own_workers, st)
-                     : launch_part<HD, 1, false>(w, w.own_workers, st);
+  const bool after = w.a.shared_len > 0;
+  e = w.own_mt == 32 ? launch_part<HD, 2, false>(w, w.own_workers, st, after)
+                     : launch_part<HD, 1, false>(w, w.own_workers, st, after);
   if (e != cudaSuccess) return e;
   const int64_t items = (int64_t)p.n_rows * p.n_q;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((items + 3) / 4));
-  cfg.blockDim = dim3(128);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute at;
+  launch_config(cfg, at, (unsigned)((items + 3) / 4), 128, 0, st, true);
   return cudaLaunchKernelEx(&cfg, paged_join_kernel<HD>, static_cast<const PagedWork>(w));
 }
 

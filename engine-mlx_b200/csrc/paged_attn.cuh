@@ -27,6 +27,8 @@ struct PagedWork {
 // The shared part of a batch of many rows, on tcgen05 (paged_attn_tc.cu):
 // tiles of kTcRows rows and kTcKeys positions, one worker a CTA.
 constexpr int kTcRows = 256, kTcKeys = 128;
+// Pages that are whole 8-row groups of the tiles' swizzle.
+bool paged_shared_tc_takes(const PagedArgs& p);
 cudaError_t paged_shared_tc_launch(const PagedWork& w, int num_sms, cudaStream_t st);
 
 }  // namespace emx

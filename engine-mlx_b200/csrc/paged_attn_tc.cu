@@ -9,13 +9,16 @@
 // exponentials (128 x 128 a tile, 16 an SM and clock) and the tensor pipe.
 //
 // One CTA an SM, each with an even share of the (KV head, 256 rows, 128 keys)
-// tiles in line order; twelve warps:
-//   warps 0-7   two softmax groups of 128 threads, a thread a row: S from
-//               tensor memory, the running maximum and sum, P back over S;
-//   warp 8      one thread issues every MMA;
-//   warps 9-11  the keys' rows from their pages into a ring of five 128-row
-//               slots (K, V, K, V, ...) by 16-byte asynchronous copies, so a
-//               page may have any size and end anywhere in a tile.
+// tiles in line order; eleven warps:
+//   warps 0-7  two softmax groups of 128 threads, a thread a row: S from
+//              tensor memory, the running maximum and sum, P back over S;
+//   warps 8-9  one thread each issues the MMAs of a group;
+//   warp 10    TMA: a lane for each run of keys in one page (a box of 8 to 128
+//              rows, the largest power of two that divides the page size),
+//              into a ring of five 128-row slots (K, V, K, V, ...).  Boxes
+//              behind the prefix and pages outside the cache start beyond the
+//              tensor and read as zeros.  (16-byte asynchronous copies by two or
+//              three warps, which take any page size, reached 30 GB/s an SM.)
 // Each group is a stream of its own — S, P and O in tensor memory, its Q tile
 // in shared memory: two row tiles against the same keys where the segment has
 // more than 128 rows, else the same rows against alternate key tiles (then the
@@ -25,6 +28,10 @@
 // The maximum that the exponentials use moves only when a tile's exceeds it by
 // more than 2^8 (then O and l are rescaled); O / l does not depend on it.  P is
 // rounded to bf16 for its product (off by at most 2^-9 of each weight).
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
 #include "paged_attn.cuh"
 #include "tc_attn.cuh"
 
@@ -32,12 +39,11 @@ namespace emx {
 
 namespace {
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 352;
 constexpr int kSlots = 5;
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
+constexpr int kMmaWarp = 8, kLoadWarp = 10;
 constexpr float kRescale = 8.0f;
 constexpr uint32_t kCols = 512;  // S of the groups at 0 and 128 (P over its upper half), O at 256 and 384
-constexpr int kLag = 3;          // most slots whose copies a loader leaves in flight
 constexpr int kValid = 4;        // tiles whose key masks are kept: a tile's V slot is free before the ring holds 3 later ones
 
 template <int HD>
@@ -52,7 +58,9 @@ struct Smem {
 
 struct Bars {
   uint64_t full[kSlots], empty[kSlots];
-  uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
+  uint64_t q_full[2], s_full[2], p_full[2];
+  uint64_t o_full[2];  // a segment's last product is in O
+  uint64_t turn[2];
   uint32_t tmem;
   alignas(16) unsigned char valid[kValid][16];  // by tile of the share, bit j: key j is there
 };
@@ -63,10 +71,25 @@ constexpr uint32_t idesc(int n, bool b_mn) {
          ((uint32_t)(128 >> 4) << 24);
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
-  const int n = on ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
 }
+
+// A place in the ring, and the parity of the mbarrier phase that its next use completes.
+struct Slot {
+  int s;
+  uint32_t parity;
+  __device__ __forceinline__ void step(int n) {
+    s += n;
+    if (s >= kSlots) {
+      s -= kSlots;
+      parity ^= 1;
+    }
+  }
+};
 
 // 16-byte chunk c of row r of a tile (64-column blocks, 128-byte swizzle).
 __device__ __forceinline__ uint32_t tile_at(int r, int c) {
@@ -120,7 +143,9 @@ struct Walk {
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 1) paged_shared_tc_kernel(const __grid_constant__ PagedWork w) {
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_shared_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                           const __grid_constant__ PagedWork w, int box) {
   using L = Smem<HD>;
   extern __shared__ __align__(1024) unsigned char raw[];
   unsigned char* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
@@ -129,16 +154,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_tc_kernel(const __gr
   int* status = a.p.status;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  pdl_trigger();  // the own part does not read what this one writes (it only ends after it)
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) {
-      mbar_init(&B.full[s], kLoadWarps);
-      mbar_init(&B.empty[s], 1);
+      mbar_init(&B.full[s], 1);
+      mbar_init(&B.empty[s], 2);
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(&B.q_full[g], 128);
       mbar_init(&B.s_full[g], 2);
       mbar_init(&B.p_full[g], 128);
-      mbar_init(&B.o_done[g], 1);
+      mbar_init(&B.o_full[g], 1);
+      mbar_init(&B.turn[g], 1);
     }
     fence_mbar_init();
   }
@@ -160,160 +187,150 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_tc_kernel(const __gr
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && mbar_wait_bounded(bar, parity, status); };
 
-  if (any && warp >= kLoadWarp) {
-    // ---- loaders: warp p has rows 8g .. 8g + 7 of a tile for g = p, p + 3, ... < 16
-    const int p = warp - kLoadWarp;
-    constexpr int kChunks = HD / 8;
-    constexpr int kPerGroup = 8 * kChunks / 32;
-    int slot = 0, tile = 0;
-    int loaded = 0, done = 0;            // slots begun, slots handed over
-    uint32_t parity = 1;                 // of `empty` for the next use of `slot`: the first round waits for nothing
-    auto hand_over = [&]() {
-      fence_proxy_async();  // the copies were generic writes; the MMAs read through the async proxy
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&B.full[done % kSlots]);
-      ++done;
+  if (any && warp == kLoadWarp) {
+    // ---- loader: lane b has box b of a tile
+    const int boxes = kTcKeys / box;
+    const int64_t beyond = (int64_t)a.p.n_pages * a.p.n_kv * a.p.page_size;
+    // the page is loaded a tile ahead and not looked at here: a look would wait for it
+    auto look_up = [&](int k) {
+      const int pos = k * kTcKeys + lane * box;
+      return lane < boxes && pos < a.shared_len ? a.shared_pages[pos / a.p.page_size] : -1;
     };
-    do {
-      for (int t = 0; t < wk.n; ++t) {
-        // cache rows of this warp's keys: groups 0-3 of the warp in id[0] (lane = 8 * group + row), 4-5 in id[1]
-        uint32_t id[2];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int g = p + 3 * (b * 4 + (lane >> 3));
-          const int pos = (wk.c.k + t) * kTcKeys + g * 8 + (lane & 7);
-          id[b] = ~0u;
-          if (g < 16 && pos < a.shared_len) {
-            const int pg = pos / a.p.page_size, page = a.shared_pages[pg];
-            if (page >= 0 && page < a.p.n_pages)
-              id[b] = cache_row(page, a.p.n_kv, wk.c.head(), a.p.page_size, pos - pg * a.p.page_size);
-            else
-              report_status(status, kDevBadPage);
-          }
-        }
-        const unsigned there[2] = {__ballot_sync(0xffffffffu, id[0] != ~0u), __ballot_sync(0xffffffffu, id[1] != ~0u)};
-#pragma unroll 1
-        for (int kv = 0; kv < 2; ++kv) {
-          // while the slot is not free, what has been begun goes over as it lands
-          while (loaded > done && !__all_sync(0xffffffffu, mbar_test_wait(&B.empty[slot], parity))) {
-            switch (loaded - done) {
-              case 1: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-              case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-              default: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-            }
-            hand_over();
-          }
-          wait(&B.empty[slot], parity);
-          const bf16* src = kv ? a.p.v : a.p.k;
-          const uint32_t dst = smem_u32(smem + L::kRing + slot * L::kTile);
-#pragma unroll
-          for (int y = 0; y < 6; ++y) {
-            const int g = p + 3 * y;
-            if (g >= 16) break;
-#pragma unroll
-            for (int i = 0; i < kPerGroup; ++i) {
-              const int e = i * 32 + lane, r = e / kChunks, c = e % kChunks;
-              const uint32_t row = __shfl_sync(0xffffffffu, id[y >> 2], (y & 3) * 8 + r);
-              const bool on = row != ~0u;
-              cp16(dst + tile_at(g * 8 + r, c), src + (on ? (size_t)row * HD + c * 8 : 0), on);
-            }
-            if (kv == 0 && lane == 0) B.valid[tile % kValid][g] = (unsigned char)(there[y >> 2] >> ((y & 3) * 8));
-          }
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          ++loaded;
-          if (loaded - done > kLag) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
-            hand_over();
-          }
-          if (++slot == kSlots) {
-            slot = 0;
-            parity ^= 1;
-          }
-        }
-        ++tile;
+    Slot at{0, 1};  // `empty`: the first round waits for nothing
+    int page = look_up(wk.c.k), tile = 0;
+    bool more = true;
+    for (int t = 0; more;) {
+      const int pos = (wk.c.k + t) * kTcKeys + lane * box;
+      bool on = lane < boxes && pos < a.shared_len;
+      if (on && (page < 0 || page >= a.p.n_pages)) {
+        report_status(status, kDevBadPage);
+        on = false;
       }
-    } while (wk.next(line));
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    while (done < loaded) hand_over();
-  } else if (any && warp == kMmaWarp) {
+      const int row = on ? (int)cache_row(page, a.p.n_kv, wk.c.head(), a.p.page_size, pos % a.p.page_size) : (int)beyond;
+      if (++t == wk.n) {
+        more = wk.next(line);
+        t = 0;
+      }
+      if (more) page = look_up(wk.c.k + t);
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv) {
+        wait(&B.empty[at.s], at.parity);
+        if (kv == 0 && lane < boxes)
+          for (int g = 0; g < box / 8; ++g) B.valid[tile % kValid][lane * (box / 8) + g] = on ? 0xff : 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(&B.full[at.s], (uint32_t)L::kTile);
+        __syncwarp();
+        if (lane < boxes) {
+          const uint32_t dst = smem_u32(smem + L::kRing + at.s * L::kTile) + (uint32_t)(lane * box * 128);
+#pragma unroll
+          for (int b = 0; b < HD / 64; ++b) tma_2d(dst + b * kBlk, kv ? &tv : &tk, b * 64, row, &B.full[at.s]);
+        }
+        at.step(1);
+      }
+      ++tile;
+    }
+    // copies still on their way (after a wait that gave up) have landed before the CTA ends
+    const int last = 2 * tile < kSlots ? 2 * tile : kSlots;
+    for (int i = 0; i < last; ++i) {
+      at.s = at.s == 0 ? kSlots - 1 : at.s - 1;
+      const uint32_t use = (uint32_t)((2 * tile - 1 - i) / kSlots);
+      mbar_wait_bounded(&B.full[at.s], use & 1, status);
+    }
+  } else if (any && warp >= kMmaWarp) {
     if (lane == 0) {
-      // ---- MMA issuer.  A group's QK^T of a tile follows its PV of the one before (P lies over S; MMAs run in order).
+      // ---- MMA issuer of group g.  A tile's S = Q K^T follows the O += P V of the group's tile before (P lies over S; the
+      // MMAs of a thread run in the order of their issue), so S of a tile also says that O holds all before it.
+      const int g = warp - kMmaWarp;
       constexpr uint32_t id_s = idesc(128, false), id_pv = idesc(HD, true);
-      int slot = 0;             // of the next K tile
-      uint32_t full_parity[kSlots];
-#pragma unroll
-      for (int s = 0; s < kSlots; ++s) full_parity[s] = 0;
-      uint32_t p_parity[2] = {0, 0};
-      uint32_t seg_parity = 0;
-      int pend[2] = {-1, -1};   // V slot that a group's P waits for
-      bool first[2] = {true, true}, frees[2] = {true, true};  // its PV begins O / is the slot's last use
-      // the ring's slots in order: wait for each once
-      uint32_t waited = 0;      // bit s: slot s' current contents are there
-      auto need = [&](int s) {
-        if (waited >> s & 1) return;
-        uint32_t par = 0;
-#pragma unroll
-        for (int x = 0; x < kSlots; ++x)
-          if (x == s) {
-            par = full_parity[x];
-            full_parity[x] ^= 1;
-          }
-        wait(&B.full[s], par);
-        waited |= 1u << s;
+      // operand descriptors: the low word holds the address in 16-byte units, the high word is the same for all tiles
+      const uint64_t k0 = desc_kmajor(smem), mn0 = desc_mnmajor(smem);
+      auto at16 = [](uint64_t d, uint32_t bytes) {
+        return (d & 0xffffffff00000000ull) | (uint32_t)((uint32_t)d + (bytes >> 4));
       };
-      auto release = [&](int s) {
-        umma_commit(&B.empty[s]);
-        waited &= ~(1u << s);
+      auto soon = [&](uint64_t* bar, uint32_t parity) {  // polls closely before the bounded wait's longer steps
+        for (int i = 0; i < 2000; ++i)
+          if (mbar_test_wait(bar, parity)) return;
+        wait(bar, parity);
       };
-      auto pv = [&](int g) {
-        if (pend[g] < 0) return;
-        wait(&B.p_full[g], p_parity[g]);
-        p_parity[g] ^= 1;
-        need(pend[g]);
-        tfence_after();
-        const unsigned char* V = smem + L::kRing + pend[g] * L::kTile;
+      const uint64_t Q = at16(k0, L::kQ + g * L::kTile);
+      const uint32_t tS = tmem + 128 * g, tO = tmem + 256 + 128 * g;
+      auto qk = [&](int s) {
+        const uint64_t K = at16(k0, L::kRing + s * L::kTile);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          umma_ta(tmem + 256 + 128 * g, tmem + 128 * g + 64 + 8 * k, desc_mnmajor(V + k * 2048), id_pv, (k > 0 || !first[g]) ? 1u : 0u);
-        if (frees[g]) release(pend[g]);
-        umma_commit(&B.o_done[g]);
-        pend[g] = -1;
-        first[g] = false;
+        for (int k = 0; k < HD / 16; ++k)  // 16 head dims a step: 32 bytes along the rows of a 64-column block
+          umma(tS, at16(Q, (k >> 2) * kBlk + 32 * (k & 3)), at16(K, (k >> 2) * kBlk + 32 * (k & 3)), id_s, k > 0 ? 1u : 0u);
       };
+      auto pv = [&](int s, bool first) {
+        const uint64_t V = at16(mn0, L::kRing + s * L::kTile);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)  // 16 keys a step: 8 columns of P, 16 rows of V
+          umma_ta(tO, tS + 64 + 8 * k, at16(V, k * 2048), id_pv, (k > 0 || !first) ? 1u : 0u);
+      };
+      auto s_done = [&]() {
+        umma_commit(&B.s_full[g]);
+        mbar_arrive(&B.s_full[g]);  // and the key masks, which the wait for K has seen
+      };
+      Slot ks{0, 0}, vs{1, 0};
+      uint32_t p_parity = 0, seg_parity = 0, turn_parity = g == 0 ? 1 : 0;
       do {
-        const bool pair = wk.pair();
-        for (int g = 0; g < 2; ++g) {
-          wait(&B.q_full[g], seg_parity);
-          first[g] = true;
-        }
+        wait(&B.q_full[g], seg_parity);
         seg_parity ^= 1;
-        for (int t = 0; t < wk.n; ++t) {
-          const int ks = slot, vs = slot + 1 == kSlots ? 0 : slot + 1;
-          slot = vs + 1 == kSlots ? 0 : vs + 1;
-          for (int g = pair ? 0 : t & 1; g < (pair ? 2 : (t & 1) + 1); ++g) {
-            pv(g);
-            need(ks);
+        if (wk.pair()) {
+          // The groups take turns with a tile's PV and the next one's QK^T together: one's S is done while the other takes
+          // exponentials.  (Left alone they fell into step and both waited for the pipe, then both for the exponentials.)
+          Slot before = vs;
+          for (int t = 0; t <= wk.n; ++t) {
+            if (t < wk.n) soon(&B.full[ks.s], ks.parity);
+            if (t > 0) {
+              soon(&B.full[before.s], before.parity);
+              soon(&B.p_full[g], p_parity);
+              p_parity ^= 1;
+            }
+            soon(&B.turn[g], turn_parity);
+            turn_parity ^= 1;
             tfence_after();
-            const unsigned char* Q = smem + L::kQ + g * L::kTile;
-            const unsigned char* K = smem + L::kRing + ks * L::kTile;
-#pragma unroll
-            for (int k = 0; k < HD / 16; ++k)
-              umma(tmem + 128 * g, desc_kmajor(Q + (k >> 2) * kBlk) + 2 * (k & 3), desc_kmajor(K + (k >> 2) * kBlk) + 2 * (k & 3),
-                   id_s, k > 0 ? 1u : 0u);
-            umma_commit(&B.s_full[g]);
-            mbar_arrive(&B.s_full[g]);  // and the key masks that `need` has seen
-            pend[g] = vs;
-            frees[g] = !pair || g == 1;
+            if (t > 0) pv(before.s, t == 1);
+            if (t < wk.n) qk(ks.s);
+            mbar_arrive(&B.turn[g ^ 1]);
+            if (t < wk.n) {
+              s_done();
+              umma_commit(&B.empty[ks.s]);
+            }
+            if (t > 0) umma_commit(&B.empty[before.s]);
+            if (t == wk.n) break;
+            before = vs;
+            ks.step(2);
+            vs.step(2);
           }
-          release(ks);
+          umma_commit(&B.o_full[g]);
+        } else {
+          // alternate tiles: a product at once when its P is there, so that its V slot can be filled again
+          for (int t = 0; t < wk.n; ++t) {
+            soon(&B.full[ks.s], ks.parity);
+            if ((t & 1) == g) {
+              tfence_after();
+              qk(ks.s);
+              s_done();
+              umma_commit(&B.empty[ks.s]);
+              soon(&B.full[vs.s], vs.parity);
+              soon(&B.p_full[g], p_parity);
+              p_parity ^= 1;
+              tfence_after();
+              pv(vs.s, t < 2);
+              umma_commit(&B.empty[vs.s]);
+            } else {
+              mbar_arrive(&B.empty[ks.s]);  // the other group's: free of this one
+              soon(&B.full[vs.s], vs.parity);
+              mbar_arrive(&B.empty[vs.s]);
+            }
+            ks.step(2);
+            vs.step(2);
+          }
+          if (wk.n > g) umma_commit(&B.o_full[g]);
         }
-        // the segment's last products, in the order that their tiles were begun
-        const int g0 = pair ? 0 : wk.n & 1;
-        pv(g0);
-        pv(g0 ^ 1);
       } while (wk.next(line));
     }
-  } else if (any && warp < kMmaWarp) {
+  } else if (any) {
     // ---- softmax: group g, row r of its tile
     const int g = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -321,9 +338,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_tc_kernel(const __gr
     const float sl2 = fabsf(a.scale) * kLog2e;
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
     uint32_t s_parity = 0;
-    uint32_t tiles = 0;   // of this group so far
-    int tile = -1;        // of the share
-    uint32_t other = 0;   // tiles of the other group so far
+    uint32_t o_parity = 0;  // bit x: of group x' next finished segment
+    int tile = -1;          // of the share
     do {
       const bool pair = wk.pair();
       const int h = wk.c.head();
@@ -349,11 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_tc_kernel(const __gr
       int mine_n = 0;  // tiles of this group in the segment
       for (int t = 0; t < wk.n; ++t) {
         ++tile;
-        if (!pair && (t & 1) != g) {
-          ++other;
-          continue;
-        }
-        if (pair) ++other;
+        if (!pair && (t & 1) != g) continue;
         wait(&B.s_full[g], s_parity);
         s_parity ^= 1;
         tfence_after();
@@ -394,9 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_tc_kernel(const __gr
           const bool up = mx > m + kRescale || (m == -INFINITY && mx > m);
           if (__any_sync(0xffffffffu, up)) {
             const float alpha = up ? ex2f(m - mx) : 1.f;  // 0 at the first tile
-            if (mine_n > 0) {
-              wait(&B.o_done[g], (tiles - 1) & 1);  // the products so far are in O
-              tfence_after();
+            if (mine_n > 0) {  // O holds the products so far: S came after them
 #pragma unroll
               for (int c = 0; c < HD / 32; ++c) {
                 float v[32];
@@ -434,7 +444,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_tc_kernel(const __gr
         }
         tfence_before();
         mbar_arrive(&B.p_full[g]);
-        ++tiles;
         ++mine_n;
       }
       // ---- the segment's pieces
@@ -444,7 +453,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_tc_kernel(const __gr
       dst = (first ? w.shared.first_o : w.shared.more_o) + at * HD;
       float2* ml = (first ? w.shared.first_ml : w.shared.more_ml) + at;
       if (pair) {
-        wait(&B.o_done[g], (tiles - 1) & 1);
+        wait(&B.o_full[g], o_parity >> g & 1);
+        o_parity ^= 3;
         tfence_after();
         if (busy) {
 #pragma unroll
@@ -463,17 +473,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_tc_kernel(const __gr
         tfence_before();
       } else {
         // both groups have these rows: each joins one half of the columns
-        // (maxima and sums meet where the Q tiles were: their last S is done)
+        // (maxima and sums meet where the Q tiles were: a group's last S is done, so all of its Q has been written and read)
         auto mls = [&](int x) { return reinterpret_cast<float2*>(smem + L::kQ + x * L::kTile) + r; };
-        *mls(g) = make_float2(m, l);
-        if (mine_n > 0) wait(&B.o_done[g], (tiles - 1) & 1);
-        const int other_n = wk.n - mine_n;
-        if (other_n > 0) wait(&B.o_done[g ^ 1], (other - 1) & 1);
+        if (mine_n > 0) *mls(g) = make_float2(m, l);
+        wait(&B.o_full[0], o_parity & 1);
+        if (wk.n > 1) wait(&B.o_full[1], o_parity >> 1 & 1);
+        o_parity ^= wk.n > 1 ? 3u : 1u;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         tfence_after();
         if (busy) {
-          const float2 x = *mls(0), y = *mls(1);
-          const int n0 = g == 0 ? mine_n : other_n, n1 = wk.n - n0;
+          const float2 x = *mls(0), y = wk.n > 1 ? *mls(1) : make_float2(-INFINITY, 0.f);
           const float to = fmaxf(x.x, y.x), b = to == -INFINITY ? 0.f : to;
           const float wx = ex2f(x.x - b), wy = ex2f(y.x - b);
           const uint32_t tO = tmem + lanes + 256 + g * (HD / 2);
@@ -486,9 +495,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_tc_kernel(const __gr
             wait_ld(v);
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              float z = n0 > 0 ? u[i] * wx : 0.f;  // a group without tiles: its O is not defined
-              if (n1 > 0) z = fmaf(v[i], wy, z);
-              u[i] = z;
+              u[i] *= wx;
+              if (wk.n > 1) u[i] = fmaf(v[i], wy, u[i]);  // group 1 without a tile: its O is not defined
             }
             if (mine) {
 #pragma unroll
@@ -512,16 +520,49 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_tc_kernel(const __gr
   }
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+std::once_flag g_encode_once;
+
+// The cache's rows [n_pages * n_kv * page_size][head_dim] in boxes of 64 columns x `box` rows, 128-byte swizzle.
+cudaError_t encode(CUtensorMap* map, const PagedArgs& p, const void* base, int box) {
+  std::call_once(g_encode_once, [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  });
+  if (!g_encode) return cudaErrorNotSupported;
+  const cuuint64_t dims[2] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.n_pages * p.n_kv * p.page_size};
+  const cuuint64_t strides[1] = {(cuuint64_t)p.head_dim * 2};
+  const cuuint32_t size[2] = {64, (cuuint32_t)box}, one[2] = {1, 1};
+  return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, size, one,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? cudaSuccess
+             : cudaErrorInvalidValue;
+}
+
 template <int HD>
 cudaError_t launch(const PagedWork& w, int num_sms, cudaStream_t st) {
   static cudaError_t once = cudaFuncSetAttribute(paged_shared_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  Smem<HD>::kBytes);
   if (once != cudaSuccess) return once;
-  paged_shared_tc_kernel<HD><<<num_sms, kThreads, Smem<HD>::kBytes, st>>>(w);
+  int box = kTcKeys;
+  while (w.a.p.page_size % box) box /= 2;
+  CUtensorMap tk, tv;
+  cudaError_t e = encode(&tk, w.a.p, w.a.p.k, box);
+  if (e == cudaSuccess) e = encode(&tv, w.a.p, w.a.p.v, box);
+  if (e != cudaSuccess) return e;
+  paged_shared_tc_kernel<HD><<<num_sms, kThreads, Smem<HD>::kBytes, st>>>(tk, tv, w, box);
   return cudaGetLastError();
 }
 
 }  // namespace
+
+bool paged_shared_tc_takes(const PagedArgs& p) {
+  return p.page_size % 8 == 0 && p.n_pages > 0;
+}
 
 cudaError_t paged_shared_tc_launch(const PagedWork& w, int num_sms, cudaStream_t st) {
   return w.a.p.head_dim == 128 ? launch<128>(w, num_sms, st) : launch<64>(w, num_sms, st);

@@ -43,8 +43,8 @@ EMX_HD SeqInfo seq_info(int a, int b, int len, int n_rows, int shared, int64_t r
 EMX_HD int ceil_div(int a, int b) { return (int)(((int64_t)a + b - 1) / b); }
 
 // Row (in units of head_dim elements) of the cache [n_pages, n_kv, page_size]
-// that holds position `off` of page `page` for KV head h.  A pool of
-// 64-element bf16 rows with more than 2^32 of them would not fit the device.
+// that holds position `off` of page `page` for KV head h; the host refuses a
+// cache of 2^31 rows or more.
 EMX_HD uint32_t cache_row(int page, int n_kv, int h, int page_size, int off) {
   return ((uint32_t)page * (uint32_t)n_kv + (uint32_t)h) * (uint32_t)page_size + (uint32_t)off;
 }
