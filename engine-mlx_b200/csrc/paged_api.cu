@@ -3,6 +3,7 @@
 // call checks its arguments on the host (the context last, so that a shape is
 // refused without a device), enqueues on the context's stream and allocates
 // nothing, so it may be captured into a graph.
+#include <cfloat>
 #include <cmath>
 
 #include "ctx.cuh"
@@ -150,7 +151,8 @@ int emx_sdpa_paged(emx_ctx* c, const void* q, const emx_paged_kv* kv, const emx_
   a.out = static_cast<bf16*>(out);
   a.shared_len = shared_len;
   a.shared_pages = shared_pages;
-  a.scale = scale;
+  // equal weights for a scale of 0: the kernels mask by infinite scores, which 0 would turn to NaN
+  a.scale = scale == 0.f ? FLT_MIN : scale;
   a.workspace = workspace;
   EMX_CHECK_CUDA(paged_attn_launch(a, c->num_sms, c->stream), "emx_sdpa_paged");
   return EMX_OK;

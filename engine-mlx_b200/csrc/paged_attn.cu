@@ -105,34 +105,45 @@ struct Worker {
     return (uint32_t)(r * kRowB + ((c ^ (r & 7)) << 4));
   }
 
-  // Cache row of key `lane` (< 16) of the cursor's tile, ~0 where there is none.
-  __device__ __forceinline__ uint32_t key_row(const Cursor& c) const {
+  // The page of key `lane` (< 16) of the cursor's tile and its place there, -1
+  // behind the sequence's end.  Loaded a tile ahead of its use and not looked
+  // at before: a look would wait for it.
+  struct Key {
+    int page, off;
+  };
+  __device__ __forceinline__ Key key_of(const Cursor& c) const {
     const PagedAttnArgs& a = w.a;
     const int pos = (SHARED ? 0 : a.shared_len) + c.k * kKT + (lane & 15);
-    uint32_t row = ~0u;
+    Key key{0, -1};
     if (pos < c.s.len) {
       const int pg = pos / a.p.page_size;
-      const int page = SHARED ? a.shared_pages[pg] : a.p.table[(size_t)c.seq * a.p.max_pages + pg];
-      if (page >= 0 && page < a.p.n_pages)
-        row = cache_row(page, a.p.n_kv, c.head(), a.p.page_size, pos - pg * a.p.page_size);
-      else
-        report_status(a.p.status, kDevBadPage);
+      key.page = SHARED ? a.shared_pages[pg] : a.p.table[(size_t)c.seq * a.p.max_pages + pg];
+      key.off = pos - pg * a.p.page_size;
     }
-    return row;
+    return key;
   }
 
-  __device__ __forceinline__ void issue(int stage, uint32_t row) const {
-    const uint32_t base = ring + stage * kStageB;
+  __device__ __forceinline__ void issue(int stage, const Key& key, int head) const {
+    const PagedAttnArgs& a = w.a;
+    uint32_t row = ~0u;  // cache row of key `lane`, where there is one
+    if (key.off >= 0) {
+      if (key.page >= 0 && key.page < a.p.n_pages) row = cache_row(key.page, a.p.n_kv, head, a.p.page_size, key.off);
+      else report_status(a.p.status, kDevBadPage);
+    }
     const unsigned there = __ballot_sync(0xffffffffu, row != ~0u) & 0xffffu;
     if (lane == 0) valid[stage] = there;
+    constexpr int kRows = 32 / kChunks;  // rows of one copy of the warp
+    const int sub = lane / kChunks, c = lane % kChunks;
+    const bf16 *kp = a.p.k + c * 8, *vp = a.p.v + c * 8;
+    const uint32_t dst = ring + stage * kStageB + at(sub, c);
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
-      const int r = (i * 32 + lane) / kChunks, c = lane % kChunks;
-      const uint32_t src = __shfl_sync(0xffffffffu, row, r);
+      const uint32_t src = __shfl_sync(0xffffffffu, row, i * kRows + sub);
       const bool on = src != ~0u;
-      const size_t off = on ? (size_t)src * HD + c * 8 : 0;
-      cp_async16(base + at(r, c), w.a.p.k + off, on);
-      cp_async16(base + kTileB + at(r, c), w.a.p.v + off, on);
+      const size_t off = on ? (size_t)src * HD : 0;
+      const uint32_t to = (dst ^ (uint32_t)(((i * kRows) & 7) << 4)) + (uint32_t)(i * kRows * kRowB);  // at(i kRows + sub, c)
+      cp_async16(to, kp + off, on);
+      cp_async16(to + kTileB, vp + off, on);
     }
   }
 
@@ -151,19 +162,22 @@ __device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int64_t total, int w
   const int hpg = line.hpg;
   cc.seek(line, x0);
   ld = cc;
-  uint32_t row = key_row(ld);
-  int loaded = 0;
-  for (; loaded < kStages - 1; ++loaded) {
+  Key key = key_of(ld);
+  int loaded = 0;  // tiles begun
+  auto load = [&]() {
     if (loaded < n) {
-      issue(loaded, row);
-      if (loaded + 1 < n) {
+      issue(loaded % kStages, key, ld.head());
+      if (++loaded < n) {
         ld.next(line);
-        row = key_row(ld);
+        key = key_of(ld);
       }
     }
     cp_commit();
-  }
+  };
+#pragma unroll 1
+  for (int i = 0; i < kStages - 1; ++i) load();
   const float sl2 = a.scale * kLog2e;
+  const float nothing = sl2 < 0.f ? INFINITY : -INFINITY;  // the score of a key that is not seen
   const int quad = lane >> 2, col = (lane & 3) * 2;
 
   uint32_t qf[NT][HD / 16][4];
@@ -209,15 +223,7 @@ __device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int64_t total, int w
       for (int x = 16; x > 0; x >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, x));
     }
     // ---- the next load, then this tile
-    if (loaded < n) {
-      issue(loaded % kStages, row);
-      ++loaded;
-      if (loaded < n) {
-        ld.next(line);
-        row = key_row(ld);
-      }
-    }
-    cp_commit();
+    load();
     cp_wait<kStages - 1>();
     __syncwarp();
     const int stage = t % kStages;
@@ -242,6 +248,9 @@ __device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int64_t total, int w
         mma_bf16_16816(s[nt][1], qf[nt][ks][0], qf[nt][ks][1], qf[nt][ks][2], qf[nt][ks][3], kf[2], kf[3]);
       }
     }
+    // m is the maximum of s * scale * log2 e.  Masks only where a key is missing
+    // or some row does not see the whole tile.
+    const bool masked = there != 0xffffu || key0 + kKT > least;
     uint32_t pf[NT][4];
     bool moved = false;
     float alpha[NT][2];
@@ -249,17 +258,18 @@ __device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int64_t total, int w
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        float mx = -INFINITY;
+        if (masked) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int key = j * 8 + col + e;
-            const bool on = key0 + key < vis[nt][b] && ((there >> key) & 1u);
-            float& v = s[nt][j][2 * b + e];
-            v = on ? v * sl2 : -INFINITY;
-            mx = fmaxf(mx, v);
-          }
+            for (int e = 0; e < 2; ++e) {
+              const int key = j * 8 + col + e;
+              float& v = s[nt][j][2 * b + e];
+              if (!(key0 + key < vis[nt][b] && ((there >> key) & 1u))) v = nothing;
+            }
+        }
+        float mx = fmaxf(fmaxf(s[nt][0][2 * b] * sl2, s[nt][0][2 * b + 1] * sl2),
+                         fmaxf(s[nt][1][2 * b] * sl2, s[nt][1][2 * b + 1] * sl2));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float to = fmaxf(m[nt][b], mx);
@@ -273,7 +283,7 @@ __device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int64_t total, int w
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            pv[j][e] = ex2f(s[nt][j][2 * b + e] - base);
+            pv[j][e] = ex2f(fmaf(s[nt][j][2 * b + e], sl2, -base));
           }
         // weights go to the products in bf16: each is off by at most 2^-9 of
         // itself, and l sums the rounded ones, so a constant V comes out exact
@@ -413,96 +423,92 @@ template <int HD>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedWork w) {
   const PagedAttnArgs& a = w.a;
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (item >= (int64_t)a.p.n_rows * a.p.n_q) return;
-  // ---- before the pieces are there: whose row it is and where its pieces will be
-  const int row = (int)(item / a.p.n_q), hq = (int)(item - (int64_t)row * a.p.n_q);
+  const int item = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (item >= a.p.n_rows * a.p.n_q) return;
+  // ---- before the pieces are there: whose row it is and where the shared part's pieces will be
+  const int row = item / a.p.n_q, hq = item - row * a.p.n_q;
   const int hpg = a.p.n_q / a.p.n_kv, h = hq / hpg, g = hq - h * hpg;
   const int i = warp_find_seq(a.p.indptr, a.p.n_seqs, row);
   if (i >= a.p.n_seqs || row < a.p.indptr[i]) return;  // behind the last sequence: left as it was
   const SeqInfo s = load_seq(a.p, i, a.shared_len);
   constexpr int E = HD / 32;
-  bf16* dst = a.out + (size_t)item * HD + lane * E;
-  // a part's first slot, then the slots of the workers after the first (`step` rows apart)
-  const float* src_o[2][2] = {};
-  const float2* src_ml[2][2] = {};
-  int more[2] = {0, 0}, step[2] = {0, 0};
-  auto part = [&](const Pieces& pc, int mt, int kt, int workers, int64_t T, int64_t x0, int r, int x) {
+  // the slot of a segment's second worker, and how many follow the first
+  auto more_of = [&](int mt, int kt, int workers, int64_t T, int64_t x0, int r, size_t& slot) {
     const int64_t per = share_size(T, workers, 1);
-    const int c0 = (int)(x0 / per), c1 = (int)((x0 + kt - 1) / per);
-    const size_t slot = (size_t)(c0 + 1) * mt + r % mt;
-    src_o[x][0] = pc.first_o + item * HD;
-    src_ml[x][0] = pc.first_ml + item;
-    src_o[x][1] = pc.more_o + slot * HD;
-    src_ml[x][1] = pc.more_ml + slot;
-    more[x] = c1 - c0;
-    step[x] = mt;
+    const int c0 = share_of(x0, per), c1 = share_of(x0 + kt - 1, per);
+    slot = (size_t)(c0 + 1) * mt + r % mt;
+    return c1 - c0;
   };
+  size_t slot_shared = 0, slot_own = 0;
+  int more_shared = 0;
   if (s.ok && a.shared_len > 0) {
     const Line all = make_line(a.p, a.shared_len, false, w.shared_mt, w.shared_keys, nullptr);
     const SeqInfo every = all.seq(0);
     const int r = row * hpg + g, kt = all.key_tiles(every);
-    part(w.shared, w.shared_mt, kt, w.shared_workers, all.tiles(every),
-         ((int64_t)h * all.row_tiles(every) + r / w.shared_mt) * kt, r, 1);
+    more_shared = more_of(w.shared_mt, kt, w.shared_workers, all.tiles(every),
+                          ((int64_t)h * all.row_tiles(every) + r / w.shared_mt) * kt, r, slot_shared);
   }
   const Line own = make_line(a.p, a.shared_len, true, w.own_mt, w.own_keys, w.starts);
   const int r_own = (row - s.row0) * hpg + g, kt_own = own.key_tiles(s);
   const int64_t x_own = ((int64_t)h * own.row_tiles(s) + r_own / w.own_mt) * kt_own;
-  pdl_wait();
-  if (s.ok) {
-    part(w.own, w.own_mt, kt_own, w.own_workers, w.starts[a.p.n_seqs], w.starts[i] + x_own, r_own, 0);
-    if (a.shared_len == 0 && more[0] == 0) return;  // one worker had the segment whole and wrote it
-  }
-  const int n0 = s.ok ? 1 + more[0] : 0, n = n0 + (s.ok && a.shared_len > 0 ? 1 + more[1] : 0);
-  // maxima and sums of 32 pieces in the lanes, then their O
+
   float o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
   float m = -INFINITY, l = 0.f;
-  auto o_of = [&](int x) {
-    const int b = x >= n0, y = x - (b ? n0 : 0);
-    return y == 0 ? src_o[b][0] : src_o[b][1] + (size_t)(y - 1) * step[b] * HD;
-  };
-  for (int x0 = 0; x0 < n; x0 += 32) {
-    const int x = x0 + lane;
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (x < n) {
-      const int b = x >= n0, y = x - (b ? n0 : 0);
-      ml = y == 0 ? *src_ml[b][0] : src_ml[b][1][(size_t)(y - 1) * step[b]];
-    }
-    // a NaN among the sums stays one, whatever its maximum
-    const float to = fmaxf(m, warp_max(ml.x)), base = to == -INFINITY ? 0.f : to;
-    const float was = ex2f(m - base), wx = ex2f(ml.x - base);
-    l = l * was + warp_sum(ml.y * wx);
+  // n pieces: the first slot, then those of further workers
+  auto take = [&](const Pieces& pc, size_t slot, int mt, int n) {
+    for (int x0 = 0; x0 < n; x0 += 32) {
+      const int x = x0 + lane;  // this lane's (max, sum)
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (x < n) ml = x == 0 ? pc.first_ml[item] : pc.more_ml[slot + (size_t)(x - 1) * mt];
+      constexpr int U = 8;  // pieces in flight
+      const int many = min(32, n - x0);
+      float was = 0.f, wx = 0.f;
+      for (int y = 0; y < many; y += U) {
+        float v[U][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] *= was;
-    m = to;
-    const int many = min(32, n - x0);
-    constexpr int U = 8;  // pieces in flight
-    for (int y = 0; y < many; y += U) {
-      float v[U][E];
+        for (int u = 0; u < U; ++u) {
+          const int z = x0 + y + u;
+          const bool on = y + u < many;
+          const float* p = (z == 0 ? pc.first_o + (size_t)item * HD : pc.more_o + (slot + (size_t)(on ? z - 1 : 0) * mt) * HD) +
+                           lane * E;
+          if constexpr (E == 4) {
+            const float4 f = on ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
+          } else {
+            const float2 f = on ? *reinterpret_cast<const float2*>(p) : make_float2(0.f, 0.f);
+            v[u][0] = f.x, v[u][1] = f.y;
+          }
+        }
+        if (y == 0) {  // with the first loads on their way
+          const float to = fmaxf(m, warp_max(ml.x)), base = to == -INFINITY ? 0.f : to;
+          was = ex2f(m - base), wx = ex2f(ml.x - base);
+          l = l * was + warp_sum(ml.y * wx);  // a NaN among the sums stays one
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool on = y + u < many;
-        const float* p = o_of(x0 + (on ? y + u : 0)) + lane * E;
-        if constexpr (E == 4) {
-          const float4 f = on ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
-          v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
-        } else {
-          const float2 f = on ? *reinterpret_cast<const float2*>(p) : make_float2(0.f, 0.f);
-          v[u][0] = f.x, v[u][1] = f.y;
+          for (int e = 0; e < E; ++e) o[e] *= was;
+          m = to;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float wu = __shfl_sync(0xffffffffu, wx, (y + u) & 31);
+          if (y + u < many)
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = fmaf(v[u][e], wu, o[e]);
         }
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float wu = __shfl_sync(0xffffffffu, wx, (y + u) & 31);
-        if (y + u < many)
-#pragma unroll
-          for (int e = 0; e < E; ++e) o[e] = fmaf(v[u][e], wu, o[e]);
-      }
     }
+  };
+  pdl_wait();
+  if (s.ok) {
+    const int64_t T = w.starts[a.p.n_seqs], x0 = w.starts[i] + x_own;
+    if (a.shared_len > 0) take(w.shared, slot_shared, w.shared_mt, 1 + more_shared);
+    const int more = more_of(w.own_mt, kt_own, w.own_workers, T, x0, r_own, slot_own);
+    if (a.shared_len == 0 && more == 0) return;  // one worker had the segment whole and wrote it
+    take(w.own, slot_own, w.own_mt, 1 + more);
   }
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // no key seen: zeros; NaN stays
+  bf16* dst = a.out + (size_t)item * HD + lane * E;
   uint32_t u[E / 2];
 #pragma unroll
   for (int e = 0; e < E / 2; ++e) {

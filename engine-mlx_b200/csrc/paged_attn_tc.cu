@@ -446,31 +446,53 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&B.p_full[g]);
         ++mine_n;
       }
-      // ---- the segment's pieces
-      float* dst;
+      // ---- the segment's pieces.  A thread has a row, and 32 rows 512 bytes apart would make 32 separate stores of 16
+      // bytes of one instruction: a warp turns its 32 rows x 64 columns in shared memory (where its rows of Q were) and
+      // stores two rows' 256 bytes at a time.
       const bool first = wk.whole_first;
       const size_t at = first ? head : (size_t)worker * kTcRows + (pair ? 128 * g : 0) + r;
-      dst = (first ? w.shared.first_o : w.shared.more_o) + at * HD;
-      float2* ml = (first ? w.shared.first_ml : w.shared.more_ml) + at;
+      float* const pieces = first ? w.shared.first_o : w.shared.more_o;
+      float2* const ml = (first ? w.shared.first_ml : w.shared.more_ml) + at;
+      float* const turn = reinterpret_cast<float*>(smem + L::kQ + g * L::kTile) + (warp & 3) * 32 * (HD / 2);
+      const unsigned rows_here = __ballot_sync(0xffffffffu, mine);
+      auto put_columns = [&](const float(&v)[32], int part) {  // 32 of the HD / 2 columns staged at once
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<float4*>(turn + lane * (HD / 2) + (((part * 8 + e) ^ (lane & (HD / 8 - 1))) << 2)) =
+              make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+      };
+      auto store_columns = [&](int c0) {  // columns c0 .. c0 + HD / 2 of this warp's rows
+        constexpr int kLanes = HD / 8;    // of a row
+        __syncwarp();
+#pragma unroll 4
+        for (int i = 0; i < kLanes; ++i) {
+          const int x = i * (32 / kLanes) + lane / kLanes, c = lane % kLanes;
+          const size_t to = __shfl_sync(0xffffffffu, (unsigned long long)at, x);
+          const float4 v = *reinterpret_cast<const float4*>(turn + x * (HD / 2) + ((c ^ (x & (HD / 8 - 1))) << 2));
+          if (rows_here >> x & 1u) *reinterpret_cast<float4*>(pieces + to * HD + c0 + 4 * c) = v;
+        }
+        __syncwarp();
+      };
       if (pair) {
         wait(&B.o_full[g], o_parity >> g & 1);
         o_parity ^= 3;
         tfence_after();
         if (busy) {
 #pragma unroll
-          for (int c = 0; c < HD / 32; ++c) {
-            float v[32];
-            tld32(tS + 256 + 32 * c, v);
-            wait_ld(v);
-            if (mine) {
+          for (int half = 0; half < 2; ++half) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                reinterpret_cast<float4*>(dst + 32 * c)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            for (int c = 0; c < HD / 64; ++c) {
+              float v[32];
+              tld32(tS + 256 + half * (HD / 2) + 32 * c, v);
+              wait_ld(v);
+              put_columns(v, c);
             }
+            store_columns(half * (HD / 2));
           }
           if (mine) *ml = make_float2(m, l);
         }
         tfence_before();
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory");  // the group's next Q comes where the rows were turned
       } else {
         // both groups have these rows: each joins one half of the columns
         // (maxima and sums meet where the Q tiles were: a group's last S is done, so all of its Q has been written and read)
@@ -480,9 +502,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (wk.n > 1) wait(&B.o_full[1], o_parity >> 1 & 1);
         o_parity ^= wk.n > 1 ? 3u : 1u;
         asm volatile("bar.sync 1, 256;" ::: "memory");
+        const float2 x = *mls(0), y = wk.n > 1 ? *mls(1) : make_float2(-INFINITY, 0.f);
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // both have read them: the places may be used again
         tfence_after();
         if (busy) {
-          const float2 x = *mls(0), y = wk.n > 1 ? *mls(1) : make_float2(-INFINITY, 0.f);
           const float to = fmaxf(x.x, y.x), b = to == -INFINITY ? 0.f : to;
           const float wx = ex2f(x.x - b), wy = ex2f(y.x - b);
           const uint32_t tO = tmem + lanes + 256 + g * (HD / 2);
@@ -498,17 +521,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               u[i] *= wx;
               if (wk.n > 1) u[i] = fmaf(v[i], wy, u[i]);  // group 1 without a tile: its O is not defined
             }
-            if (mine) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                reinterpret_cast<float4*>(dst + g * (HD / 2) + 32 * c)[e] =
-                    make_float4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
-            }
+            put_columns(u, c);
           }
+          store_columns(g * (HD / 2));
           if (mine && g == 0) *ml = make_float2(to, x.y * wx + y.y * wy);
         }
         tfence_before();
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // both have read both
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // both have read both O
       }
     } while (wk.next(line));
   }

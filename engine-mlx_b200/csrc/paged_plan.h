@@ -54,8 +54,13 @@ EMX_HD uint32_t cache_row(int page, int n_kv, int h, int page_size, int off) {
 // the batch's T; worker c takes [c per, (c + 1) per) of them, so no worker of
 // the first ceil(T / per) is without work and tile x is worker x / per's.
 EMX_HD int64_t share_size(int64_t T, int workers, int least) {
-  const int64_t per = (T + workers - 1) / workers;
+  const int64_t up = T + workers - 1;
+  const int64_t per = up >> 32 ? up / workers : (int64_t)((uint32_t)up / (uint32_t)workers);
   return per > least ? per : least;
+}
+// x / per, by the short 32-bit division wherever both fit it.
+EMX_HD int share_of(int64_t x, int64_t per) {
+  return (x | per) >> 32 ? (int)(x / per) : (int)((uint32_t)x / (uint32_t)per);
 }
 
 // The line of key tiles of one part of a batch's positions: the common prefix

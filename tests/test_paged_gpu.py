@@ -190,11 +190,23 @@ def test_sequences_out_of_order_give_zeros_and_a_status(ctx, shared):
     assert c.status == 0
 
 
-def test_the_same_call_gives_the_same_bits(ctx):
-    c = Case(13, [1, 2, 1, 1] * 8, [400 + 13 * i for i in range(32)], 8, 2, shared=256).device(ctx)
+@pytest.mark.parametrize("seqs,n_q,n_kv,shared", [(32, 8, 2, 256), (300, 8, 8, 144), (300, 8, 8, 128), (70, 64, 8, 2080),
+                                                  (40, 32, 4, 8192)])
+def test_the_same_call_gives_the_same_bits(ctx, seqs, n_q, n_kv, shared):
+    r = np.random.default_rng(seqs)
+    rows = r.choice([0, 1, 1, 2], seqs)
+    c = Case(13, rows, shared + rows + r.integers(0, 300, seqs), n_q, n_kv, shared=shared).device(ctx)
     first = attend(ctx, c)
-    for _ in range(3):
+    for _ in range(20):
         assert (attend(ctx, c) == first).all()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+@pytest.mark.parametrize("seqs", [3, 40])
+def test_scales_that_are_not_positive(ctx, scale, seqs):
+    c = Case(26, [1, 2] + [1] * seqs, [200, 90] + [130] * seqs, 8, 2, shared=64)
+    c.scale = scale
+    check_attend(c, attend(ctx, c.device(ctx)))
 
 
 def test_one_sequence_equals_the_static_cache(ctx):
