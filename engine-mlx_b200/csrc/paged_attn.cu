@@ -26,6 +26,9 @@ namespace {
 constexpr int kKT = 16;       // keys of a tile
 constexpr int kWarps = 4;     // workers of a CTA
 constexpr int kStages = 3;    // tiles in flight a worker
+// Units of a segment's set-up (q, its pieces): a worker's share of 14 one-tile
+// segments took 38 us where 14 tiles of one or two segments took 23.
+constexpr int kSetup = 1;
 constexpr int kMaxSeqs = 1024;
 constexpr int kCtasPerSm = 2;
 
@@ -60,7 +63,7 @@ __device__ __forceinline__ void plan_starts(const PagedAttnArgs& a, const Line& 
   for (int i = i0; i < i1; ++i) {
     const SeqInfo s = line.seq(i);
     if (!s.ok && report) report_status(a.p.status, seq_status(a.p, i));
-    const int64_t t = line.tiles(s);
+    const int64_t t = line.units(s);
     starts[i] = t;
     sum += t;
   }
@@ -147,31 +150,32 @@ struct Worker {
     }
   }
 
-  __device__ __forceinline__ void run(int64_t total, int worker, int64_t per) const;
+  __device__ __forceinline__ void run(int worker, int64_t x0, int64_t x1) const;
 };
 
-// The share of `worker`, `per` tiles of the line's `total`.
+// The tiles among units [x0, x1) of the line.
 template <int HD, int NT, bool SHARED>
-__device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int64_t total, int worker, int64_t per) const {
+__device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int worker, int64_t x0, int64_t x1) const {
   const PagedAttnArgs& a = w.a;
   const Pieces& pc = SHARED ? w.shared : w.own;
-  const int64_t x0 = worker * per;
-  if (x0 >= total) return;
-  const int n = (int)min(per, total - x0);
   Cursor ld, cc;
   const int hpg = line.hpg;
   cc.seek(line, x0);
+  if (cc.x >= x1) return;  // nothing but a set-up
   ld = cc;
   Key key = key_of(ld);
-  int loaded = 0;  // tiles begun
+  int loaded = 0;  // stage of the next load
   auto load = [&]() {
-    if (loaded < n) {
-      issue(loaded % kStages, key, ld.head());
-      if (++loaded < n) {
+    if (ld.x < x1) {
+      issue(loaded, key, ld.head());
+      if (ld.x + 1 < x1) {
         ld.next(line);
-        key = key_of(ld);
+        if (ld.x < x1) key = key_of(ld);
+      } else {
+        ld.x = x1;
       }
     }
+    loaded = loaded + 1 == kStages ? 0 : loaded + 1;
     cp_commit();
   };
 #pragma unroll 1
@@ -187,7 +191,7 @@ __device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int64_t total, int w
   int least = 0;   // fewest of them over the tile's rows
   bool fresh = true, whole = false;
   int R = 0, row_base = 0, h = 0;
-  for (int t = 0; t < n; ++t) {
+  for (int stage = 0;; stage = stage + 1 == kStages ? 0 : stage + 1) {
     if (fresh) {
       // a segment begins for this worker: its rows of q, and how far they see
       fresh = false;
@@ -226,7 +230,6 @@ __device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int64_t total, int w
     load();
     cp_wait<kStages - 1>();
     __syncwarp();
-    const int stage = t % kStages;
     const uint32_t K = ring + stage * kStageB, V = K + kTileB;
     const uint32_t there = valid[stage];
     const int key0 = cc.k * kKT;  // within the part
@@ -354,7 +357,9 @@ __device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int64_t total, int w
     __syncwarp();  // the stage may be filled again
 
     const bool last = cc.k + 1 == cc.kt;
-    if (last || t + 1 == n) {
+    // the next tile is this worker's if its unit is; a segment's last is followed by a set-up
+    const bool more = cc.x + 1 + (last ? line.setup : 0) < x1;
+    if (last || !more) {
       // ---- this worker's piece of the segment
       const bool direct = whole && last && !SHARED && a.shared_len == 0;
 #pragma unroll
@@ -386,7 +391,8 @@ __device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int64_t total, int w
         }
       fresh = true;
     }
-    if (t + 1 < n) cc.next(line);
+    if (!more) break;
+    cc.next(line);
   }
   cp_wait<0>();
 }
@@ -398,43 +404,55 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const __grid_co
   __shared__ uint32_t valid[kWarps][kStages];
   using Wk = Worker<HD, NT, SHARED>;
   const int warp = threadIdx.x >> 5;
-  const Line line = make_line(w.a.p, w.a.shared_len, !SHARED, Wk::MT, kKT, starts);
+  const Line line = make_line(w.a.p, w.a.shared_len, !SHARED, Wk::MT, kKT, SHARED ? 0 : kSetup, starts);
+  // The first kernel of a call waits for what ran before it.  An own part that
+  // follows a shared one has been let go by it after such a wait; it needs
+  // nothing of that one, but the join waits for this kernel alone, so it ends
+  // after the other.
+  const bool first = SHARED || w.a.shared_len == 0;
+  if (first) pdl_wait();
   pdl_trigger();
   int64_t total;
   if (SHARED) {
-    total = line.tiles(line.seq(0));
+    total = line.units(line.seq(0));
   } else {
     plan_starts<kWarps * 32>(w.a, line, starts, blockIdx.x == 0);
     total = starts[w.a.p.n_seqs];
     if (blockIdx.x == 0)
       for (int i = threadIdx.x; i <= w.a.p.n_seqs; i += kWarps * 32) w.starts[i] = starts[i];
   }
-  if (total > 0) {
+  const int worker = blockIdx.x * kWarps + warp;
+  const int64_t per = SHARED ? w.shared_per : share_size(total, gridDim.x * kWarps, 1);
+  if (worker * per < total) {
     Wk k{w, line, (int)(threadIdx.x & 31), smem_u32(smem) + warp * (uint32_t)(kStages * Wk::kStageB), valid[warp]};
-    k.run(total, blockIdx.x * kWarps + warp, share_size(total, gridDim.x * kWarps, 1));
+    k.run(worker, worker * per, min(total, (worker + 1) * per));
   }
-  // The own part is launched while the shared one runs and needs nothing of
-  // it, but the join waits for this kernel alone: so it ends after the other.
-  if (!SHARED) pdl_wait();
+  if (!first) pdl_wait();
 }
 
 // One warp a (row, q head): joins its pieces.
 template <int HD>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedWork w) {
+__global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constant__ PagedWork w) {
   const PagedAttnArgs& a = w.a;
   const int lane = threadIdx.x & 31;
   const int item = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (item >= a.p.n_rows * a.p.n_q) return;
+  pdl_trigger();
+  if (item >= a.p.n_rows * a.p.n_q) {
+    pdl_wait();
+    return;
+  }
   // ---- before the pieces are there: whose row it is and where the shared part's pieces will be
   const int row = item / a.p.n_q, hq = item - row * a.p.n_q;
   const int hpg = a.p.n_q / a.p.n_kv, h = hq / hpg, g = hq - h * hpg;
   const int i = warp_find_seq(a.p.indptr, a.p.n_seqs, row);
-  if (i >= a.p.n_seqs || row < a.p.indptr[i]) return;  // behind the last sequence: left as it was
+  if (i >= a.p.n_seqs || row < a.p.indptr[i]) {  // behind the last sequence: left as it was
+    pdl_wait();  // (every CTA waits, so that what follows this kernel follows the ones before it)
+    return;
+  }
   const SeqInfo s = load_seq(a.p, i, a.shared_len);
   constexpr int E = HD / 32;
   // the slot of a segment's second worker, and how many follow the first
-  auto more_of = [&](int mt, int kt, int workers, int64_t T, int64_t x0, int r, size_t& slot) {
-    const int64_t per = share_size(T, workers, 1);
+  auto more_of = [&](int mt, int kt, int64_t per, int64_t x0, int r, size_t& slot) {
     const int c0 = share_of(x0, per), c1 = share_of(x0 + kt - 1, per);
     slot = (size_t)(c0 + 1) * mt + r % mt;
     return c1 - c0;
@@ -442,15 +460,16 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   size_t slot_shared = 0, slot_own = 0;
   int more_shared = 0;
   if (s.ok && a.shared_len > 0) {
-    const Line all = make_line(a.p, a.shared_len, false, w.shared_mt, w.shared_keys, nullptr);
+    const Line all = make_line(a.p, a.shared_len, false, w.shared_mt, w.shared_keys, 0, nullptr);
     const SeqInfo every = all.seq(0);
-    const int r = row * hpg + g, kt = all.key_tiles(every);
-    more_shared = more_of(w.shared_mt, kt, w.shared_workers, all.tiles(every),
-                          ((int64_t)h * all.row_tiles(every) + r / w.shared_mt) * kt, r, slot_shared);
+    const int r = row * hpg + g, kt = all.key_tiles(every), seg = h * all.row_tiles(every) + r / w.shared_mt;
+    // with workers of their own, segments are as long as those workers' shares
+    const int64_t begin = (int64_t)seg * (w.shared_split ? (int64_t)w.shared_split * w.shared_per : kt);
+    more_shared = more_of(w.shared_mt, kt, w.shared_per, begin, r, slot_shared);
   }
-  const Line own = make_line(a.p, a.shared_len, true, w.own_mt, w.own_keys, w.starts);
+  const Line own = make_line(a.p, a.shared_len, true, w.own_mt, w.own_keys, kSetup, w.starts);
   const int r_own = (row - s.row0) * hpg + g, kt_own = own.key_tiles(s);
-  const int64_t x_own = ((int64_t)h * own.row_tiles(s) + r_own / w.own_mt) * kt_own;
+  const int64_t x_own = ((int64_t)h * own.row_tiles(s) + r_own / w.own_mt) * (kt_own + kSetup) + kSetup;
 
   float o[E];
 #pragma unroll
@@ -503,7 +522,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   if (s.ok) {
     const int64_t T = w.starts[a.p.n_seqs], x0 = w.starts[i] + x_own;
     if (a.shared_len > 0) take(w.shared, slot_shared, w.shared_mt, 1 + more_shared);
-    const int more = more_of(w.own_mt, kt_own, w.own_workers, T, x0, r_own, slot_own);
+    const int more = more_of(w.own_mt, kt_own, share_size(T, w.own_workers, 1), x0, r_own, slot_own);
     if (a.shared_len == 0 && more == 0) return;  // one worker had the segment whole and wrote it
     take(w.own, slot_own, w.own_mt, 1 + more);
   }
@@ -545,29 +564,15 @@ size_t lay_out(PagedWork& w, int num_sms, unsigned char* base) {
   return off;
 }
 
-// `overlap`: the launch may begin while the kernel before it runs.
-void launch_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& at, unsigned grid, int threads, int smem, cudaStream_t st,
-                          bool overlap) {
-  cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = overlap ? 1 : 0;
-}
-
 template <int HD, int NT, bool SHARED>
-cudaError_t launch_part(const PagedWork& w, int workers, cudaStream_t st, bool overlap) {
+cudaError_t launch_part(const PagedWork& w, int workers, cudaStream_t st) {
   const int smem = kWarps * kStages * Worker<HD, NT, SHARED>::kStageB;
   static cudaError_t once = cudaFuncSetAttribute(paged_attn_kernel<HD, NT, SHARED>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (once != cudaSuccess) return once;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute at;
-  launch_config(cfg, at, workers / kWarps, kWarps * 32, smem, st, overlap);
+  overlapped(cfg, at, workers / kWarps, kWarps * 32, smem, st);
   return cudaLaunchKernelEx(&cfg, paged_attn_kernel<HD, NT, SHARED>, w);
 }
 
@@ -579,27 +584,38 @@ cudaError_t launch(PagedWork& w, int num_sms, cudaStream_t st) {
   w.own_keys = kKT;
   cudaError_t e = cudaSuccess;
   if (w.a.shared_len > 0) {
-    if ((int64_t)p.n_rows * hpg > 32 && paged_shared_tc_takes(p)) {
-      w.shared_mt = kTcRows;
-      w.shared_keys = kTcKeys;
-      w.shared_workers = num_sms;
-      e = paged_shared_tc_launch(w, num_sms, st);
-    } else {
-      w.shared_mt = (int64_t)p.n_rows * hpg > 16 ? 32 : 16;
-      w.shared_keys = kKT;
-      e = w.shared_mt == 32 ? launch_part<HD, 2, true>(w, w.shared_workers, st, false)
-                            : launch_part<HD, 1, true>(w, w.shared_workers, st, false);
+    const int64_t rows = (int64_t)p.n_rows * hpg;
+    const bool tc = rows > 32 && paged_shared_tc_takes(p);
+    w.shared_mt = tc ? kTcRows : rows > 16 ? 32 : 16;
+    w.shared_keys = tc ? kTcKeys : kKT;
+    if (tc) w.shared_workers = num_sms;
+    const int kt = ceil_div(w.a.shared_len, w.shared_keys);
+    const int64_t segments = (int64_t)p.n_kv * ((rows + w.shared_mt - 1) / w.shared_mt);
+    w.shared_per = (int)share_size(segments * kt, w.shared_workers, 1);
+    w.shared_split = 0;
+    if (tc && segments <= w.shared_workers) {
+      // A worker that goes from one segment to the next stores one's rows and
+      // loads the other's Q with nothing to compute meanwhile: about four
+      // tiles' time.  Whole workers to a segment where the tiles that costs are
+      // fewer (64 rows a head on 32768: 15 tiles against 14 and a change).
+      const int split = (int)(w.shared_workers / segments), per = ceil_div(kt, split);
+      if (per <= w.shared_per + 4) {
+        w.shared_split = split;
+        w.shared_per = per;
+      }
     }
+    e = tc                   ? paged_shared_tc_launch(w, num_sms, st)
+        : w.shared_mt == 32 ? launch_part<HD, 2, true>(w, w.shared_workers, st)
+                            : launch_part<HD, 1, true>(w, w.shared_workers, st);
     if (e != cudaSuccess) return e;
   }
-  const bool after = w.a.shared_len > 0;
-  e = w.own_mt == 32 ? launch_part<HD, 2, false>(w, w.own_workers, st, after)
-                     : launch_part<HD, 1, false>(w, w.own_workers, st, after);
+  e = w.own_mt == 32 ? launch_part<HD, 2, false>(w, w.own_workers, st)
+                     : launch_part<HD, 1, false>(w, w.own_workers, st);
   if (e != cudaSuccess) return e;
   const int64_t items = (int64_t)p.n_rows * p.n_q;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute at;
-  launch_config(cfg, at, (unsigned)((items + 3) / 4), 128, 0, st, true);
+  overlapped(cfg, at, (unsigned)((items + 3) / 4), 128, 0, st);
   return cudaLaunchKernelEx(&cfg, paged_join_kernel<HD>, static_cast<const PagedWork>(w));
 }
 

@@ -22,7 +22,26 @@ struct PagedWork {
   int own_workers, shared_workers;
   int own_mt, shared_mt;      // rows of a tile
   int own_keys, shared_keys;  // positions of a tile
+  // Shares of the shared part (its sizes are known to the host): `shared_per`
+  // tiles each, in one line, or (shared_split > 0) shared_split workers to each
+  // segment, so that none has tiles of two.
+  int shared_per, shared_split;
 };
+
+// A launch that may begin while the kernel before it in the stream still runs:
+// the kernel waits (pdl_wait) before it reads or writes anything but its own
+// shared and tensor memory.
+inline void overlapped(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& at, unsigned grid, int threads, int smem, cudaStream_t st) {
+  cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+}
 
 // The shared part of a batch of many rows, on tcgen05 (paged_attn_tc.cu):
 // tiles of kTcRows rows and kTcKeys positions, one worker a CTA.

@@ -118,11 +118,22 @@ struct Walk {
   int n;     // tiles of this segment in the share
   int rows;  // rows of this segment's 256
   bool whole_first;  // its first tile is in the share
-  __device__ __forceinline__ bool begin(const Line& line, int64_t total, int worker, int64_t per) {
-    const int64_t x0 = worker * per;
-    if (x0 >= total) return false;
-    left = (int)min(per, total - x0);
-    c.seek(line, x0);
+  __device__ __forceinline__ bool begin(const Line& line, int worker, int per, int split) {
+    c.seq = 0;
+    c.enter(line);
+    const int segments = c.mt * line.n_kv;
+    if (split) {  // this many workers to a segment
+      c.seg = worker / split;
+      c.k = (worker - c.seg * split) * per;
+      left = min(per, c.kt - c.k);
+      if (c.seg >= segments || left <= 0) return false;
+    } else {
+      const int64_t x0 = (int64_t)worker * per, total = (int64_t)segments * c.kt;
+      if (x0 >= total) return false;
+      left = (int)min((int64_t)per, total - x0);
+      c.seg = share_of(x0, c.kt);
+      c.k = (int)(x0 - (int64_t)c.seg * c.kt);
+    }
     enter(line);
     return true;
   }
@@ -154,35 +165,41 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* status = a.p.status;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  // The loader sets the barriers up and begins: it needs no tensor memory.
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      for (int s = 0; s < kSlots; ++s) {
+        mbar_init(&B.full[s], 1);
+        mbar_init(&B.empty[s], 2);
+      }
+      for (int g = 0; g < 2; ++g) {
+        mbar_init(&B.q_full[g], 128);
+        mbar_init(&B.s_full[g], 2);
+        mbar_init(&B.p_full[g], 128);
+        mbar_init(&B.o_full[g], 1);
+        mbar_init(&B.turn[g], 1);
+      }
+      fence_mbar_init();
+    }
+    __syncwarp();
+    asm volatile("bar.arrive 4, %0;" ::"n"(kThreads) : "memory");
+  } else {
+    if (warp == kMmaWarp) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&B.tmem)), "r"(kCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tfence_before();
+    asm volatile("bar.sync 4, %0;" ::"n"(kThreads) : "memory");
+    tfence_after();
+  }
+  pdl_wait();     // what ran before has written q, the cache and the batch
   pdl_trigger();  // the own part does not read what this one writes (it only ends after it)
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kSlots; ++s) {
-      mbar_init(&B.full[s], 1);
-      mbar_init(&B.empty[s], 2);
-    }
-    for (int g = 0; g < 2; ++g) {
-      mbar_init(&B.q_full[g], 128);
-      mbar_init(&B.s_full[g], 2);
-      mbar_init(&B.p_full[g], 128);
-      mbar_init(&B.o_full[g], 1);
-      mbar_init(&B.turn[g], 1);
-    }
-    fence_mbar_init();
-  }
-  if (warp == kMmaWarp) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&B.tmem)), "r"(kCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  tfence_before();
-  __syncthreads();
-  tfence_after();
-  const uint32_t tmem = B.tmem;
-  const Line line = make_line(a.p, a.shared_len, false, kTcRows, kTcKeys, nullptr);
-  const int64_t total = line.tiles(line.seq(0)), per = share_size(total, w.shared_workers, 1);
+  const uint32_t tmem = warp == kLoadWarp ? 0u : B.tmem;
+  const Line line = make_line(a.p, a.shared_len, false, kTcRows, kTcKeys, 0, nullptr);
   const int worker = blockIdx.x;
   Walk wk;
-  const bool any = wk.begin(line, total, worker, per);
+  const bool any = wk.begin(line, worker, w.shared_per, w.shared_split);
   // a wait that gave up leaves `ok` false: later waits are skipped, the work runs out on whatever is there
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && mbar_wait_bounded(bar, parity, status); };
@@ -349,14 +366,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tok = mine ? (base + r) / line.hpg : 0;
       const size_t head = (size_t)tok * a.p.n_q + h * line.hpg + (mine ? base + r - tok * line.hpg : 0);
       const bool busy = base + (r & ~31) < R;  // some row of this warp is there
+      const unsigned rows_here = __ballot_sync(0xffffffffu, mine);
       {
+        // this warp's 32 rows of q, two (at D = 64 four) at a time
         unsigned char* Q = smem + L::kQ + g * L::kTile;
-        const uint4* src = reinterpret_cast<const uint4*>(a.q + head * HD);
+        constexpr int kLanes = HD / 8;  // of a row
+        const int c = lane % kLanes;
+        uint4 v[kLanes];
 #pragma unroll
-        for (int c = 0; c < HD / 8; ++c) {
-          uint4 v = mine ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-          v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-          *reinterpret_cast<uint4*>(Q + tile_at(r, c)) = v;
+        for (int i = 0; i < kLanes; ++i) {
+          const int x = i * (32 / kLanes) + lane / kLanes;
+          const size_t from = __shfl_sync(0xffffffffu, (unsigned long long)head, x);
+          v[i] = rows_here >> x & 1u ? *reinterpret_cast<const uint4*>(a.q + from * HD + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < kLanes; ++i) {
+          const int x = i * (32 / kLanes) + lane / kLanes;
+          v[i].x ^= flip, v[i].y ^= flip, v[i].z ^= flip, v[i].w ^= flip;
+          *reinterpret_cast<uint4*>(Q + tile_at((warp & 3) * 32 + x, c)) = v[i];
         }
         fence_proxy_async();
         mbar_arrive(&B.q_full[g]);
@@ -454,7 +481,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       float* const pieces = first ? w.shared.first_o : w.shared.more_o;
       float2* const ml = (first ? w.shared.first_ml : w.shared.more_ml) + at;
       float* const turn = reinterpret_cast<float*>(smem + L::kQ + g * L::kTile) + (warp & 3) * 32 * (HD / 2);
-      const unsigned rows_here = __ballot_sync(0xffffffffu, mine);
       auto put_columns = [&](const float(&v)[32], int part) {  // 32 of the HD / 2 columns staged at once
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -573,8 +599,10 @@ cudaError_t launch(const PagedWork& w, int num_sms, cudaStream_t st) {
   cudaError_t e = encode(&tk, w.a.p, w.a.p.k, box);
   if (e == cudaSuccess) e = encode(&tv, w.a.p, w.a.p.v, box);
   if (e != cudaSuccess) return e;
-  paged_shared_tc_kernel<HD><<<num_sms, kThreads, Smem<HD>::kBytes, st>>>(tk, tv, w, box);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute at;
+  overlapped(cfg, at, (unsigned)num_sms, kThreads, Smem<HD>::kBytes, st);
+  return cudaLaunchKernelEx(&cfg, paged_shared_tc_kernel<HD>, tk, tv, w, box);
 }
 
 }  // namespace

@@ -8,9 +8,9 @@ __device__ __forceinline__ SeqInfo load_seq(const PagedArgs& p, int i, int share
   return seq_info(p.indptr[i], p.indptr[i + 1], p.lengths[i], p.n_rows, shared, (int64_t)p.max_pages * p.page_size);
 }
 
-__device__ __forceinline__ Line make_line(const PagedArgs& p, int shared_len, bool own, int mt, int keys,
+__device__ __forceinline__ Line make_line(const PagedArgs& p, int shared_len, bool own, int mt, int keys, int setup,
                                           const int64_t* starts) {
-  return Line{own, p.n_seqs, p.n_rows, p.n_kv, p.n_q / p.n_kv, shared_len, mt, keys, (int64_t)p.max_pages * p.page_size,
+  return Line{own, p.n_seqs, p.n_rows, p.n_kv, p.n_q / p.n_kv, shared_len, mt, keys, setup, (int64_t)p.max_pages * p.page_size,
               p.indptr, p.lengths, starts};
 }
 

@@ -50,9 +50,11 @@ EMX_HD uint32_t cache_row(int page, int n_kv, int h, int page_size, int off) {
 }
 
 // Segments: (KV head, row tile) pairs of one sequence, row tiles innermost,
-// each of `kt` key tiles.  Tiles of sequence i are [start_i, start_{i+1}) of
-// the batch's T; worker c takes [c per, (c + 1) per) of them, so no worker of
-// the first ceil(T / per) is without work and tile x is worker x / per's.
+// each of `kt` key tiles and, before them, `setup` units for what a segment
+// costs its worker besides its tiles.  Units of sequence i are [start_i,
+// start_{i+1}) of the batch's T; worker c takes the tiles among units [c per,
+// (c + 1) per), so the tile at unit x is worker x / per's, and the workers of a
+// segment's tiles follow one another.
 EMX_HD int64_t share_size(int64_t T, int workers, int least) {
   const int64_t up = T + workers - 1;
   const int64_t per = up >> 32 ? up / workers : (int64_t)((uint32_t)up / (uint32_t)workers);
@@ -69,11 +71,11 @@ EMX_HD int share_of(int64_t x, int64_t per) {
 // being one q head of one new token), key tiles `keys` positions.
 struct Line {
   bool own;
-  int n_seqs, n_rows, n_kv, hpg, shared_len, mt, keys;
+  int n_seqs, n_rows, n_kv, hpg, shared_len, mt, keys, setup;
   int64_t room;          // positions of a page table
   const int* indptr;
   const int* lengths;
-  const int64_t* starts;  // own: tiles before each sequence
+  const int64_t* starts;  // own: units before each sequence
 
   EMX_HD SeqInfo seq(int i) const {
     if (own) return seq_info(indptr[i], indptr[i + 1], lengths[i], n_rows, shared_len, room);
@@ -86,16 +88,17 @@ struct Line {
   }
   EMX_HD int row_tiles(const SeqInfo& s) const { return (int)(((int64_t)s.rows * hpg + mt - 1) / mt); }
   EMX_HD int key_tiles(const SeqInfo& s) const { return ceil_div(own ? s.len - shared_len : s.len, keys); }
-  EMX_HD int64_t tiles(const SeqInfo& s) const {
+  EMX_HD int64_t units(const SeqInfo& s) const {
     if (!s.ok || s.rows == 0) return 0;
-    return (int64_t)n_kv * row_tiles(s) * key_tiles(s);
+    return (int64_t)n_kv * row_tiles(s) * (key_tiles(s) + setup);
   }
 };
 
-// Where a worker stands in a line.
+// Where a worker stands in a line: at a tile, or behind the last one.
 struct Cursor {
   int seq, seg, k;  // sequence, segment within it, key tile within that
   int mt, kt;       // row tiles a KV head, key tiles a segment
+  int64_t x;        // the tile's unit
   SeqInfo s;
 
   EMX_HD void enter(const Line& line) {
@@ -103,27 +106,34 @@ struct Cursor {
     mt = line.row_tiles(s);
     kt = line.key_tiles(s);
   }
-  // To tile x < T.
-  EMX_HD void seek(const Line& line, int64_t x) {
+  // To the first tile at or behind unit `to` < T.
+  EMX_HD void seek(const Line& line, int64_t to) {
     seq = 0;
+    int64_t at = 0;
     if (line.own) {
-      int lo = 0, hi = line.n_seqs - 1;  // the last sequence that begins at or before x
+      int lo = 0, hi = line.n_seqs - 1;  // the last sequence that begins at or before it
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (line.starts[mid] <= x) lo = mid;
+        if (line.starts[mid] <= to) lo = mid;
         else hi = mid - 1;
       }
       seq = lo;
-      x -= line.starts[lo];
+      at = line.starts[lo];
     }
     enter(line);
-    seg = (int)(x / kt);
-    k = (int)(x - (int64_t)seg * kt);
+    const int each = kt + line.setup;
+    seg = share_of(to - at, each);
+    at += (int64_t)seg * each;
+    k = (int)(to - at) - line.setup;
+    if (k < 0) k = 0;
+    x = at + line.setup + k;
   }
-  // To the next tile; the caller does not go past the last one.
+  // To the next tile; the caller does not go on from the last one's unit T - 1.
   EMX_HD void next(const Line& line) {
+    ++x;
     if (++k < kt) return;
     k = 0;
+    x += line.setup;
     if (++seg < mt * line.n_kv || !line.own) return;
     seg = 0;
     do ++seq;

@@ -101,63 +101,64 @@ HARNESS = r"""
 #include "paged_plan.h"
 #include <stdio.h>
 using namespace emx;
-// Walks every worker's share of the line the way the kernel does.  seen[x] counts tile x = (segment, key tile) in line
-// order; pieces[segment] gets the pieces written (first, more); returns 0, or where an index left its range.
-extern "C" int walk(int own, int n_seqs, int n_rows, int n_kv, int hpg, int shared, int mt, int keys, long room,
-                    const int* indptr, const int* lengths, int64_t* starts, int workers, int least, int* seen, long n_seen, int* pieces) {
-  Line line{own != 0, n_seqs, n_rows, n_kv, hpg, shared, mt, keys, room, indptr, lengths, starts};
-  int64_t T = 0;
-  if (own) {
-    for (int i = 0; i < n_seqs; ++i) { starts[i] = T; T += line.tiles(line.seq(i)); }
-    starts[n_seqs] = T;
-  } else {
-    T = line.tiles(line.seq(0));
+// Walks every worker's share of the line the way the kernel does.  seen[] counts the tiles in line order, pieces[] (at a
+// segment's first tile) the pieces written of it; returns 0, or where an index left its range.
+extern "C" int walk(int own, int n_seqs, int n_rows, int n_kv, int hpg, int shared, int mt, int keys, int setup, long room,
+                    const int* indptr, const int* lengths, int64_t* starts, int workers, int least, int* seen, long n_seen,
+                    int* pieces) {
+  Line line{own != 0, n_seqs, n_rows, n_kv, hpg, shared, mt, keys, setup, room, indptr, lengths, starts};
+  int64_t T = 0, tiles = 0;
+  for (int i = 0; i < (own ? n_seqs : 1); ++i) {
+    const SeqInfo s = line.seq(i);
+    if (own) starts[i] = T;
+    const int64_t u = line.units(s);
+    T += u;
+    if (u) tiles += u / (line.key_tiles(s) + setup) * line.key_tiles(s);
   }
-  if (T != n_seen) return 1;
+  if (own) starts[n_seqs] = T;
+  if (tiles != n_seen) return 1;
   if (T == 0) return 0;
   const int64_t per = share_size(T, workers, least);
   if ((T + per - 1) / per > workers) return 13;
+  int64_t at = 0;  // tiles seen: workers follow the line
   for (int c = 0; c < workers; ++c) {
     const int64_t x0 = c * per, x1 = x0 + per < T ? x0 + per : T;
-    if (x1 <= x0) continue;
+    if (x0 >= T) continue;
     Cursor cur;
     cur.seek(line, x0);
+    if (cur.x >= x1) continue;
     bool fresh = true, whole = false;
-    int more = 0;
-    for (int64_t x = x0; x < x1; ++x) {
+    int more_pieces = 0;
+    for (;;) {
       if (cur.seq < 0 || (own && cur.seq >= n_seqs)) return 2;
       if (!cur.s.ok || cur.s.rows <= 0 || cur.s.row0 < 0 || cur.s.row0 + cur.s.rows > n_rows) return 3;
       if (cur.k < 0 || cur.k >= cur.kt || cur.seg < 0 || cur.seg >= cur.mt * n_kv) return 4;
       if (cur.head() < 0 || cur.head() >= n_kv) return 5;
       const int row = (cur.seg - cur.head() * cur.mt) * mt;
       if (row >= cur.s.rows * hpg) return 6;
-      const int64_t before = own ? starts[cur.seq] : 0;
-      if (before + (int64_t)cur.seg * cur.kt + cur.k != x) return 7;
+      const int64_t seg0 = (own ? starts[cur.seq] : 0) + (int64_t)cur.seg * (cur.kt + setup) + setup;
+      if (seg0 + cur.k != cur.x || cur.x < x0 || cur.x >= x1) return 7;
       const int first_pos = (own ? shared : 0) + cur.k * keys;
       if (first_pos >= cur.s.len) return 8;  // every tile has a position
-      seen[x]++;
+      if (at >= n_seen) return 14;
+      seen[at]++;
       if (fresh) { fresh = false; whole = cur.k == 0; }
-      if (cur.k + 1 == cur.kt || x + 1 == x1) {
+      const bool last = cur.k + 1 == cur.kt, more = cur.x + 1 + (last ? setup : 0) < x1;
+      if (last || !more) {
         // what the join will look for: the worker of the segment's first tile has the first piece
-        const int64_t s0 = before + (int64_t)cur.seg * cur.kt;
-        const int c0 = (int)(s0 / per), c1 = (int)((s0 + cur.kt - 1) / per);
+        const int c0 = share_of(seg0, per), c1 = share_of(seg0 + cur.kt - 1, per);
         if (whole ? c != c0 : !(c > c0 && c <= c1)) return 9;
-        if (!whole && ++more > 1) return 10;  // one slot a worker
-        pieces[x - cur.k + 0] += 1;           // counted at the segment's tile that the piece ends in
+        if (!whole && ++more_pieces > 1) return 10;  // one slot a worker
+        pieces[at - cur.k] += 1;
+        if (last && pieces[at - cur.k] != c1 - c0 + 1) return 12;
         fresh = true;
       }
-      if (x + 1 < x1) cur.next(line);
+      ++at;
+      if (!more) break;
+      cur.next(line);
     }
   }
-  // every share that reaches into a segment wrote exactly one piece of it
-  Cursor cur;
-  cur.seek(line, 0);
-  for (int64_t x = 0; x < T;) {
-    if (pieces[x] != (x + cur.kt - 1) / per - x / per + 1) return 12;
-    x += cur.kt;
-    if (x < T) for (int k = cur.kt; k > 0; --k) cur.next(line);
-  }
-  return 0;
+  return at == n_seen ? 0 : 15;
 }
 """
 
@@ -171,9 +172,9 @@ def walk(tmp_path_factory):
                     str(src), "-o", str(lib)], check=True)
     f = C.CDLL(str(lib)).walk
     f.restype = C.c_int
-    f.argtypes = [C.c_int] * 8 + [C.c_long] + [C.c_void_p] * 3 + [C.c_int, C.c_int, C.c_void_p, C.c_long, C.c_void_p]
+    f.argtypes = [C.c_int] * 9 + [C.c_long] + [C.c_void_p] * 3 + [C.c_int, C.c_int, C.c_void_p, C.c_long, C.c_void_p]
 
-    def run(own, indptr, lengths, n_rows, n_kv, hpg, shared, mt, keys, room, workers, least=1):
+    def run(own, indptr, lengths, n_rows, n_kv, hpg, shared, mt, keys, room, workers, least=1, setup=0):
         indptr, lengths = np.asarray(indptr, np.int32), np.asarray(lengths, np.int32)
         n = len(lengths)
         total = 0
@@ -187,7 +188,7 @@ def walk(tmp_path_factory):
             total = n_kv * -(-n_rows * hpg // mt) * -(-shared // keys)
         seen, pieces = np.zeros(total + 1, np.int32), np.zeros(total + 1, np.int32)
         starts = np.zeros(n + 1, np.int64)
-        rc = f(own, n, n_rows, n_kv, hpg, shared, mt, keys, room, indptr.ctypes.data, lengths.ctypes.data, starts.ctypes.data,
+        rc = f(own, n, n_rows, n_kv, hpg, shared, mt, keys, setup, room, indptr.ctypes.data, lengths.ctypes.data, starts.ctypes.data,
                workers, least, seen.ctypes.data, total, pieces.ctypes.data)
         assert rc == 0, rc
         assert (seen[:total] == 1).all()
@@ -208,7 +209,7 @@ def test_every_tile_has_one_worker_and_every_piece_is_joined(walk, seed):
     for own in (0, 1):
         if own or (shared and indptr[-1]):
             walk(own, indptr, lens, int(indptr[-1]) + 3, n_kv, hpg, shared, int(r.choice([16, 32, 128])),
-                 int(r.choice([16, 64, 128])), 8192, int(r.choice([1, 7, 148, 1184])), int(r.choice([1, 4])))
+                 int(r.choice([16, 64, 128])), 8192, int(r.choice([1, 7, 148, 1184])), int(r.choice([1, 4])), int(r.choice([0, 1, 3])))
 
 
 @pytest.mark.parametrize("seed", range(40))
@@ -218,5 +219,5 @@ def test_batches_out_of_order_stay_in_range(walk, seed):
     n = int(r.integers(1, 12))
     indptr = r.integers(-3, 20, n + 1)
     lens = r.choice([-5, 0, 1, 20, 64, 100, 513, 2**31 - 1], n)
-    walk(1, indptr, lens, 15, 2, int(r.choice([1, 4])), int(r.choice([0, 64])), 16, 16, 512, int(r.choice([1, 148])))
+    walk(1, indptr, lens, 15, 2, int(r.choice([1, 4])), int(r.choice([0, 64])), 16, 16, 512, int(r.choice([1, 148])), 1, int(r.choice([0, 1])))
     walk(1, [0] * (n + 1), lens, 15, 2, 1, 0, 16, 16, 512, 148)
