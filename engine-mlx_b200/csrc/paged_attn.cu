@@ -10,10 +10,10 @@
 // prefix is read once for all rows of the batch, as one sequence whose rows
 // are every row, and the own parts once for their few rows.
 //
-// Workers.  A warp is a worker: it takes an even share of the key tiles (16
-// keys) of all segments — (sequence, KV head, tile of 16 or 32 rows) — in one
-// line (paged_plan.h), so lengths from one to the longest balance to within a
-// tile, without the host knowing them.  A share's pieces: a segment's first
+// Workers.  A worker — a warp with 16 rows and tiles of 16 keys, or a CTA with
+// 64 and 64 — takes an even share of the key tiles of all segments (sequence,
+// KV head, row tile) in one line (paged_plan.h), so lengths from one to the
+// longest balance to within a tile, without the host knowing them.  A share's pieces: a segment's first
 // tiles go to the piece slot of its rows, a share that begins inside a segment
 // to the slot of its worker; a second kernel joins the pieces of each row
 // (and a segment that one worker has whole is written by it).
@@ -23,9 +23,9 @@ namespace emx {
 
 namespace {
 
-constexpr int kKT = 16;       // keys of a tile
-constexpr int kWarps = 4;     // workers of a CTA
-constexpr int kStages = 3;    // tiles in flight a worker
+constexpr int kKT = 16;     // keys of one step of a warp
+constexpr int kWarps = 4;   // of a CTA
+constexpr int kStages = 3;  // tiles a worker keeps, two of them in flight
 // Units of a segment's set-up (q, its pieces): a worker's share of 14 one-tile
 // segments took 38 us where 14 tiles of one or two segments took 23.
 constexpr int kSetup = 1;
@@ -88,233 +88,158 @@ __device__ __forceinline__ void plan_starts(const PagedAttnArgs& a, const Line& 
   __syncthreads();
 }
 
-template <int HD, int NT, bool SHARED>
-struct Worker {
-  static constexpr int MT = 16 * NT;
-  static constexpr int kRowB = HD * 2;             // bytes of a cached row
-  static constexpr int kTileB = kKT * kRowB;       // one tile of K (or V)
-  static constexpr int kStageB = 2 * kTileB;
-  static constexpr int kChunks = HD / 8;           // 16-byte chunks of a row
-  static constexpr int kCopies = kKT * kChunks / 32;
+// K and V of 16 or 64 keys in shared memory: 16-byte chunk c of row r.  Rows of
+// a tile hit all banks of ldmatrix.
+template <int HD>
+__device__ __forceinline__ uint32_t at(int r, int c) {
+  return (uint32_t)(r * HD * 2 + ((c ^ (r & 7)) << 4));
+}
 
-  const PagedWork& w;
-  Line line;
-  int lane;
-  uint32_t ring;       // this warp's stages
-  uint32_t* valid;     // [kStages] bit j: key j of the tile is there
-
-  // 16-byte chunk c of row r: rows of a tile hit all banks of ldmatrix
-  static __device__ __forceinline__ uint32_t at(int r, int c) {
-    return (uint32_t)(r * kRowB + ((c ^ (r & 7)) << 4));
-  }
-
-  // The page of key `lane` (< 16) of the cursor's tile and its place there, -1
-  // behind the sequence's end.  Loaded a tile ahead of its use and not looked
-  // at before: a look would wait for it.
-  struct Key {
-    int page, off;
-  };
-  __device__ __forceinline__ Key key_of(const Cursor& c) const {
-    const PagedAttnArgs& a = w.a;
-    const int pos = (SHARED ? 0 : a.shared_len) + c.k * kKT + (lane & 15);
-    Key key{0, -1};
-    if (pos < c.s.len) {
-      const int pg = pos / a.p.page_size;
-      key.page = SHARED ? a.shared_pages[pg] : a.p.table[(size_t)c.seq * a.p.max_pages + pg];
-      key.off = pos - pg * a.p.page_size;
-    }
-    return key;
-  }
-
-  __device__ __forceinline__ void issue(int stage, const Key& key, int head) const {
-    const PagedAttnArgs& a = w.a;
-    uint32_t row = ~0u;  // cache row of key `lane`, where there is one
-    if (key.off >= 0) {
-      if (key.page >= 0 && key.page < a.p.n_pages) row = cache_row(key.page, a.p.n_kv, head, a.p.page_size, key.off);
-      else report_status(a.p.status, kDevBadPage);
-    }
-    const unsigned there = __ballot_sync(0xffffffffu, row != ~0u) & 0xffffu;
-    if (lane == 0) valid[stage] = there;
-    constexpr int kRows = 32 / kChunks;  // rows of one copy of the warp
-    const int sub = lane / kChunks, c = lane % kChunks;
-    const bf16 *kp = a.p.k + c * 8, *vp = a.p.v + c * 8;
-    const uint32_t dst = ring + stage * kStageB + at(sub, c);
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      const uint32_t src = __shfl_sync(0xffffffffu, row, i * kRows + sub);
-      const bool on = src != ~0u;
-      const size_t off = on ? (size_t)src * HD : 0;
-      const uint32_t to = (dst ^ (uint32_t)(((i * kRows) & 7) << 4)) + (uint32_t)(i * kRows * kRowB);  // at(i kRows + sub, c)
-      cp_async16(to, kp + off, on);
-      cp_async16(to + kTileB, vp + off, on);
-    }
-  }
-
-  __device__ __forceinline__ void run(int worker, int64_t x0, int64_t x1) const;
+// The page of a key and its place there, -1 where there is none.  Loaded ahead
+// of its use and not looked at before: a look would wait for it.
+struct Key {
+  int page, off;
 };
 
-// The tiles among units [x0, x1) of the line.
-template <int HD, int NT, bool SHARED>
-__device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int worker, int64_t x0, int64_t x1) const {
-  const PagedAttnArgs& a = w.a;
-  const Pieces& pc = SHARED ? w.shared : w.own;
-  Cursor ld, cc;
-  const int hpg = line.hpg;
-  cc.seek(line, x0);
-  if (cc.x >= x1) return;  // nothing but a set-up
-  ld = cc;
-  Key key = key_of(ld);
-  int loaded = 0;  // stage of the next load
-  auto load = [&]() {
-    if (ld.x < x1) {
-      issue(loaded, key, ld.head());
-      if (ld.x + 1 < x1) {
-        ld.next(line);
-        if (ld.x < x1) key = key_of(ld);
-      } else {
-        ld.x = x1;
+template <bool SHARED>
+__device__ __forceinline__ Key key_at(const PagedAttnArgs& a, const Cursor& c, int pos) {
+  Key key{0, -1};
+  if (pos < c.s.len) {
+    const int pg = pos / a.p.page_size;
+    key.page = SHARED ? a.shared_pages[pg] : a.p.table[(size_t)c.seq * a.p.max_pages + pg];
+    key.off = pos - pg * a.p.page_size;
+  }
+  return key;
+}
+
+// Its cache row, ~0 where there is none.
+__device__ __forceinline__ uint32_t key_row(const PagedAttnArgs& a, const Key& key, int head) {
+  if (key.off < 0) return ~0u;
+  if (key.page >= 0 && key.page < a.p.n_pages) return cache_row(key.page, a.p.n_kv, head, a.p.page_size, key.off);
+  report_status(a.p.status, kDevBadPage);
+  return ~0u;
+}
+
+// Copies 16 bytes of K and of V; row ~0 reads as zeros.
+template <int HD>
+__device__ __forceinline__ void copy_kv(const PagedAttnArgs& a, uint32_t to_k, uint32_t to_v, uint32_t row, int c) {
+  const bool on = row != ~0u;
+  const size_t off = (on ? (size_t)row * HD : 0) + c * 8;
+  cp_async16(to_k, a.p.k + off, on);
+  cp_async16(to_v, a.p.v + off, on);
+}
+
+// Sixteen rows of one segment, by a warp: q as MMA operands, the running
+// maximum and sum of each row and its O.
+template <int HD, bool SHARED>
+struct Rows {
+  uint32_t qf[HD / 16][4];
+  float o[HD / 8][4];
+  float m[2], l[2];
+  int vis[2];  // keys of this part that the row sees
+  int least;   // fewest of them over the rows
+  int R, base, h;
+
+  // Rows base .. base + 15 (of R) of the cursor's segment.
+  __device__ __forceinline__ void begin(const PagedWork& w, const Cursor& c, int hpg, int first_row) {
+    const PagedAttnArgs& a = w.a;
+    const int lane = threadIdx.x & 31, quad = lane >> 2, col = (lane & 3) * 2;
+    h = c.head();
+    base = first_row;
+    R = c.s.rows * hpg;
+    least = 0x7fffffff;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int r = base + quad + b * 8;
+      const bool on = r < R;
+      const int tok = r / hpg;
+      vis[b] = !on ? 0 : SHARED ? a.shared_len : c.s.len - c.s.rows + tok + 1 - a.shared_len;
+      if (on) least = min(least, vis[b]);
+      m[b] = -INFINITY;
+      l[b] = 0.f;
+      const bf16* qr = a.q + ((size_t)(c.s.row0 + (on ? tok : 0)) * a.p.n_q + h * hpg + (on ? r - tok * hpg : 0)) * HD;
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks) {
+        qf[ks][b] = on ? *reinterpret_cast<const uint32_t*>(qr + ks * 16 + col) : 0u;
+        qf[ks][b + 2] = on ? *reinterpret_cast<const uint32_t*>(qr + ks * 16 + col + 8) : 0u;
       }
     }
-    loaded = loaded + 1 == kStages ? 0 : loaded + 1;
-    cp_commit();
-  };
-#pragma unroll 1
-  for (int i = 0; i < kStages - 1; ++i) load();
-  const float sl2 = a.scale * kLog2e;
-  const float nothing = sl2 < 0.f ? INFINITY : -INFINITY;  // the score of a key that is not seen
-  const int quad = lane >> 2, col = (lane & 3) * 2;
+#pragma unroll
+    for (int d = 0; d < HD / 8; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, x));
+  }
 
-  uint32_t qf[NT][HD / 16][4];
-  float o[NT][HD / 8][4];
-  float m[NT][2], l[NT][2];
-  int vis[NT][2];  // keys of this part that the row sees
-  int least = 0;   // fewest of them over the tile's rows
-  bool fresh = true, whole = false;
-  int R = 0, row_base = 0, h = 0;
-  for (int stage = 0;; stage = stage + 1 == kStages ? 0 : stage + 1) {
-    if (fresh) {
-      // a segment begins for this worker: its rows of q, and how far they see
-      fresh = false;
-      whole = cc.k == 0;
-      h = cc.seg / cc.mt;
-      row_base = (cc.seg - h * cc.mt) * MT;
-      R = cc.s.rows * hpg;
-      least = 0x7fffffff;
+  // Sixteen keys, key0 of the part the first, rows r0 .. r0 + 15 of the tiles at K and V; bit j of `there`: key j is.
+  __device__ __forceinline__ void keys16(float sl2, uint32_t K, uint32_t V, int r0, int key0, uint32_t there) {
+    const int lane = threadIdx.x & 31, col = (lane & 3) * 2;
+    const float nothing = sl2 < 0.f ? INFINITY : -INFINITY;  // the score of a key that is not seen
+    float s[2][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int r = row_base + nt * 16 + quad + b * 8;
-          const bool on = r < R;
-          const int tok = r / hpg;
-          vis[nt][b] = !on ? 0 : SHARED ? a.shared_len : cc.s.len - cc.s.rows + tok + 1 - a.shared_len;
-          if (on) least = min(least, vis[nt][b]);
-          m[nt][b] = -INFINITY;
-          l[nt][b] = 0.f;
-          const bf16* qr = a.q + ((size_t)(cc.s.row0 + (on ? tok : 0)) * a.p.n_q + h * hpg + (on ? r - tok * hpg : 0)) * HD;
-#pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks) {
-            qf[nt][ks][b] = on ? *reinterpret_cast<const uint32_t*>(qr + ks * 16 + col) : 0u;
-            qf[nt][ks][b + 2] = on ? *reinterpret_cast<const uint32_t*>(qr + ks * 16 + col + 8) : 0u;
-          }
-        }
-#pragma unroll
-        for (int d = 0; d < HD / 8; ++d)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[nt][d][e] = 0.f;
-      }
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, x));
-    }
-    // ---- the next load, then this tile
-    load();
-    cp_wait<kStages - 1>();
-    __syncwarp();
-    const uint32_t K = ring + stage * kStageB, V = K + kTileB;
-    const uint32_t there = valid[stage];
-    const int key0 = cc.k * kKT;  // within the part
-
-    float s[NT][2][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][j][e] = 0.f;
+      for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) {
       uint32_t kf[4];  // keys 0-7 (dims lo, hi), keys 8-15 (dims lo, hi)
-      ldsm4(kf, K + at((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        mma_bf16_16816(s[nt][0], qf[nt][ks][0], qf[nt][ks][1], qf[nt][ks][2], qf[nt][ks][3], kf[0], kf[1]);
-        mma_bf16_16816(s[nt][1], qf[nt][ks][0], qf[nt][ks][1], qf[nt][ks][2], qf[nt][ks][3], kf[2], kf[3]);
-      }
+      ldsm4(kf, K + at<HD>(r0 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
+      mma_bf16_16816(s[0], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], kf[0], kf[1]);
+      mma_bf16_16816(s[1], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], kf[2], kf[3]);
     }
     // m is the maximum of s * scale * log2 e.  Masks only where a key is missing
     // or some row does not see the whole tile.
     const bool masked = there != 0xffffu || key0 + kKT > least;
-    uint32_t pf[NT][4];
+    uint32_t pf[4];
     bool moved = false;
-    float alpha[NT][2];
+    float alpha[2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        if (masked) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int key = j * 8 + col + e;
-              float& v = s[nt][j][2 * b + e];
-              if (!(key0 + key < vis[nt][b] && ((there >> key) & 1u))) v = nothing;
-            }
-        }
-        float mx = fmaxf(fmaxf(s[nt][0][2 * b] * sl2, s[nt][0][2 * b + 1] * sl2),
-                         fmaxf(s[nt][1][2 * b] * sl2, s[nt][1][2 * b + 1] * sl2));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float to = fmaxf(m[nt][b], mx);
-        const float base = to == -INFINITY ? 0.f : to;  // nothing seen yet: weights 2^-inf = 0
-        alpha[nt][b] = ex2f(m[nt][b] - base);
-        moved |= to > m[nt][b];
-        m[nt][b] = to;
-        float sum = 0.f;
-        float pv[2][2];
+    for (int b = 0; b < 2; ++b) {
+      if (masked) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            pv[j][e] = ex2f(fmaf(s[nt][j][2 * b + e], sl2, -base));
+            const int key = j * 8 + col + e;
+            if (!(key0 + key < vis[b] && ((there >> key) & 1u))) s[j][2 * b + e] = nothing;
           }
-        // weights go to the products in bf16: each is off by at most 2^-9 of
-        // itself, and l sums the rounded ones, so a constant V comes out exact
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const __nv_bfloat162 two = __floats2bfloat162_rn(pv[j][0], pv[j][1]);
-          const uint32_t u = *reinterpret_cast<const uint32_t*>(&two);
-          pf[nt][b + 2 * j] = u;
-          sum += __uint_as_float(u << 16) + __uint_as_float(u & 0xffff0000u);
-        }
-        l[nt][b] = l[nt][b] * alpha[nt][b] + sum;
       }
+      float mx = fmaxf(fmaxf(s[0][2 * b] * sl2, s[0][2 * b + 1] * sl2), fmaxf(s[1][2 * b] * sl2, s[1][2 * b + 1] * sl2));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float to = fmaxf(m[b], mx);
+      const float from = to == -INFINITY ? 0.f : to;  // nothing seen yet: weights 2^-inf = 0
+      alpha[b] = ex2f(m[b] - from);
+      moved |= to > m[b];
+      m[b] = to;
+      // weights go to the products in bf16: each is off by at most 2^-9 of
+      // itself, and l sums the rounded ones, so a constant V comes out exact
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const __nv_bfloat162 two =
+            __floats2bfloat162_rn(ex2f(fmaf(s[j][2 * b], sl2, -from)), ex2f(fmaf(s[j][2 * b + 1], sl2, -from)));
+        const uint32_t u = *reinterpret_cast<const uint32_t*>(&two);
+        pf[b + 2 * j] = u;
+        sum += __uint_as_float(u << 16) + __uint_as_float(u & 0xffff0000u);
+      }
+      l[b] = l[b] * alpha[b] + sum;
+    }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int d = 0; d < HD / 8; ++d)
 #pragma unroll
-        for (int d = 0; d < HD / 8; ++d)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[nt][d][e] *= alpha[nt][e >> 1];
+        for (int e = 0; e < 4; ++e) o[d][e] *= alpha[e >> 1];
     }
-    // A row that does not see a key gives it weight 0, and 0 * inf is NaN: a
-    // tile that some rows see further into than others and whose V holds
-    // something not finite takes its products one visible key at a time.
+    // A row that does not see a key gives it weight 0, and 0 * inf is NaN: where
+    // some rows see further than others and V holds something not finite, the
+    // products are taken one visible key at a time.
     bool odd = false;
     if (!SHARED && key0 + kKT > least) {
 #pragma unroll
-      for (int i = 0; i < kCopies; ++i) {
-        const uint4 u = *reinterpret_cast<const uint4*>(__cvta_shared_to_generic(V + (i * 32 + lane) * 16));
+      for (int i = 0; i < HD / 16; ++i) {
+        const uint4 u = *reinterpret_cast<const uint4*>(__cvta_shared_to_generic(V + r0 * HD * 2 + (i * 32 + lane) * 16));
         const uint32_t x[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) odd |= (x[e] & 0x7f80u) == 0x7f80u || (x[e] & 0x7f800000u) == 0x7f800000u;
@@ -325,86 +250,248 @@ __device__ __forceinline__ void Worker<HD, NT, SHARED>::run(int worker, int64_t 
 #pragma unroll
       for (int d = 0; d < HD / 16; ++d) {
         uint32_t vf[4];  // dims lo (keys lo, hi), dims hi (keys lo, hi)
-        ldsm4t(vf, V + at((lane & 7) + (((lane >> 3) & 1) << 3), d * 2 + (lane >> 4)));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma_bf16_16816(o[nt][2 * d], pf[nt][0], pf[nt][1], pf[nt][2], pf[nt][3], vf[0], vf[1]);
-          mma_bf16_16816(o[nt][2 * d + 1], pf[nt][0], pf[nt][1], pf[nt][2], pf[nt][3], vf[2], vf[3]);
-        }
+        ldsm4t(vf, V + at<HD>(r0 + (lane & 7) + (((lane >> 3) & 1) << 3), d * 2 + (lane >> 4)));
+        mma_bf16_16816(o[2 * d], pf[0], pf[1], pf[2], pf[3], vf[0], vf[1]);
+        mma_bf16_16816(o[2 * d + 1], pf[0], pf[1], pf[2], pf[3], vf[2], vf[3]);
       }
     } else {
       for (int key = 0; key < kKT; ++key) {
         const int from = (lane & ~3) | ((key & 7) >> 1);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const uint32_t u = __shfl_sync(0xffffffffu, key < 8 ? pf[nt][b] : pf[nt][b + 2], from);
-            const float pw = (key & 1) ? __uint_as_float(u & 0xffff0000u) : __uint_as_float(u << 16);
-            const bool on = key0 + key < vis[nt][b] && ((there >> key) & 1u);
-#pragma unroll
-            for (int d = 0; d < HD / 8; ++d) {
-              const uint32_t x =
-                  *reinterpret_cast<const uint32_t*>(__cvta_shared_to_generic(V + at(key, d) + (lane & 3) * 4));
-              if (on) {
-                o[nt][d][2 * b] = fmaf(pw, __uint_as_float(x << 16), o[nt][d][2 * b]);
-                o[nt][d][2 * b + 1] = fmaf(pw, __uint_as_float(x & 0xffff0000u), o[nt][d][2 * b + 1]);
-              }
-            }
-          }
-      }
-    }
-    __syncwarp();  // the stage may be filled again
-
-    const bool last = cc.k + 1 == cc.kt;
-    // the next tile is this worker's if its unit is; a segment's last is followed by a set-up
-    const bool more = cc.x + 1 + (last ? line.setup : 0) < x1;
-    if (last || !more) {
-      // ---- this worker's piece of the segment
-      const bool direct = whole && last && !SHARED && a.shared_len == 0;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
         for (int b = 0; b < 2; ++b) {
-          float ls = l[nt][b];
-          ls += __shfl_xor_sync(0xffffffffu, ls, 1);
-          ls += __shfl_xor_sync(0xffffffffu, ls, 2);
-          const int r = row_base + nt * 16 + quad + b * 8;
-          if (r >= R) continue;
-          const int tok = r / hpg;
-          const size_t head = (size_t)(cc.s.row0 + tok) * a.p.n_q + h * hpg + (r - tok * hpg);
-          if (direct) {
-            const float inv = ls > 0.f ? 1.f / ls : ls == 0.f ? 0.f : ls;  // no key seen: zeros; NaN stays
+          const uint32_t u = __shfl_sync(0xffffffffu, key < 8 ? pf[b] : pf[b + 2], from);
+          const float pw = (key & 1) ? __uint_as_float(u & 0xffff0000u) : __uint_as_float(u << 16);
+          const bool on = key0 + key < vis[b] && ((there >> key) & 1u);
 #pragma unroll
-            for (int d = 0; d < HD / 8; ++d) {
-              const __nv_bfloat162 two = __floats2bfloat162_rn(o[nt][d][2 * b] * inv, o[nt][d][2 * b + 1] * inv);
-              *reinterpret_cast<__nv_bfloat162*>(a.out + head * HD + d * 8 + col) = two;
+          for (int d = 0; d < HD / 8; ++d) {
+            const uint32_t x =
+                *reinterpret_cast<const uint32_t*>(__cvta_shared_to_generic(V + at<HD>(r0 + key, d) + (lane & 3) * 4));
+            if (on) {
+              o[d][2 * b] = fmaf(pw, __uint_as_float(x << 16), o[d][2 * b]);
+              o[d][2 * b + 1] = fmaf(pw, __uint_as_float(x & 0xffff0000u), o[d][2 * b + 1]);
             }
-          } else {
-            const size_t slot = whole ? head : (size_t)worker * MT + (r - row_base);
-            float* dst = (whole ? pc.first_o : pc.more_o) + slot * HD;
-#pragma unroll
-            for (int d = 0; d < HD / 8; ++d)
-              *reinterpret_cast<float2*>(dst + d * 8 + col) = make_float2(o[nt][d][2 * b], o[nt][d][2 * b + 1]);
-            if ((lane & 3) == 0) (whole ? pc.first_ml : pc.more_ml)[slot] = make_float2(m[nt][b], ls);
           }
         }
-      fresh = true;
+      }
     }
-    if (!more) break;
-    cc.next(line);
   }
-  cp_wait<0>();
-}
 
-template <int HD, int NT, bool SHARED>
+  // The rows' piece of the segment: to the output (`direct`: it is all there is), to the rows' first slots (the
+  // segment's first tile was this worker's) or, from slot `more` on, to the worker's.
+  __device__ __forceinline__ void end(const PagedWork& w, const Cursor& c, int hpg, bool direct, bool first, size_t more) {
+    const PagedAttnArgs& a = w.a;
+    const Pieces& pc = SHARED ? w.shared : w.own;
+    const int lane = threadIdx.x & 31, quad = lane >> 2, col = (lane & 3) * 2;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      float ls = l[b];
+      ls += __shfl_xor_sync(0xffffffffu, ls, 1);
+      ls += __shfl_xor_sync(0xffffffffu, ls, 2);
+      const int r = base + quad + b * 8;
+      if (r >= R) continue;
+      const int tok = r / hpg;
+      const size_t head = (size_t)(c.s.row0 + tok) * a.p.n_q + h * hpg + (r - tok * hpg);
+      if (direct) {
+        const float inv = ls > 0.f ? 1.f / ls : ls == 0.f ? 0.f : ls;  // no key seen: zeros; NaN stays
+#pragma unroll
+        for (int d = 0; d < HD / 8; ++d)
+          *reinterpret_cast<__nv_bfloat162*>(a.out + head * HD + d * 8 + col) =
+              __floats2bfloat162_rn(o[d][2 * b] * inv, o[d][2 * b + 1] * inv);
+      } else {
+        const size_t slot = first ? head : more + quad + b * 8;
+        float* dst = (first ? pc.first_o : pc.more_o) + slot * HD;
+#pragma unroll
+        for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<float2*>(dst + d * 8 + col) = make_float2(o[d][2 * b], o[d][2 * b + 1]);
+        if ((lane & 3) == 0) (first ? pc.first_ml : pc.more_ml)[slot] = make_float2(m[b], ls);
+      }
+    }
+  }
+};
+
+// A worker's place in the line, for the loads and for the products, which run
+// kStages - 1 tiles behind: the tiles among units [.., x1).
+struct Share {
+  Cursor ld, cc;
+  int64_t x1;
+  __device__ __forceinline__ bool begin(const Line& line, int64_t x0, int64_t end) {
+    x1 = end;
+    cc.seek(line, x0);
+    ld = cc;
+    return cc.x < x1;  // else nothing but a set-up
+  }
+  __device__ __forceinline__ bool loading() const { return ld.x < x1; }
+  __device__ __forceinline__ void loaded(const Line& line) {
+    if (ld.x + 1 < x1) ld.next(line);
+    else ld.x = x1;
+  }
+  __device__ __forceinline__ bool last() const { return cc.k + 1 == cc.kt; }
+  // the next tile is this worker's if its unit is; a segment's last is followed by a set-up
+  __device__ __forceinline__ bool more(const Line& line) const { return cc.x + 1 + (last() ? line.setup : 0) < x1; }
+};
+
+// Few rows (up to 16 a sequence and KV head): a warp is a worker, with 16 keys
+// a tile and three tiles in flight of its own, and never meets another.
+template <int HD, bool SHARED>
+struct WarpWorker {
+  static constexpr int kRows = 16, kKeys = 16, kPerCta = kWarps;
+  static constexpr int kTileB = kKeys * HD * 2;  // one tile of K (or V)
+  static constexpr int kSmem = kWarps * kStages * 2 * kTileB;
+
+  static __device__ __forceinline__ void run(const PagedWork& w, const Line& line, unsigned char* smem, int worker, int64_t x0,
+                                             int64_t x1) {
+    __shared__ uint32_t there_[kWarps][kStages];  // bit j: key j of the tile is there
+    const PagedAttnArgs& a = w.a;
+    const int lane = threadIdx.x & 31;
+    const uint32_t ring = smem_u32(smem) + (threadIdx.x >> 5) * (uint32_t)(kStages * 2 * kTileB);
+    uint32_t* there = there_[threadIdx.x >> 5];
+    Share sh;
+    if (!sh.begin(line, x0, x1)) return;
+    auto next_key = [&]() {
+      return key_at<SHARED>(a, sh.ld, (SHARED ? 0 : a.shared_len) + sh.ld.k * kKeys + (lane & 15));
+    };
+    Key key = next_key();
+    int at_stage = 0;  // of the next load
+    auto load = [&]() {
+      if (sh.loading()) {
+        const uint32_t row = key_row(a, key, sh.ld.head());
+        const unsigned mask = __ballot_sync(0xffffffffu, row != ~0u) & 0xffffu;
+        if (lane == 0) there[at_stage] = mask;
+        constexpr int kChunks = HD / 8, kPer = 32 / kChunks;  // of a row; rows of one copy of the warp
+        const int sub = lane / kChunks, c = lane % kChunks;
+        const uint32_t dst = ring + at_stage * 2 * kTileB + at<HD>(sub, c);
+#pragma unroll
+        for (int i = 0; i < kKeys / kPer; ++i) {
+          const uint32_t src = __shfl_sync(0xffffffffu, row, i * kPer + sub);
+          // chunk c of row i * kPer + sub: the swizzle's bits of the two parts of the row number do not meet
+          const uint32_t to = (dst ^ (uint32_t)(((i * kPer) & 7) << 4)) + (uint32_t)(i * kPer * HD * 2);
+          copy_kv<HD>(a, to, to + kTileB, src, c);
+        }
+        sh.loaded(line);
+        if (sh.loading()) key = next_key();
+      }
+      at_stage = at_stage + 1 == kStages ? 0 : at_stage + 1;
+      cp_commit();
+    };
+#pragma unroll 1
+    for (int i = 0; i < kStages - 1; ++i) load();
+    const float sl2 = a.scale * kLog2e;
+    Rows<HD, SHARED> rows;
+    bool fresh = true, first = false;
+    for (int stage = 0;; stage = stage + 1 == kStages ? 0 : stage + 1) {
+      if (fresh) {
+        first = sh.cc.k == 0;
+        rows.begin(w, sh.cc, line.hpg, (sh.cc.seg - sh.cc.head() * sh.cc.mt) * kRows);
+      }
+      load();
+      cp_wait<kStages - 1>();
+      __syncwarp();
+      const uint32_t K = ring + stage * 2 * kTileB;
+      rows.keys16(sl2, K, K + kTileB, 0, sh.cc.k * kKeys, there[stage]);
+      __syncwarp();  // the stage may be filled again
+      const bool last = sh.last(), more = sh.more(line);
+      fresh = last || !more;
+      if (fresh) rows.end(w, sh.cc, line.hpg, first && last && !SHARED && a.shared_len == 0, first, (size_t)worker * kRows);
+      if (!more) break;
+      sh.cc.next(line);
+    }
+    cp_wait<0>();
+  }
+};
+
+// More rows: a CTA is a worker, 64 rows (16 a warp) against tiles of 64 keys
+// that its warps load together.  One barrier a tile: behind it the tile's keys
+// are there, every warp is done with the tile before, whose stage the next load
+// takes, and the rows of that load's keys are known.
+template <int HD, bool SHARED>
+struct CtaWorker {
+  static constexpr int kRows = 16 * kWarps, kKeys = 64, kPerCta = 1;
+  static constexpr int kTileB = kKeys * HD * 2;
+  static constexpr int kSmem = kStages * 2 * kTileB;
+
+  static __device__ __forceinline__ void run(const PagedWork& w, const Line& line, unsigned char* smem, int worker, int64_t x0,
+                                             int64_t x1) {
+    __shared__ uint32_t row_[2][kKeys];        // cache rows of the next load's keys
+    __shared__ uint32_t there[kStages + 1][2];  // bit j: key j of the tile is there (one more than tiles are kept)
+    const PagedAttnArgs& a = w.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t ring = smem_u32(smem);
+    Share sh;
+    if (!sh.begin(line, x0, x1)) return;
+    auto next_key = [&]() {  // threads 0-63
+      return tid < kKeys ? key_at<SHARED>(a, sh.ld, (SHARED ? 0 : a.shared_len) + sh.ld.k * kKeys + tid) : Key{0, -1};
+    };
+    Key key = next_key();
+    int tile = 0;  // of the next load
+    // the rows of the next load's keys, for all warps after the next barrier
+    auto name = [&]() {
+      if (sh.loading() && tid < kKeys) {
+        const uint32_t row = key_row(a, key, sh.ld.head());
+        row_[tile & 1][tid] = row;
+        const unsigned mask = __ballot_sync(0xffffffffu, row != ~0u);
+        if (lane == 0) there[tile % (kStages + 1)][warp] = mask;
+      }
+    };
+    auto load = [&]() {
+      if (sh.loading()) {
+        constexpr int kChunks = HD / 8, kPer = kWarps * 32 / kChunks;  // of a row; rows of one copy of the CTA
+        const int sub = tid / kChunks, c = tid % kChunks;
+        const uint32_t dst = ring + (tile % kStages) * 2 * kTileB;
+#pragma unroll
+        for (int i = 0; i < kKeys / kPer; ++i) {
+          const int r = i * kPer + sub;
+          const uint32_t to = dst + at<HD>(r, c);
+          copy_kv<HD>(a, to, to + kTileB, row_[tile & 1][r], c);
+        }
+        sh.loaded(line);
+        if (sh.loading()) key = next_key();
+      }
+      ++tile;
+      cp_commit();
+    };
+#pragma unroll 1
+    for (int i = 0; i < kStages - 1; ++i) {
+      name();
+      __syncthreads();
+      load();
+    }
+    const float sl2 = a.scale * kLog2e;
+    Rows<HD, SHARED> rows;
+    bool fresh = true, first = false;
+    for (int t = 0;; ++t) {
+      if (fresh) {
+        first = sh.cc.k == 0;
+        rows.begin(w, sh.cc, line.hpg, (sh.cc.seg - sh.cc.head() * sh.cc.mt) * kRows + warp * 16);
+      }
+      name();
+      cp_wait<kStages - 2>();
+      __syncthreads();
+      load();
+      const uint32_t K = ring + (t % kStages) * 2 * kTileB;
+      const int key0 = sh.cc.k * kKeys;
+      if (rows.base < rows.R) {
+#pragma unroll 1
+        for (int i = 0; i < kKeys / 16; ++i) {
+          const uint32_t mask = there[t % (kStages + 1)][i >> 1] >> ((i & 1) * 16) & 0xffffu;
+          if (mask) rows.keys16(sl2, K, K + kTileB, i * 16, key0 + i * 16, mask);
+        }
+      }
+      const bool last = sh.last(), more = sh.more(line);
+      fresh = last || !more;
+      if (fresh && rows.base < rows.R)
+        rows.end(w, sh.cc, line.hpg, first && last && !SHARED && a.shared_len == 0, first, (size_t)worker * kRows + warp * 16);
+      if (!more) break;
+      sh.cc.next(line);
+    }
+    cp_wait<0>();
+  }
+};
+
+template <int HD, bool SHARED, template <int, bool> class W>
 __global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const __grid_constant__ PagedWork w) {
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ int64_t starts[SHARED ? 1 : kMaxSeqs + 1];
-  __shared__ uint32_t valid[kWarps][kStages];
-  using Wk = Worker<HD, NT, SHARED>;
-  const int warp = threadIdx.x >> 5;
-  const Line line = make_line(w.a.p, w.a.shared_len, !SHARED, Wk::MT, kKT, SHARED ? 0 : kSetup, starts);
+  using Worker = W<HD, SHARED>;
+  const Line line = make_line(w.a.p, w.a.shared_len, !SHARED, Worker::kRows, Worker::kKeys, SHARED ? 0 : kSetup, starts);
   // The first kernel of a call waits for what ran before it.  An own part that
   // follows a shared one has been let go by it after such a wait; it needs
   // nothing of that one, but the join waits for this kernel alone, so it ends
@@ -421,12 +508,10 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const __grid_co
     if (blockIdx.x == 0)
       for (int i = threadIdx.x; i <= w.a.p.n_seqs; i += kWarps * 32) w.starts[i] = starts[i];
   }
-  const int worker = blockIdx.x * kWarps + warp;
-  const int64_t per = SHARED ? w.shared_per : share_size(total, gridDim.x * kWarps, 1);
-  if (worker * per < total) {
-    Wk k{w, line, (int)(threadIdx.x & 31), smem_u32(smem) + warp * (uint32_t)(kStages * Wk::kStageB), valid[warp]};
-    k.run(worker, worker * per, min(total, (worker + 1) * per));
-  }
+  const int workers = gridDim.x * Worker::kPerCta;
+  const int worker = Worker::kPerCta == 1 ? blockIdx.x : blockIdx.x * Worker::kPerCta + (threadIdx.x >> 5);
+  const int64_t per = SHARED ? w.shared_per : share_size(total, workers, 1);
+  if (worker * per < total) Worker::run(w, line, smem, worker, worker * per, min(total, (worker + 1) * per));
   if (!first) pdl_wait();
 }
 
@@ -551,44 +636,46 @@ size_t lay_out(PagedWork& w, int num_sms, unsigned char* base) {
     return q;
   };
   w.starts = static_cast<int64_t*>(take(sizeof(int64_t) * (kMaxSeqs + 1)));
-  w.own_workers = w.shared_workers = num_sms * kCtasPerSm * kWarps;
   auto pieces = [&](Pieces& pc, size_t rows) {
     pc.first_o = static_cast<float*>(take(heads * p.head_dim * sizeof(float)));
     pc.first_ml = static_cast<float2*>(take(heads * sizeof(float2)));
     pc.more_o = static_cast<float*>(take(rows * p.head_dim * sizeof(float)));
     pc.more_ml = static_cast<float2*>(take(rows * sizeof(float2)));
   };
-  const size_t warps = (size_t)w.own_workers * 32, ctas = (size_t)num_sms * kTcRows;
-  pieces(w.own, warps);
-  if (w.a.shared_len > 0) pieces(w.shared, warps > ctas ? warps : ctas);
+  // slots of every kind of worker's rows: warps of 16, CTAs of 64, tcgen05 CTAs of 256
+  static_assert(kWarps * 16 == 64, "");
+  const size_t rows = (size_t)num_sms * kCtasPerSm * 64, tc = (size_t)num_sms * kTcRows;
+  pieces(w.own, rows);
+  if (w.a.shared_len > 0) pieces(w.shared, rows > tc ? rows : tc);
   return off;
 }
 
-template <int HD, int NT, bool SHARED>
-cudaError_t launch_part(const PagedWork& w, int workers, cudaStream_t st) {
-  const int smem = kWarps * kStages * Worker<HD, NT, SHARED>::kStageB;
-  static cudaError_t once = cudaFuncSetAttribute(paged_attn_kernel<HD, NT, SHARED>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <int HD, bool SHARED, template <int, bool> class W>
+cudaError_t launch_part(const PagedWork& w, int ctas, cudaStream_t st) {
+  constexpr int smem = W<HD, SHARED>::kSmem;
+  static cudaError_t once =
+      cudaFuncSetAttribute(paged_attn_kernel<HD, SHARED, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (once != cudaSuccess) return once;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute at;
-  overlapped(cfg, at, workers / kWarps, kWarps * 32, smem, st);
-  return cudaLaunchKernelEx(&cfg, paged_attn_kernel<HD, NT, SHARED>, w);
+  overlapped(cfg, at, (unsigned)ctas, kWarps * 32, smem, st);
+  return cudaLaunchKernelEx(&cfg, paged_attn_kernel<HD, SHARED, W>, w);
 }
 
 template <int HD>
 cudaError_t launch(PagedWork& w, int num_sms, cudaStream_t st) {
+  using Few = WarpWorker<HD, false>;
+  using Many = CtaWorker<HD, false>;
   const PagedArgs& p = w.a.p;
-  const int hpg = p.n_q / p.n_kv;
-  w.own_mt = (int64_t)p.n_rows * hpg > 16 * (int64_t)p.n_seqs ? 32 : 16;
-  w.own_keys = kKT;
+  const int64_t rows = (int64_t)p.n_rows * (p.n_q / p.n_kv);  // of a KV head
+  const int ctas = num_sms * kCtasPerSm;
   cudaError_t e = cudaSuccess;
   if (w.a.shared_len > 0) {
-    const int64_t rows = (int64_t)p.n_rows * hpg;
-    const bool tc = rows > 32 && paged_shared_tc_takes(p);
-    w.shared_mt = tc ? kTcRows : rows > 16 ? 32 : 16;
-    w.shared_keys = tc ? kTcKeys : kKT;
-    if (tc) w.shared_workers = num_sms;
+    // tcgen05 from 17 rows a head on, where it takes the pages
+    const bool few = rows <= Few::kRows, tc = !few && paged_shared_tc_takes(p);
+    w.shared_mt = few ? Few::kRows : tc ? kTcRows : Many::kRows;
+    w.shared_keys = few ? Few::kKeys : tc ? kTcKeys : Many::kKeys;
+    w.shared_workers = few ? ctas * Few::kPerCta : tc ? num_sms : ctas;
     const int kt = ceil_div(w.a.shared_len, w.shared_keys);
     const int64_t segments = (int64_t)p.n_kv * ((rows + w.shared_mt - 1) / w.shared_mt);
     w.shared_per = (int)share_size(segments * kt, w.shared_workers, 1);
@@ -604,13 +691,18 @@ cudaError_t launch(PagedWork& w, int num_sms, cudaStream_t st) {
         w.shared_per = per;
       }
     }
-    e = tc                   ? paged_shared_tc_launch(w, num_sms, st)
-        : w.shared_mt == 32 ? launch_part<HD, 2, true>(w, w.shared_workers, st)
-                            : launch_part<HD, 1, true>(w, w.shared_workers, st);
+    e = few  ? launch_part<HD, true, WarpWorker>(w, ctas, st)
+        : tc ? paged_shared_tc_launch(w, num_sms, st)
+             : launch_part<HD, true, CtaWorker>(w, ctas, st);
     if (e != cudaSuccess) return e;
   }
-  e = w.own_mt == 32 ? launch_part<HD, 2, false>(w, w.own_workers, st)
-                     : launch_part<HD, 1, false>(w, w.own_workers, st);
+  // The own part by warps up to 16 rows a sequence and KV head, on average;
+  // beyond that a warp's 16 keys would be loaded again for every 16 rows.
+  const bool few = rows <= Few::kRows * (int64_t)p.n_seqs;
+  w.own_mt = few ? Few::kRows : Many::kRows;
+  w.own_keys = few ? Few::kKeys : Many::kKeys;
+  w.own_workers = few ? ctas * Few::kPerCta : ctas;
+  e = few ? launch_part<HD, false, WarpWorker>(w, ctas, st) : launch_part<HD, false, CtaWorker>(w, ctas, st);
   if (e != cudaSuccess) return e;
   const int64_t items = (int64_t)p.n_rows * p.n_q;
   cudaLaunchConfig_t cfg;
