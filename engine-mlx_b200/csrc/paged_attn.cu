@@ -515,112 +515,159 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const __grid_co
   if (!first) pdl_wait();
 }
 
-// One warp a (row, q head): joins its pieces.
+// Joins the pieces of each (row, q head), an item.  `parts` warps share an item
+// where there are few; else a warp has several, 32 in its lanes: where their
+// pieces are (a search, divisions) is found by all lanes together, mostly before
+// the pieces are written, and what is left of an item then is one L2 latency for
+// eight pieces.  (A warp an item, finding its place itself: 7 to 16 us of the
+// shared cases, most of it in a second wave of CTAs.)
 template <int HD>
-__global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constant__ PagedWork w) {
-  const PagedAttnArgs& a = w.a;
-  const int lane = threadIdx.x & 31;
-  const int item = blockIdx.x * 4 + (threadIdx.x >> 5);
-  pdl_trigger();
-  if (item >= a.p.n_rows * a.p.n_q) {
-    pdl_wait();
-    return;
-  }
-  // ---- before the pieces are there: whose row it is and where the shared part's pieces will be
-  const int row = item / a.p.n_q, hq = item - row * a.p.n_q;
-  const int hpg = a.p.n_q / a.p.n_kv, h = hq / hpg, g = hq - h * hpg;
-  const int i = warp_find_seq(a.p.indptr, a.p.n_seqs, row);
-  if (i >= a.p.n_seqs || row < a.p.indptr[i]) {  // behind the last sequence: left as it was
-    pdl_wait();  // (every CTA waits, so that what follows this kernel follows the ones before it)
-    return;
-  }
-  const SeqInfo s = load_seq(a.p, i, a.shared_len);
+__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedWork w, int parts) {
+  __shared__ float sm[4], sl[4];
+  __shared__ float so[4][HD];
   constexpr int E = HD / 32;
-  // the slot of a segment's second worker, and how many follow the first
-  auto more_of = [&](int mt, int kt, int64_t per, int64_t x0, int r, size_t& slot) {
-    const int c0 = share_of(x0, per), c1 = share_of(x0 + kt - 1, per);
-    slot = (size_t)(c0 + 1) * mt + r % mt;
-    return c1 - c0;
-  };
-  size_t slot_shared = 0, slot_own = 0;
-  int more_shared = 0;
-  if (s.ok && a.shared_len > 0) {
-    const Line all = make_line(a.p, a.shared_len, false, w.shared_mt, w.shared_keys, 0, nullptr);
-    const SeqInfo every = all.seq(0);
-    const int r = row * hpg + g, kt = all.key_tiles(every), seg = h * all.row_tiles(every) + r / w.shared_mt;
-    // with workers of their own, segments are as long as those workers' shares
-    const int64_t begin = (int64_t)seg * (w.shared_split ? (int64_t)w.shared_split * w.shared_per : kt);
-    more_shared = more_of(w.shared_mt, kt, w.shared_per, begin, r, slot_shared);
-  }
+  const PagedAttnArgs& a = w.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_trigger();
+  const int hpg = a.p.n_q / a.p.n_kv, items = a.p.n_rows * a.p.n_q;
+  const int part = warp % parts, stride = gridDim.x * (4 / parts);
   const Line own = make_line(a.p, a.shared_len, true, w.own_mt, w.own_keys, kSetup, w.starts);
-  const int r_own = (row - s.row0) * hpg + g, kt_own = own.key_tiles(s);
-  const int64_t x_own = ((int64_t)h * own.row_tiles(s) + r_own / w.own_mt) * (kt_own + kSetup) + kSetup;
-
-  float o[E];
+  const Line all = make_line(a.p, a.shared_len, false, w.shared_mt, w.shared_keys, 0, nullptr);
+  bool waited = false;
+  for (int first = blockIdx.x * (4 / parts) + warp / parts; first < items; first += 32 * stride) {
+    // ---- lane j: item first + j * stride
+    const int64_t item64 = (int64_t)first + (int64_t)lane * stride;
+    int item = item64 < items ? (int)item64 : -1;
+    const int row = item < 0 ? 0 : item / a.p.n_q, hq = item < 0 ? 0 : item - row * a.p.n_q;
+    const int h = hq / hpg, g = hq - h * hpg;
+    int seq = 0, n = a.p.n_seqs;  // the first sequence that ends behind the row
+    while (n > 0) {
+      const int mid = n >> 1;
+      if (a.p.indptr[seq + mid + 1] > row) n = mid;
+      else seq += mid + 1, n -= mid + 1;
+    }
+    SeqInfo s{0, 0, 0, false};
+    if (seq >= a.p.n_seqs || row < a.p.indptr[seq]) item = -1;  // behind the last sequence: left as it was
+    else s = own.seq(seq);
+    const bool ok = item >= 0 && s.ok;
+    // pieces of the row's segment in each part, and the slot of its second worker's
+    auto place = [&](int mt, int kt, int64_t each, int64_t per, int64_t begin, int r, uint32_t& slot) {
+      const int64_t x0 = begin + (int64_t)(r / mt) * each;
+      const int c0 = share_of(x0, per), c1 = share_of(x0 + kt - 1, per);
+      slot = (uint32_t)((c0 + 1) * mt + r % mt);
+      return c1 - c0 + 1;
+    };
+    int n_all = 0, n_own = 0;
+    uint32_t slot_all = 0, slot_own = 0;
+    if (ok && a.shared_len > 0) {
+      const SeqInfo every = all.seq(0);
+      const int kt = all.key_tiles(every);
+      // with workers of their own, shared segments are as long as those workers' shares
+      const int64_t each = w.shared_split ? (int64_t)w.shared_split * w.shared_per : kt;
+      n_all = place(w.shared_mt, kt, each, w.shared_per, (int64_t)h * all.row_tiles(every) * each, row * hpg + g, slot_all);
+    }
+    const int kt_own = ok ? own.key_tiles(s) : 1;
+    const int64_t x_own = ok ? (int64_t)h * own.row_tiles(s) * (kt_own + kSetup) + kSetup : 0;
+    if (!waited) pdl_wait();
+    waited = true;
+    if (ok) {
+      const int64_t per = share_size(w.starts[a.p.n_seqs], w.own_workers, 1);
+      n_own = place(w.own_mt, kt_own, kt_own + kSetup, per, w.starts[seq] + x_own, (row - s.row0) * hpg + g, slot_own);
+      if (a.shared_len == 0 && n_own == 1) item = -1;  // one worker had the segment whole and wrote it
+    }
+    // ---- item by item
+    const int many = min(32, (items - first + stride - 1) / stride);
+    for (int j = 0; j < many; ++j) {
+      const int it = __shfl_sync(0xffffffffu, item, j);
+      const int na = __shfl_sync(0xffffffffu, n_all, j), np = na + __shfl_sync(0xffffffffu, n_own, j);
+      const uint32_t sa = __shfl_sync(0xffffffffu, slot_all, j), sw = __shfl_sync(0xffffffffu, slot_own, j);
+      if (it < 0 && parts == 1) continue;
+      float o[E], m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  // n pieces: the first slot, then those of further workers
-  auto take = [&](const Pieces& pc, size_t slot, int mt, int n) {
-    for (int x0 = 0; x0 < n; x0 += 32) {
-      const int x = x0 + lane;  // this lane's (max, sum)
-      float2 ml = make_float2(-INFINITY, 0.f);
-      if (x < n) ml = x == 0 ? pc.first_ml[item] : pc.more_ml[slot + (size_t)(x - 1) * mt];
-      constexpr int U = 8;  // pieces in flight
-      const int many = min(32, n - x0);
-      float was = 0.f, wx = 0.f;
-      for (int y = 0; y < many; y += U) {
-        float v[U][E];
+      for (int e = 0; e < E; ++e) o[e] = 0.f;
+      // piece z: the shared part's first slot and further workers', then the own part's; this warp's are part, part + parts, ...
+      auto slot_of = [&](int z, bool& own_part, bool& is_first) {
+        own_part = z >= na;
+        const int y = own_part ? z - na : z;
+        is_first = y == 0;
+        return is_first ? (size_t)it : (size_t)(own_part ? sw : sa) + (size_t)(y - 1) * (own_part ? w.own_mt : w.shared_mt);
+      };
+      for (int z0 = part; it >= 0 && z0 < np; z0 += 32 * parts) {
+        const int z = z0 + parts * lane;  // this lane's (max, sum)
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (z < np) {
+          bool op, fs;
+          const size_t at = slot_of(z, op, fs);
+          ml = (op ? (fs ? w.own.first_ml : w.own.more_ml) : (fs ? w.shared.first_ml : w.shared.more_ml))[at];
+        }
+        constexpr int U = 8;  // pieces in flight
+        const int here = min(32, (np - z0 + parts - 1) / parts);
+        float wx = 0.f;
+        for (int y = 0; y < here; y += U) {
+          float v[U][E];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int z = x0 + y + u;
-          const bool on = y + u < many;
-          const float* p = (z == 0 ? pc.first_o + (size_t)item * HD : pc.more_o + (slot + (size_t)(on ? z - 1 : 0) * mt) * HD) +
-                           lane * E;
-          if constexpr (E == 4) {
-            const float4 f = on ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
-            v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
-          } else {
-            const float2 f = on ? *reinterpret_cast<const float2*>(p) : make_float2(0.f, 0.f);
-            v[u][0] = f.x, v[u][1] = f.y;
+          for (int u = 0; u < U; ++u) {
+            const bool on = y + u < here;
+            bool op, fs;
+            const size_t at = slot_of(on ? z0 + parts * (y + u) : 0, op, fs);
+            const float* p = (op ? (fs ? w.own.first_o : w.own.more_o) : (fs ? w.shared.first_o : w.shared.more_o)) + at * HD + lane * E;
+            if constexpr (E == 4) {
+              const float4 f = on ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+              v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
+            } else {
+              const float2 f = on ? *reinterpret_cast<const float2*>(p) : make_float2(0.f, 0.f);
+              v[u][0] = f.x, v[u][1] = f.y;
+            }
+          }
+          if (y == 0) {  // with the first loads on their way
+            const float to = fmaxf(m, warp_max(ml.x)), base = to == -INFINITY ? 0.f : to;
+            const float was = ex2f(m - base);
+            wx = ex2f(ml.x - base);
+            l = l * was + warp_sum(ml.y * wx);  // a NaN among the sums stays one
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] *= was;
+            m = to;
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const float wu = __shfl_sync(0xffffffffu, wx, (y + u) & 31);
+            if (y + u < here)
+#pragma unroll
+              for (int e = 0; e < E; ++e) o[e] = fmaf(v[u][e], wu, o[e]);
           }
         }
-        if (y == 0) {  // with the first loads on their way
-          const float to = fmaxf(m, warp_max(ml.x)), base = to == -INFINITY ? 0.f : to;
-          was = ex2f(m - base), wx = ex2f(ml.x - base);
-          l = l * was + warp_sum(ml.y * wx);  // a NaN among the sums stays one
+      }
+      if (parts > 1) {  // one item a warp: every warp of the CTA comes here once
 #pragma unroll
-          for (int e = 0; e < E; ++e) o[e] *= was;
+        for (int e = 0; e < E; ++e) so[warp][lane * E + e] = o[e];
+        if (lane == 0) {
+          sm[warp] = m;
+          sl[warp] = l;
+        }
+        __syncthreads();
+        if (part > 0 || it < 0) break;
+        for (int k = warp + 1; k < warp + parts; ++k) {
+          const float to = fmaxf(m, sm[k]), base = to == -INFINITY ? 0.f : to;
+          const float x = ex2f(m - base), y = ex2f(sm[k] - base);
+          l = l * x + sl[k] * y;
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] = o[e] * x + so[k][lane * E + e] * y;
           m = to;
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const float wu = __shfl_sync(0xffffffffu, wx, (y + u) & 31);
-          if (y + u < many)
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf(v[u][e], wu, o[e]);
-        }
       }
-    }
-  };
-  pdl_wait();
-  if (s.ok) {
-    const int64_t T = w.starts[a.p.n_seqs], x0 = w.starts[i] + x_own;
-    if (a.shared_len > 0) take(w.shared, slot_shared, w.shared_mt, 1 + more_shared);
-    const int more = more_of(w.own_mt, kt_own, share_size(T, w.own_workers, 1), x0, r_own, slot_own);
-    if (a.shared_len == 0 && more == 0) return;  // one worker had the segment whole and wrote it
-    take(w.own, slot_own, w.own_mt, 1 + more);
-  }
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // no key seen: zeros; NaN stays
-  bf16* dst = a.out + (size_t)item * HD + lane * E;
-  uint32_t u[E / 2];
+      const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // no key seen: zeros; NaN stays
+      bf16* dst = a.out + (size_t)it * HD + lane * E;
+      uint32_t u[E / 2];
 #pragma unroll
-  for (int e = 0; e < E / 2; ++e) {
-    const __nv_bfloat162 two = __floats2bfloat162_rn(o[2 * e] * inv, o[2 * e + 1] * inv);
-    u[e] = *reinterpret_cast<const uint32_t*>(&two);
+      for (int e = 0; e < E / 2; ++e) {
+        const __nv_bfloat162 two = __floats2bfloat162_rn(o[2 * e] * inv, o[2 * e + 1] * inv);
+        u[e] = *reinterpret_cast<const uint32_t*>(&two);
+      }
+      if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(u[0], u[1]);
+      else *reinterpret_cast<uint32_t*>(dst) = u[0];
+    }
   }
-  if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(u[0], u[1]);
-  else *reinterpret_cast<uint32_t*>(dst) = u[0];
+  if (!waited) pdl_wait();  // every CTA waits, so that what follows this kernel follows the ones before it
 }
 
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -704,11 +751,15 @@ cudaError_t launch(PagedWork& w, int num_sms, cudaStream_t st) {
   w.own_workers = few ? ctas * Few::kPerCta : ctas;
   e = few ? launch_part<HD, false, WarpWorker>(w, ctas, st) : launch_part<HD, false, CtaWorker>(w, ctas, st);
   if (e != cudaSuccess) return e;
-  const int64_t items = (int64_t)p.n_rows * p.n_q;
+  // five CTAs an SM fit beside what the own part's have not left yet; fewer
+  // items than their warps are shared by two or four
+  const int64_t items = (int64_t)p.n_rows * p.n_q, warps = (int64_t)num_sms * 20;
+  const int parts = items * 4 <= warps ? 4 : items * 2 <= warps ? 2 : 1;
+  const int64_t grid = (items * parts + 3) / 4;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute at;
-  overlapped(cfg, at, (unsigned)((items + 3) / 4), 128, 0, st);
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<HD>, static_cast<const PagedWork>(w));
+  overlapped(cfg, at, (unsigned)(grid < warps / 4 ? grid : warps / 4), 128, 0, st);
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<HD>, static_cast<const PagedWork>(w), parts);
 }
 
 }  // namespace
