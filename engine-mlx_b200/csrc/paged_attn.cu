@@ -32,9 +32,12 @@ constexpr int kSetup = 1;
 constexpr int kMaxSeqs = 1024;
 constexpr int kCtasPerSm = 2;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+// `policy`: first out of L2.  K and V are read once or, by a sequence's next row
+// tile, soon again; the pieces, which the join reads, are to stay.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on, uint64_t policy) {
   const int n = on ? 16 : 0;  // 0: the 16 bytes become zeros, nothing is read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(n), "l"(policy)
+               : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -122,11 +125,12 @@ __device__ __forceinline__ uint32_t key_row(const PagedAttnArgs& a, const Key& k
 
 // Copies 16 bytes of K and of V; row ~0 reads as zeros.
 template <int HD>
-__device__ __forceinline__ void copy_kv(const PagedAttnArgs& a, uint32_t to_k, uint32_t to_v, uint32_t row, int c) {
+__device__ __forceinline__ void copy_kv(const PagedAttnArgs& a, uint32_t to_k, uint32_t to_v, uint32_t row, int c,
+                                        uint64_t policy) {
   const bool on = row != ~0u;
   const size_t off = (on ? (size_t)row * HD : 0) + c * 8;
-  cp_async16(to_k, a.p.k + off, on);
-  cp_async16(to_v, a.p.v + off, on);
+  cp_async16(to_k, a.p.k + off, on, policy);
+  cp_async16(to_v, a.p.v + off, on, policy);
 }
 
 // Sixteen rows of one segment, by a warp: q as MMA operands, the running
@@ -346,6 +350,7 @@ struct WarpWorker {
     uint32_t* there = there_[threadIdx.x >> 5];
     Share sh;
     if (!sh.begin(line, x0, x1)) return;
+    const uint64_t policy = l2_evict_first_policy();
     auto next_key = [&]() {
       return key_at<SHARED>(a, sh.ld, (SHARED ? 0 : a.shared_len) + sh.ld.k * kKeys + (lane & 15));
     };
@@ -364,7 +369,7 @@ struct WarpWorker {
           const uint32_t src = __shfl_sync(0xffffffffu, row, i * kPer + sub);
           // chunk c of row i * kPer + sub: the swizzle's bits of the two parts of the row number do not meet
           const uint32_t to = (dst ^ (uint32_t)(((i * kPer) & 7) << 4)) + (uint32_t)(i * kPer * HD * 2);
-          copy_kv<HD>(a, to, to + kTileB, src, c);
+          copy_kv<HD>(a, to, to + kTileB, src, c, policy);
         }
         sh.loaded(line);
         if (sh.loading()) key = next_key();
@@ -417,6 +422,7 @@ struct CtaWorker {
     const uint32_t ring = smem_u32(smem);
     Share sh;
     if (!sh.begin(line, x0, x1)) return;
+    const uint64_t policy = l2_evict_first_policy();
     auto next_key = [&]() {  // threads 0-63
       return tid < kKeys ? key_at<SHARED>(a, sh.ld, (SHARED ? 0 : a.shared_len) + sh.ld.k * kKeys + tid) : Key{0, -1};
     };
@@ -440,7 +446,7 @@ struct CtaWorker {
         for (int i = 0; i < kKeys / kPer; ++i) {
           const int r = i * kPer + sub;
           const uint32_t to = dst + at<HD>(r, c);
-          copy_kv<HD>(a, to, to + kTileB, row_[tile & 1][r], c);
+          copy_kv<HD>(a, to, to + kTileB, row_[tile & 1][r], c, policy);
         }
         sh.loaded(line);
         if (sh.loading()) key = next_key();

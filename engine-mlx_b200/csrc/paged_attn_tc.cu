@@ -71,11 +71,18 @@ constexpr uint32_t idesc(int n, bool b_mn) {
          ((uint32_t)(128 >> 4) << 24);
 }
 
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar, uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+      "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar)), "l"(policy)
       : "memory");
+}
+
+__device__ __forceinline__ uint64_t l2_evict_normal_policy() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+  return p;
 }
 
 // A place in the ring, and the parity of the mbarrier phase that its next use completes.
@@ -207,6 +214,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (any && warp == kLoadWarp) {
     // ---- loader: lane b has box b of a tile
     const int boxes = kTcKeys / box;
+    // keys that one row tile reads are first out of L2; more row tiles read them again
+    const uint64_t policy = wk.c.mt == 1 ? l2_evict_first_policy() : l2_evict_normal_policy();
     const int64_t beyond = (int64_t)a.p.n_pages * a.p.n_kv * a.p.page_size;
     // the page is loaded a tile ahead and not looked at here: a look would wait for it
     auto look_up = [&](int k) {
@@ -240,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane < boxes) {
           const uint32_t dst = smem_u32(smem + L::kRing + at.s * L::kTile) + (uint32_t)(lane * box * 128);
 #pragma unroll
-          for (int b = 0; b < HD / 64; ++b) tma_2d(dst + b * kBlk, kv ? &tv : &tk, b * 64, row, &B.full[at.s]);
+          for (int b = 0; b < HD / 64; ++b) tma_2d(dst + b * kBlk, kv ? &tv : &tk, b * 64, row, &B.full[at.s], policy);
         }
         at.step(1);
       }
