@@ -28,21 +28,6 @@ struct PagedWork {
   int shared_per, shared_split;
 };
 
-// A launch that may begin while the kernel before it in the stream still runs:
-// the kernel waits (pdl_wait) before it reads or writes anything but its own
-// shared and tensor memory.
-inline void overlapped(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& at, unsigned grid, int threads, int smem, cudaStream_t st) {
-  cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-}
-
 // The shared part of a batch of many rows, on tcgen05 (paged_attn_tc.cu):
 // tiles of kTcRows rows and kTcKeys positions, one worker a CTA.
 constexpr int kTcRows = 256, kTcKeys = 128;

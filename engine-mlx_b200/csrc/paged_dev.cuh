@@ -39,4 +39,19 @@ __device__ __forceinline__ int warp_find_seq(const int* indptr, int n_seqs, int 
   return lo;
 }
 
+// A launch that may begin while the kernel before it in the stream still runs:
+// the kernel waits (pdl_wait) before it reads or writes anything but its own
+// shared and tensor memory.
+inline void overlapped(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& at, unsigned grid, int threads, int smem, cudaStream_t st) {
+  cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+}
+
 }  // namespace emx

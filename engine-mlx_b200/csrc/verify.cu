@@ -16,9 +16,10 @@
 // and, after a refusal, V of q, once; that stream bounds a batch, and one
 // sequence the latency of its chain (drafts -> their p and q -> the row ->
 // the sums of all CTAs -> the token).  A thread-block cluster has a sequence:
-// each CTA a slice of the vocabulary, each warp a run of it, the sums meet in
-// distributed shared memory, and the one warp whose run the token lies in
-// walks it again (out of L2) with a running sum.
+// each CTA a slice of the vocabulary, each warp a run of it.  Every CTA stores
+// its sum in all CTAs' shared memory before the one cluster barrier, so nothing
+// remote is touched behind it; the CTA whose slice holds the token then walks
+// the run of the warp that does, all its threads together, out of L2.
 #include <cooperative_groups.h>
 
 #include "paged.cuh"
@@ -29,8 +30,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
+constexpr int kMost = 16;  // CTAs of a cluster
 
 template <typename T>
 __device__ __forceinline__ float val(T v);
@@ -46,57 +46,56 @@ __device__ __forceinline__ float val<bf16>(bf16 v) {
 // Mass of a value: nothing but a positive, finite one has any.
 __device__ __forceinline__ double mass(float v) { return v > 0.f && v < INFINITY ? (double)v : 0.0; }
 
-// r at one index: p there, less what the draft had.
-__device__ __forceinline__ double rest(float p, float q) {
-  const double d = mass(p) - mass(q);
-  return d > 0.0 ? d : 0.0;
-}
-
-// Values [at, at + VEC) of a row, one vector load where VEC > 1.
+// Sixteen bytes of a row (VEC values), or one value.
 template <typename T, int VEC>
-__device__ __forceinline__ void load(const T* row, int at, float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    v[0] = val<T>(row[at]);
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(row + at);
+struct Raw {
+  uint4 u;
+  __device__ __forceinline__ void load(const T* p) { u = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ float get(int e) const {
     const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (sizeof(T) == 4) {
-        v[e] = __uint_as_float(x[e]);
-      } else {
-        v[2 * e] = __uint_as_float(x[e] << 16);
-        v[2 * e + 1] = __uint_as_float(x[e] & 0xffff0000u);
-      }
-    }
+    if constexpr (sizeof(T) == 4) return __uint_as_float(x[e]);
+    else return __uint_as_float(e & 1 ? x[e >> 1] & 0xffff0000u : x[e >> 1] << 16);
   }
-}
-
-struct Shared {
-  int accepted, count, stop;
-  double warp_sum[kWarps];
-  double sum;  // of this CTA's slice, read by the cluster
+};
+template <typename T>
+struct Raw<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ float get(int) const { return val<T>(v); }
 };
 
-// r over [at, at + VEC) of the row, after `how`: 0 p alone, 1 p - q, 2 p less 1 at the index `one`.
-template <typename T, int VEC>
-__device__ __forceinline__ void rests(const T* p, const T* q, int how, int one, int at, double (&r)[VEC]) {
-  float a[VEC];
-  load<T, VEC>(p, at, a);
-  if (how == 1) {
-    float b[VEC];
-    load<T, VEC>(q, at, b);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) r[e] = rest(a[e], b[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) r[e] = how == 2 && at + e == one ? rest(a[e], 1.f) : mass(a[e]);
-  }
+// r at one index: p there, less q (both finite and not negative or without
+// mass); in fp64 exact wherever their exponents are within 29 of each other.
+__device__ __forceinline__ double rest(float p, float q) {
+  const double a = mass(p), b = mass(q);
+  return a > b ? a - b : 0.0;
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
-  __shared__ Shared S;
+template <int WARPS>
+struct Shared {
+  int accepted, count;
+  double warp_sum[WARPS];
+  double cta_sum[2][kMost];  // of the cluster's CTAs, by turn
+  double scan[WARPS];
+  int found;
+};
+
+// Inclusive sum over the lanes.
+__device__ __forceinline__ double warp_scan(double v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
+
+template <typename T, int VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const VerifyArgs a) {
+  constexpr int kWarps = THREADS / 32;
+  constexpr int kTile = 32 * VEC;  // values of one step of a warp
+  __shared__ Shared<kWarps> S;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const int i = blockIdx.x / parts;
@@ -106,6 +105,11 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
   const float* u = a.uniforms + (size_t)i * (m + 1);
   const T* target = static_cast<const T*>(a.target) + (size_t)i * (m + 1) * a.vocab;
   const T* draft = a.draft ? static_cast<const T*>(a.draft) + (size_t)i * m * a.vocab : nullptr;
+  // nobody stores into a CTA that has not begun: arrives here, waits before the stores
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  auto all_began = [] { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); };
+  pdl_wait();
+  pdl_trigger();
 
   // ---- the accepted drafts (every CTA of the cluster finds them for itself)
   if (warp == 0) {
@@ -135,6 +139,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
     if (lane == 0) {
       S.accepted = n;
       S.count = count;
+      S.found = -1;
     }
   }
   __syncthreads();
@@ -142,180 +147,170 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
   int* out = a.out + (size_t)i * (m + 1);
   if (count < 0) {  // an empty slot
     if (part == 0) {
-      for (int j = tid; j <= m; j += kThreads) out[j] = -1;
+      for (int j = tid; j <= m; j += THREADS) out[j] = -1;
       if (tid == 0) a.accepted[i] = 0;
     }
+    all_began();
     return;  // the whole cluster
   }
   if (part == 0) {
-    for (int j = tid; j <= m; j += kThreads)
+    for (int j = tid; j <= m; j += THREADS)
       if (j != n) out[j] = j < n ? tokens[j] : -1;
     if (tid == 0) a.accepted[i] = n;
   }
 
-  // ---- this warp's run [b, e) of the row
+  // ---- the sums: this warp's run is [begin(run), begin(run + 1)) of the row
   const T* p = target + (size_t)n * a.vocab;
   const T* q = draft && n < count ? draft + (size_t)n * a.vocab : nullptr;
   const int one = !draft && n < count ? tokens[n] : -1;
-  constexpr int kTile = 32 * VEC;
   const int tiles = (a.vocab + kTile - 1) / kTile, each = (tiles + parts * kWarps - 1) / (parts * kWarps);
-  const int run = part * kWarps + warp;
-  const int b = min((int64_t)run * each, (int64_t)tiles) * kTile;
-  const int e = min(min((int64_t)(run + 1) * each, (int64_t)tiles) * kTile, (int64_t)a.vocab);
-  for (int how = n < count ? (draft ? 1 : 2) : 0;; how = 0) {
+  auto begin = [&](int run) { return (int)min((int64_t)run * each * kTile, (int64_t)a.vocab); };
+  const int b = begin(part * kWarps + warp), e = begin(part * kWarps + warp + 1);
+  // r of value x of a vector at `at`; minus: p - q, else p (less 1 at the draft)
+  auto r_of = [&](const Raw<T, VEC>& x, const Raw<T, VEC>& y, bool minus, bool certain, int at, int k) {
+    return minus ? rest(x.get(k), y.get(k)) : certain && at + k == one ? rest(x.get(k), 1.f) : mass(x.get(k));
+  };
+  for (int turn = 0;; ++turn) {
+    const bool minus = turn == 0 && q, certain = turn == 0 && one >= 0;
+    constexpr int U = sizeof(T) == 4 ? 4 : 2;  // steps whose loads are in flight together
     double sum = 0.0;
-    int at = b + lane * VEC;
-    // four tiles' loads in flight
-    for (; at + 3 * kTile + VEC <= e; at += 4 * kTile) {
-      double r[4][VEC];
+    for (int at0 = b + lane * VEC; at0 < e; at0 += U * kTile) {
+      Raw<T, VEC> x[U], y[U];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) rests<T, VEC>(p, q, how, one, at + k * kTile, r[k]);
+      for (int k = 0; k < U; ++k) {
+        if (at0 + k * kTile < e) {  // VEC divides the vocabulary, and the runs' ends
+          x[k].load(p + at0 + k * kTile);
+          if (minus) y[k].load(q + at0 + k * kTile);
+        }
+      }
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < U; ++k)
+        if (at0 + k * kTile < e)
 #pragma unroll
-        for (int x = 0; x < VEC; ++x) sum += r[k][x];
-    }
-    for (; at + VEC <= e; at += kTile) {  // VEC divides the vocabulary
-      double r[VEC];
-      rests<T, VEC>(p, q, how, one, at, r);
-#pragma unroll
-      for (int x = 0; x < VEC; ++x) sum += r[x];
+          for (int v = 0; v < VEC; ++v) sum += r_of(x[k], y[k], minus, certain, at0 + k * kTile, v);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) S.warp_sum[warp] = sum;
     __syncthreads();
-    if (tid == 0) {
-      double t = 0.0;
-      for (int k = 0; k < kWarps; ++k) t += S.warp_sum[k];
-      S.sum = t;
-    }
+    // every warp has the CTA's warps' running sums in its lanes
+    const double w_sum = lane < kWarps ? S.warp_sum[lane] : 0.0, w_incl = warp_scan(w_sum);
+    const double cta = __shfl_sync(0xffffffffu, w_incl, kWarps - 1);
+    if (turn == 0) all_began();
+    if (tid < parts) *cluster.map_shared_rank(&S.cta_sum[turn & 1][part], tid) = cta;
     cluster.sync();
-    // every warp takes the sums of all CTAs, in order
-    double before = 0.0, total = 0.0;
-    int last = -1;  // the last CTA with any mass
-    for (int k = 0; k < parts; ++k) {
-      const double t = *cluster.map_shared_rank(&S.sum, k);
-      if (k < part) before += t;
-      total += t;
-      if (t > 0.0) last = k;
+    // ... and, in the same way, the cluster's CTAs'
+    const double c_sum = lane < parts ? S.cta_sum[turn & 1][lane] : 0.0, c_incl = warp_scan(c_sum);
+    const double total = __shfl_sync(0xffffffffu, c_incl, 31);
+    if (!(total > 0.0)) {
+      if (minus || certain) continue;  // nothing left of p - q: p itself
+      if (part == 0 && tid == 0) out[n] = -1;  // no mass at all
+      return;
     }
-    if (total <= 0.0) {
-      if (how == 0) {
-        if (part == 0 && tid == 0) out[n] = -1;  // no mass at all
-        break;
-      }
-      cluster.sync();  // all have read the sums of this turn
-      continue;        // nothing left of p - q: p itself
-    }
-    // The token's CTA is the first whose end passes the goal (the last with
-    // mass if rounding leaves none), its warp and index likewise.
+    // The token's CTA is the first whose running sum passes the goal (where
+    // rounding leaves none, the last with mass), its warp and index likewise.
     const double goal = (double)u[m] * total;
-    int mine = 0;
-    if (before + S.sum > goal || part == last) {
-      bool earlier = false;  // does an earlier CTA's end pass it?
-      double end = 0.0;
-      for (int k = 0; k < part; ++k) {
-        end += *cluster.map_shared_rank(&S.sum, k);
-        earlier |= end > goal;
+    const unsigned c_past = __ballot_sync(0xffffffffu, lane < parts && c_sum > 0.0 && c_incl > goal);
+    const unsigned c_any = __ballot_sync(0xffffffffu, c_sum > 0.0);
+    const int owner = c_past ? __ffs(c_past) - 1 : 31 - __clz(c_any);
+    if (owner != part) return;
+    const double before = __shfl_sync(0xffffffffu, c_incl - c_sum, part);
+    const unsigned w_past = __ballot_sync(0xffffffffu, lane < kWarps && before + w_incl > goal && w_sum > 0.0);
+    const unsigned w_any = __ballot_sync(0xffffffffu, w_sum > 0.0);
+    const int run = w_past ? __ffs(w_past) - 1 : 31 - __clz(w_any);
+    double base = before + __shfl_sync(0xffffffffu, w_incl - w_sum, run);
+    const int rb = begin(part * kWarps + run), re = begin(part * kWarps + run + 1);
+    // ---- the index: the CTA walks the run, VEC values a thread
+    int fallback = -1;
+    for (int c0 = rb; c0 < re; c0 += THREADS * VEC) {
+      const int at = c0 + tid * VEC;
+      double r[VEC];
+      double own = 0.0;
+      Raw<T, VEC> x, y;
+      if (at < re) {
+        x.load(p + at);
+        if (minus) y.load(q + at);
       }
-      mine = !earlier && S.sum > 0.0;
-    }
-    if (mine) {
-      double from = before;
-      int at_warp = -1, last_warp = -1;
-      double start = 0.0;
-      for (int k = 0; k < kWarps; ++k) {
-        const double t = S.warp_sum[k];
-        if (t > 0.0) {
-          last_warp = k;
-          if (at_warp < 0 && from + t > goal) {
-            at_warp = k;
-            start = from;
-          }
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        r[v] = at < re ? r_of(x, y, minus, certain, at, v) : 0.0;
+        own += r[v];
+      }
+      const double incl = warp_scan(own);
+      if (lane == 31) S.scan[warp] = incl;
+      __syncthreads();
+      const double ws = lane < kWarps ? S.scan[lane] : 0.0, wi = warp_scan(ws);
+      double s = base + __shfl_sync(0xffffffffu, wi - ws, warp) + (incl - own);
+      int hit = -1, last = -1;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        s += r[v];
+        if (r[v] > 0.0) {
+          last = at + v;
+          if (hit < 0 && s > goal) hit = at + v;
         }
-        from += t;
       }
-      if (at_warp < 0) {
-        at_warp = last_warp;
-        start = INFINITY;  // rounding: the last index with mass
-      }
-      if (warp == at_warp) {
-        int found = -1, fallback = -1;
-        double base = start;
-        for (int t0 = b; t0 < e && found < 0; t0 += kTile) {
-          const int at2 = t0 + lane * VEC;
-          double r[VEC];
-          if (at2 + VEC <= e) {
-            rests<T, VEC>(p, q, how, one, at2, r);
-          } else {
+      // the first index past the goal; where there is none in the run, the last with mass
+      if (hit >= 0) atomicMin(reinterpret_cast<unsigned*>(&S.found), (unsigned)hit);  // -1: the largest
 #pragma unroll
-            for (int x = 0; x < VEC; ++x) r[x] = 0.0;
-          }
-          double own = 0.0;
-          int lastx = -1;
-#pragma unroll
-          for (int x = 0; x < VEC; ++x) {
-            own += r[x];
-            if (r[x] > 0.0) lastx = at2 + x;
-          }
-          double incl = own;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double v = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += v;
-          }
-          if (start < INFINITY) {
-            double s = base + (incl - own);
-            int hit = -1;
-#pragma unroll
-            for (int x = 0; x < VEC; ++x) {
-              s += r[x];
-              if (hit < 0 && r[x] > 0.0 && s > goal) hit = at2 + x;
-            }
-            const unsigned who = __ballot_sync(0xffffffffu, hit >= 0);
-            if (who) found = __shfl_sync(0xffffffffu, hit, __ffs(who) - 1);
-            base += __shfl_sync(0xffffffffu, incl, 31);
-          }
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) lastx = max(lastx, __shfl_xor_sync(0xffffffffu, lastx, o));
-          fallback = max(fallback, lastx);
-        }
-        if (lane == 0) out[n] = found >= 0 ? found : fallback;
-      }
+      for (int o = 16; o > 0; o >>= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+      fallback = max(fallback, last);
+      base += __shfl_sync(0xffffffffu, wi, kWarps - 1);
+      __syncthreads();  // found is there; scan may be written again
+      if (S.found >= 0) break;
     }
-    break;
+    if (S.found < 0) {
+      // (all threads are here: found is the same for them)
+      if (lane == 0) S.scan[warp] = (double)fallback;
+      __syncthreads();
+      if (tid == 0) {
+        for (int k = 0; k < kWarps; ++k) fallback = max(fallback, (int)S.scan[k]);
+        out[n] = fallback;
+      }
+    } else if (tid == 0) {
+      out[n] = S.found;
+    }
+    return;
   }
-  cluster.sync();  // no CTA leaves while another may read its sum
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, int THREADS>
 cudaError_t run(const VerifyArgs& a, int parts, cudaStream_t st) {
   static cudaError_t once =
-      cudaFuncSetAttribute(verify_kernel<T, VEC>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      cudaFuncSetAttribute(verify_kernel<T, VEC, THREADS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (once != cudaSuccess) return once;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.n_seqs * parts));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(THREADS);
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)parts;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, verify_kernel<T, VEC>, a);
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, verify_kernel<T, VEC, THREADS>, a);
+}
+
+template <typename T, int VEC>
+cudaError_t run(const VerifyArgs& a, int num_sms, cudaStream_t st) {
+  // few sequences: sixteen CTAs of 512 threads each, so that a thread's share of
+  // the row is a load or two; many: eight of 256, four on an SM, so that one's
+  // chain of latencies passes under the others' streams
+  if (a.n_seqs * 16 <= num_sms) return run<T, VEC, 512>(a, 16, st);
+  return run<T, VEC, 256>(a, 8, st);
 }
 
 }  // namespace
 
 cudaError_t verify_launch(const VerifyArgs& a, int num_sms, cudaStream_t st) {
-  const int parts = 8;
   const int vec = a.is_bf16 ? 8 : 4;
   // rows keep the first one's 16-byte alignment only if they are whole vectors long
   const bool whole = a.vocab % vec == 0 && ((reinterpret_cast<uintptr_t>(a.target) | reinterpret_cast<uintptr_t>(a.draft)) & 15) == 0;
-  if (a.is_bf16) return whole ? run<bf16, 8>(a, parts, st) : run<bf16, 1>(a, parts, st);
-  return whole ? run<float, 4>(a, parts, st) : run<float, 1>(a, parts, st);
+  if (a.is_bf16) return whole ? run<bf16, 8>(a, num_sms, st) : run<bf16, 1>(a, num_sms, st);
+  return whole ? run<float, 4>(a, num_sms, st) : run<float, 1>(a, num_sms, st);
 }
 
 }  // namespace emx
