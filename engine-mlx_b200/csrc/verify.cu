@@ -44,7 +44,7 @@ __device__ __forceinline__ float val<bf16>(bf16 v) {
 }
 
 // Mass of a value: nothing but a positive, finite one has any.
-__device__ __forceinline__ double mass(float v) { return v > 0.f && v < INFINITY ? (double)v : 0.0; }
+__device__ __forceinline__ float mass(float v) { return v > 0.f && v < INFINITY ? v : 0.f; }
 
 // Sixteen bytes of a row (VEC values), or one value.
 template <typename T, int VEC>
@@ -67,8 +67,8 @@ struct Raw<T, 1> {
 // r at one index: p there, less q (both finite and not negative or without
 // mass); in fp64 exact wherever their exponents are within 29 of each other.
 __device__ __forceinline__ double rest(float p, float q) {
-  const double a = mass(p), b = mass(q);
-  return a > b ? a - b : 0.0;
+  const float a = mass(p), b = mass(q);
+  return a > b ? (double)a - (double)b : 0.0;
 }
 
 template <int WARPS>
@@ -168,12 +168,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
   const int b = begin(part * kWarps + warp), e = begin(part * kWarps + warp + 1);
   // r of value x of a vector at `at`; minus: p - q, else p (less 1 at the draft)
   auto r_of = [&](const Raw<T, VEC>& x, const Raw<T, VEC>& y, bool minus, bool certain, int at, int k) {
-    return minus ? rest(x.get(k), y.get(k)) : certain && at + k == one ? rest(x.get(k), 1.f) : mass(x.get(k));
+    return minus ? rest(x.get(k), y.get(k)) : certain && at + k == one ? rest(x.get(k), 1.f) : (double)mass(x.get(k));
   };
   for (int turn = 0;; ++turn) {
     const bool minus = turn == 0 && q, certain = turn == 0 && one >= 0;
-    constexpr int U = sizeof(T) == 4 ? 4 : 2;  // steps whose loads are in flight together
-    double sum = 0.0;
+    constexpr int U = 4;  // steps whose loads are in flight together
+    double sums[U] = {};  // one chain of additions would take longer than the loads
     for (int at0 = b + lane * VEC; at0 < e; at0 += U * kTile) {
       Raw<T, VEC> x[U], y[U];
 #pragma unroll
@@ -187,8 +187,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
       for (int k = 0; k < U; ++k)
         if (at0 + k * kTile < e)
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) sum += r_of(x[k], y[k], minus, certain, at0 + k * kTile, v);
+          for (int v = 0; v < VEC; ++v) sums[k] += r_of(x[k], y[k], minus, certain, at0 + k * kTile, v);
     }
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < U; ++k) sum += sums[k];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) S.warp_sum[warp] = sum;
@@ -296,10 +299,14 @@ cudaError_t run(const VerifyArgs& a, int parts, cudaStream_t st) {
 
 template <typename T, int VEC>
 cudaError_t run(const VerifyArgs& a, int num_sms, cudaStream_t st) {
-  // few sequences: sixteen CTAs of 512 threads each, so that a thread's share of
-  // the row is a load or two; many: eight of 256, four on an SM, so that one's
-  // chain of latencies passes under the others' streams
+  // As many threads as there is room for, so that a thread's share of the row is
+  // a load or two: sixteen CTAs of 512 a sequence while each has an SM of its own
+  // (one sequence of 151936: 7.2 us, with eight 9.4), then eight (16 sequences:
+  // 12.2 us, of 256 threads 13.5).  Beyond that eight of 256, four on an SM, so
+  // that one's chain of latencies passes under the others' streams (64 sequences:
+  // 24.7 us, of 512 threads 29.1).
   if (a.n_seqs * 16 <= num_sms) return run<T, VEC, 512>(a, 16, st);
+  if (a.n_seqs * 8 <= num_sms) return run<T, VEC, 512>(a, 8, st);
   return run<T, VEC, 256>(a, 8, st);
 }
 
