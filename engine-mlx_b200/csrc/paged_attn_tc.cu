@@ -22,8 +22,10 @@
 // Each group is a stream of its own — S, P and O in tensor memory, its Q tile
 // in shared memory: two row tiles against the same keys where the segment has
 // more than 128 rows, else the same rows against alternate key tiles (then the
-// two halves join at the segment's end).  While one group takes exponentials
-// the tensor pipe works for the other.
+// two halves join at the segment's end).  A tile's S comes in two halves of 64
+// keys: while a group takes one half's exponentials the tensor pipe adds the
+// other's products to O and computes that half of the next tile's S in its
+// place, so the group finds its next S ready.
 //
 // The maximum that the exponentials use moves only when a tile's exceeds it by
 // more than 2^8 (then O and l are rescaled); O / l does not depend on it.  P is
@@ -43,7 +45,7 @@ constexpr int kThreads = 352;
 constexpr int kSlots = 5;
 constexpr int kMmaWarp = 8, kLoadWarp = 10;
 constexpr float kRescale = 8.0f;
-constexpr uint32_t kCols = 512;  // S of the groups at 0 and 128 (P over its upper half), O at 256 and 384
+constexpr uint32_t kCols = 512;  // S of the groups at 0 and 128 (P of a half over its first 32 columns), O at 256 and 384
 constexpr int kValid = 4;        // tiles whose key masks are kept: a tile's V slot is free before the ring holds 3 later ones
 
 template <int HD>
@@ -58,9 +60,9 @@ struct Smem {
 
 struct Bars {
   uint64_t full[kSlots], empty[kSlots];
-  uint64_t q_full[2], s_full[2], p_full[2];
-  uint64_t o_full[2];  // a segment's last product is in O
-  uint64_t turn[2];
+  uint64_t q_full[2];
+  uint64_t s_full[2][2], p_full[2][2];  // by group and half
+  uint64_t pv_done[2][2];               // a half's products (and all before) are in O
   uint32_t tmem;
   alignas(16) unsigned char valid[kValid][16];  // by tile of the share, bit j: key j is there
 };
@@ -181,10 +183,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int g = 0; g < 2; ++g) {
         mbar_init(&B.q_full[g], 128);
-        mbar_init(&B.s_full[g], 2);
-        mbar_init(&B.p_full[g], 128);
-        mbar_init(&B.o_full[g], 1);
-        mbar_init(&B.turn[g], 1);
+        for (int x = 0; x < 2; ++x) {
+          mbar_init(&B.s_full[g][x], 2);
+          mbar_init(&B.p_full[g][x], 128);
+          mbar_init(&B.pv_done[g][x], 1);
+        }
       }
       fence_mbar_init();
     }
@@ -264,10 +267,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (any && warp >= kMmaWarp) {
     if (lane == 0) {
-      // ---- MMA issuer of group g.  A tile's S = Q K^T follows the O += P V of the group's tile before (P lies over S; the
-      // MMAs of a thread run in the order of their issue), so S of a tile also says that O holds all before it.
+      // ---- MMA issuer of group g.  S of a half follows the products of that half of the group's tile before (P lies
+      // over S; the MMAs of a thread run in the order of their issue).
       const int g = warp - kMmaWarp;
-      constexpr uint32_t id_s = idesc(128, false), id_pv = idesc(HD, true);
+      constexpr uint32_t id_s = idesc(64, false), id_pv = idesc(HD, true);
       // operand descriptors: the low word holds the address in 16-byte units, the high word is the same for all tiles
       const uint64_t k0 = desc_kmajor(smem), mn0 = desc_mnmajor(smem);
       auto at16 = [](uint64_t d, uint32_t bytes) {
@@ -280,70 +283,66 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       const uint64_t Q = at16(k0, L::kQ + g * L::kTile);
       const uint32_t tS = tmem + 128 * g, tO = tmem + 256 + 128 * g;
-      auto qk = [&](int s) {
-        const uint64_t K = at16(k0, L::kRing + s * L::kTile);
+      auto qk = [&](int s, int half) {
+        const uint64_t K = at16(k0, L::kRing + s * L::kTile + half * 64 * 128);  // its 64 rows
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)  // 16 head dims a step: 32 bytes along the rows of a 64-column block
-          umma(tS, at16(Q, (k >> 2) * kBlk + 32 * (k & 3)), at16(K, (k >> 2) * kBlk + 32 * (k & 3)), id_s, k > 0 ? 1u : 0u);
+          umma(tS + 64 * half, at16(Q, (k >> 2) * kBlk + 32 * (k & 3)), at16(K, (k >> 2) * kBlk + 32 * (k & 3)), id_s,
+               k > 0 ? 1u : 0u);
+        umma_commit(&B.s_full[g][half]);
+        mbar_arrive(&B.s_full[g][half]);  // and the key masks, which the wait for K has seen
       };
-      auto pv = [&](int s, bool first) {
-        const uint64_t V = at16(mn0, L::kRing + s * L::kTile);
+      uint32_t p_parity = 0, seg_parity = 0;
+      auto pv = [&](int s, int half, bool first) {
+        soon(&B.p_full[g][half], p_parity);
+        tfence_after();
+        const uint64_t V = at16(mn0, L::kRing + s * L::kTile + half * 64 * 128);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)  // 16 keys a step: 8 columns of P, 16 rows of V
-          umma_ta(tO, tS + 64 + 8 * k, at16(V, k * 2048), id_pv, (k > 0 || !first) ? 1u : 0u);
-      };
-      auto s_done = [&]() {
-        umma_commit(&B.s_full[g]);
-        mbar_arrive(&B.s_full[g]);  // and the key masks, which the wait for K has seen
+        for (int k = 0; k < 4; ++k)  // 16 keys a step: 8 columns of P, 16 rows of V
+          umma_ta(tO, tS + 64 * half + 8 * k, at16(V, k * 2048), id_pv, (k > 0 || half > 0 || !first) ? 1u : 0u);
+        umma_commit(&B.pv_done[g][half]);
       };
       Slot ks{0, 0}, vs{1, 0};
-      uint32_t p_parity = 0, seg_parity = 0, turn_parity = g == 0 ? 1 : 0;
       do {
         wait(&B.q_full[g], seg_parity);
         seg_parity ^= 1;
         if (wk.pair()) {
-          // The groups take turns with a tile's PV and the next one's QK^T together: one's S is done while the other takes
-          // exponentials.  (Left alone they fell into step and both waited for the pipe, then both for the exponentials.)
-          Slot before = vs;
-          for (int t = 0; t <= wk.n; ++t) {
-            if (t < wk.n) soon(&B.full[ks.s], ks.parity);
-            if (t > 0) {
-              soon(&B.full[before.s], before.parity);
-              soon(&B.p_full[g], p_parity);
-              p_parity ^= 1;
-            }
-            soon(&B.turn[g], turn_parity);
-            turn_parity ^= 1;
-            tfence_after();
-            if (t > 0) pv(before.s, t == 1);
-            if (t < wk.n) qk(ks.s);
-            mbar_arrive(&B.turn[g ^ 1]);
-            if (t < wk.n) {
-              s_done();
+          soon(&B.full[ks.s], ks.parity);
+          tfence_after();
+          qk(ks.s, 0);
+          qk(ks.s, 1);
+          umma_commit(&B.empty[ks.s]);
+          ks.step(2);
+          for (int t = 0; t < wk.n; ++t) {
+            const bool next = t + 1 < wk.n;
+            soon(&B.full[vs.s], vs.parity);
+            if (next) soon(&B.full[ks.s], ks.parity);
+            pv(vs.s, 0, t == 0);
+            if (next) qk(ks.s, 0);
+            pv(vs.s, 1, false);
+            umma_commit(&B.empty[vs.s]);
+            if (next) {
+              qk(ks.s, 1);
               umma_commit(&B.empty[ks.s]);
+              ks.step(2);
             }
-            if (t > 0) umma_commit(&B.empty[before.s]);
-            if (t == wk.n) break;
-            before = vs;
-            ks.step(2);
+            p_parity ^= 1;
             vs.step(2);
           }
-          umma_commit(&B.o_full[g]);
         } else {
-          // alternate tiles: a product at once when its P is there, so that its V slot can be filled again
+          // alternate tiles: nothing waits for a later tile's keys, so that its V slot can be filled again soon
           for (int t = 0; t < wk.n; ++t) {
             soon(&B.full[ks.s], ks.parity);
             if ((t & 1) == g) {
               tfence_after();
-              qk(ks.s);
-              s_done();
+              qk(ks.s, 0);
+              qk(ks.s, 1);
               umma_commit(&B.empty[ks.s]);
               soon(&B.full[vs.s], vs.parity);
-              soon(&B.p_full[g], p_parity);
-              p_parity ^= 1;
-              tfence_after();
-              pv(vs.s, t < 2);
+              pv(vs.s, 0, t < 2);
+              pv(vs.s, 1, false);
               umma_commit(&B.empty[vs.s]);
+              p_parity ^= 1;
             } else {
               mbar_arrive(&B.empty[ks.s]);  // the other group's: free of this one
               soon(&B.full[vs.s], vs.parity);
@@ -352,7 +351,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             ks.step(2);
             vs.step(2);
           }
-          if (wk.n > g) umma_commit(&B.o_full[g]);
         }
       } while (wk.next(line));
     }
@@ -364,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float sl2 = fabsf(a.scale) * kLog2e;
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
     uint32_t s_parity = 0;
-    uint32_t o_parity = 0;  // bit x: of group x' next finished segment
+    uint32_t tiles = 0;     // of this group so far
     int tile = -1;          // of the share
     do {
       const bool pair = wk.pair();
@@ -402,84 +400,77 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = 0; t < wk.n; ++t) {
         ++tile;
         if (!pair && (t & 1) != g) continue;
-        wait(&B.s_full[g], s_parity);
-        s_parity ^= 1;
-        tfence_after();
-        if (busy) {
-          // keys 64-127 stay in registers between the maximum and the
-          // exponentials, keys 0-63 are read twice (128 floats would spill)
-          float sa[32], sb[32];
-          const uint4 there = *reinterpret_cast<const uint4*>(B.valid[tile % kValid]);
-          const bool all = (there.x & there.y & there.z & there.w) == 0xffffffffu;
-          auto get = [&](int c) {  // 32 c .. 32 c + 63
-            tld32(tS + 32 * c, sa);
-            tld32(tS + 32 * c + 32, sb);
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          wait(&B.s_full[g][half], s_parity);
+          tfence_after();
+          if (busy) {
+            float sa[32], sb[32];
+            tld32(tS + 64 * half, sa);
+            tld32(tS + 64 * half + 32, sb);
             wait_ld(sa);
             wait_ld(sb);
-            if (!all) {
-              const uint32_t ba = c ? there.z : there.x, bb = c ? there.w : there.y;
+            const uint2 there = *reinterpret_cast<const uint2*>(&B.valid[tile % kValid][8 * half]);
+            const uint32_t ba = there.x, bb = there.y;
+            if ((ba & bb) != 0xffffffffu) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
                 if (!(ba >> i & 1u)) sa[i] = -INFINITY;
                 if (!(bb >> i & 1u)) sb[i] = -INFINITY;
               }
             }
-          };
-          float mx0 = -INFINITY, mx1 = -INFINITY;
-          auto most = [&]() {
+            float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               mx0 = fmaxf(mx0, sa[i]);
               mx1 = fmaxf(mx1, sb[i]);
             }
-          };
-          get(0);
-          most();
-          get(2);
-          most();
-          float mx = fmaxf(mx0, mx1) * sl2;
-          if (sl2 == 0.f) mx = 0.f;
-          const bool up = mx > m + kRescale || (m == -INFINITY && mx > m);
-          if (__any_sync(0xffffffffu, up)) {
-            const float alpha = up ? ex2f(m - mx) : 1.f;  // 0 at the first tile
-            if (mine_n > 0) {  // O holds the products so far: S came after them
+            float mx = fmaxf(mx0, mx1) * sl2;
+            if (sl2 == 0.f) mx = 0.f;
+            const bool up = mx > m + kRescale || (m == -INFINITY && mx > m);
+            if (__any_sync(0xffffffffu, up)) {
+              const float alpha = up ? ex2f(m - mx) : 1.f;  // 0 at the first tile
+              if (mine_n > 0 || half > 0) {
+                // O holds all products so far: the half before's (those before it are done, S came after them)
+                wait(&B.pv_done[g][half ^ 1], half ? tiles & 1 : (tiles - 1) & 1);
+                tfence_after();
 #pragma unroll
-              for (int c = 0; c < HD / 32; ++c) {
-                float v[32];
-                tld32(tS + 256 + 32 * c, v);
-                wait_ld(v);
+                for (int c = 0; c < HD / 32; ++c) {
+                  float v[32];
+                  tld32(tS + 256 + 32 * c, v);
+                  wait_ld(v);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] *= alpha;
-                tst32(tS + 256 + 32 * c, v);
+                  for (int i = 0; i < 32; ++i) v[i] *= alpha;
+                  tst32(tS + 256 + 32 * c, v);
+                }
               }
+              l *= alpha;
+              if (up) m = mx;
             }
-            l *= alpha;
-            if (up) m = mx;
-          }
-          const float nb = m == -INFINITY ? 0.f : -m;
-          float sum0 = 0.f, sum1 = 0.f;
-          auto put = [&](int c, const float(&s)[32]) {  // P of keys 32 c .. 32 c + 31
-            uint32_t u[16];
+            const float nb = m == -INFINITY ? 0.f : -m;
+            float sum0 = 0.f, sum1 = 0.f;
+            auto put = [&](int c, const float(&s)[32]) {  // P of keys 32 c .. 32 c + 31 of the half
+              uint32_t u[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float p0 = ex2f(fmaf(s[2 * e], sl2, nb)), p1 = ex2f(fmaf(s[2 * e + 1], sl2, nb));
-              sum0 += p0;
-              sum1 += p1;
-              const __nv_bfloat162 two = __floats2bfloat162_rn(p0, p1);
-              u[e] = *reinterpret_cast<const uint32_t*>(&two);
-            }
-            tst16u(tS + 64 + 16 * c, u);
-          };
-          put(2, sa);
-          put(3, sb);
-          get(0);
-          put(0, sa);
-          put(1, sb);
-          l += sum0 + sum1;
-          tmem_wait_st_();
+              for (int e = 0; e < 16; ++e) {
+                const float p0 = ex2f(fmaf(s[2 * e], sl2, nb)), p1 = ex2f(fmaf(s[2 * e + 1], sl2, nb));
+                sum0 += p0;
+                sum1 += p1;
+                const __nv_bfloat162 two = __floats2bfloat162_rn(p0, p1);
+                u[e] = *reinterpret_cast<const uint32_t*>(&two);
+              }
+              tst16u(tS + 64 * half + 16 * c, u);
+            };
+            put(0, sa);
+            put(1, sb);
+            l += sum0 + sum1;
+            tmem_wait_st_();
+          }
+          tfence_before();
+          mbar_arrive(&B.p_full[g][half]);
         }
-        tfence_before();
-        mbar_arrive(&B.p_full[g]);
+        s_parity ^= 1;
+        ++tiles;
         ++mine_n;
       }
       // ---- the segment's pieces.  A thread has a row, and 32 rows 512 bytes apart would make 32 separate stores of 16
@@ -509,8 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       };
       if (pair) {
-        wait(&B.o_full[g], o_parity >> g & 1);
-        o_parity ^= 3;
+        wait(&B.pv_done[g][1], (tiles - 1) & 1);
         tfence_after();
         if (busy) {
 #pragma unroll
@@ -532,11 +522,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         // both groups have these rows: each joins one half of the columns
         // (maxima and sums meet where the Q tiles were: a group's last S is done, so all of its Q has been written and read)
         auto mls = [&](int x) { return reinterpret_cast<float2*>(smem + L::kQ + x * L::kTile) + r; };
-        if (mine_n > 0) *mls(g) = make_float2(m, l);
-        wait(&B.o_full[0], o_parity & 1);
-        if (wk.n > 1) wait(&B.o_full[1], o_parity >> 1 & 1);
-        o_parity ^= wk.n > 1 ? 3u : 1u;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (mine_n > 0) {
+          *mls(g) = make_float2(m, l);
+          wait(&B.pv_done[g][1], (tiles - 1) & 1);
+        }
+        tfence_before();
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // both groups' O are done
         const float2 x = *mls(0), y = wk.n > 1 ? *mls(1) : make_float2(-INFINITY, 0.f);
         asm volatile("bar.sync 1, 256;" ::: "memory");  // both have read them: the places may be used again
         tfence_after();
