@@ -9,10 +9,13 @@
 // exponentials (128 x 128 a tile, 16 an SM and clock) and the tensor pipe.
 //
 // One CTA an SM, each with an even share of the (KV head, 256 rows, 128 keys)
-// tiles in line order; eleven warps:
+// tiles in line order; twelve warps:
 //   warps 0-7  two softmax groups of 128 threads, a thread a row: S from
 //              tensor memory, the running maximum and sum, P back over S;
 //   warps 8-9  one thread each issues the MMAs of a group;
+//   warp 11    one thread waits for the slots that a half's products and the
+//              next scores read, and arrives with their P: each wait costs an
+//              issuing thread some 200 cycles of the tensor pipe;
 //   warp 10    TMA: a lane for each run of keys in one page (a box of 8 to 128
 //              rows, the largest power of two that divides the page size),
 //              into a ring of five 128-row slots (K, V, K, V, ...).  Boxes
@@ -41,9 +44,9 @@ namespace emx {
 
 namespace {
 
-constexpr int kThreads = 352;
+constexpr int kThreads = 384;
 constexpr int kSlots = 5;
-constexpr int kMmaWarp = 8, kLoadWarp = 10;
+constexpr int kMmaWarp = 8, kLoadWarp = 10, kKeyWarp = 11;
 constexpr float kRescale = 8.0f;
 constexpr uint32_t kCols = 512;  // S of the groups at 0 and 128 (P of a half over its first 32 columns), O at 256 and 384
 constexpr int kValid = 4;        // tiles whose key masks are kept: a tile's V slot is free before the ring holds 3 later ones
@@ -111,6 +114,12 @@ __device__ __forceinline__ void tst16u(uint32_t taddr, const uint32_t (&r)[16]) 
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // Waits for this thread's tensor-memory loads; what they loaded into v may be used after it only.
@@ -185,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&B.q_full[g], 128);
         for (int x = 0; x < 2; ++x) {
           mbar_init(&B.s_full[g][x], 2);
-          mbar_init(&B.p_full[g][x], 128);
+          mbar_init(&B.p_full[g][x], x == 0 ? 129 : 128);  // the first half's with its keys
           mbar_init(&B.pv_done[g][x], 1);
         }
       }
@@ -265,6 +274,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t use = (uint32_t)((2 * tile - 1 - i) / kSlots);
       mbar_wait_bounded(&B.full[at.s], use & 1, status);
     }
+  } else if (any && warp == kKeyWarp) {
+    if (lane == 0) {
+      Slot ks{0, 0}, vs{1, 0};
+      uint32_t p_parity[2] = {0, 0};
+      auto there = [&](int g) { mbar_arrive(&B.p_full[g][0]); };
+      auto passed = [&](int g) {  // before the next arrival
+        wait(&B.p_full[g][0], p_parity[g]);
+        p_parity[g] ^= 1;
+      };
+      do {
+        for (int t = 0; t < wk.n; ++t) {
+          ks.step(2);
+          wait(&B.full[vs.s], vs.parity);
+          if (wk.pair()) {
+            if (t + 1 < wk.n) wait(&B.full[ks.s], ks.parity);
+            there(0);
+            there(1);
+            passed(0);
+            passed(1);
+          } else if (t & 1) {
+            there(1);
+            passed(1);
+          } else {
+            there(0);
+            passed(0);
+          }
+          vs.step(2);
+        }
+      } while (wk.next(line));
+    }
   } else if (any && warp >= kMmaWarp) {
     if (lane == 0) {
       // ---- MMA issuer of group g.  S of a half follows the products of that half of the group's tile before (P lies
@@ -315,8 +354,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           ks.step(2);
           for (int t = 0; t < wk.n; ++t) {
             const bool next = t + 1 < wk.n;
-            soon(&B.full[vs.s], vs.parity);
-            if (next) soon(&B.full[ks.s], ks.parity);
             pv(vs.s, 0, t == 0);
             if (next) qk(ks.s, 0);
             pv(vs.s, 1, false);
@@ -338,7 +375,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               qk(ks.s, 0);
               qk(ks.s, 1);
               umma_commit(&B.empty[ks.s]);
-              soon(&B.full[vs.s], vs.parity);
               pv(vs.s, 0, t < 2);
               pv(vs.s, 1, false);
               umma_commit(&B.empty[vs.s]);
@@ -364,8 +400,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t s_parity = 0;
     uint32_t tiles = 0;     // of this group so far
     int tile = -1;          // of the share
+    // The groups of a pair take their exponentials in turn: in step (which they fall into) both want that unit at the same
+    // time and leave it idle while both load, take maxima and wait.
+    auto my_turn = [&](bool pair) {
+      if (pair) asm volatile("bar.sync %0, 256;" ::"r"(5 + g) : "memory");
+    };
+    auto your_turn = [&](bool pair) {
+      if (pair) asm volatile("bar.arrive %0, 256;" ::"r"(5 + (g ^ 1)) : "memory");
+    };
+    bool begun = false;  // group 1 gives the first turn, once
     do {
       const bool pair = wk.pair();
+      if (pair && g == 1 && !begun) {
+        your_turn(true);
+        begun = true;
+      }
       const int h = wk.c.head();
       const int base = (wk.c.seg - h * wk.c.mt) * kTcRows + (pair ? 128 * g : 0);
       const int R = line.n_rows * line.hpg;
@@ -421,9 +470,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              mx0 = fmaxf(mx0, sa[i]);
-              mx1 = fmaxf(mx1, sb[i]);
+            for (int i = 0; i < 32; i += 2) {
+              mx0 = max3(mx0, sa[i], sa[i + 1]);
+              mx1 = max3(mx1, sb[i], sb[i + 1]);
             }
             float mx = fmaxf(mx0, mx1) * sl2;
             if (sl2 == 0.f) mx = 0.f;
@@ -461,10 +510,15 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               tst16u(tS + 64 * half + 16 * c, u);
             };
+            my_turn(pair);
             put(0, sa);
             put(1, sb);
+            your_turn(pair);
             l += sum0 + sum1;
             tmem_wait_st_();
+          } else {
+            my_turn(pair);
+            your_turn(pair);
           }
           tfence_before();
           mbar_arrive(&B.p_full[g][half]);
