@@ -122,6 +122,26 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// Two fp32 values of one register pair, and the instructions on both.
+__device__ __forceinline__ uint64_t pair32(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split32(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // Waits for this thread's tensor-memory loads; what they loaded into v may be used after it only.
 __device__ __forceinline__ void wait_ld(float (&v)[32]) {
   tmem_wait_ld_();
@@ -468,13 +488,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(bb >> i & 1u)) sb[i] = -INFINITY;
               }
             }
-            float mx0 = -INFINITY, mx1 = -INFINITY;
+            float mx0 = max3(sa[0], sa[1], sa[2]), mx1 = max3(sa[16], sa[17], sa[18]);
+            float mx2 = max3(sb[0], sb[1], sb[2]), mx3 = max3(sb[16], sb[17], sb[18]);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
+            for (int i = 3; i < 15; i += 2) {
               mx0 = max3(mx0, sa[i], sa[i + 1]);
-              mx1 = max3(mx1, sb[i], sb[i + 1]);
+              mx1 = max3(mx1, sa[16 + i], sa[17 + i]);
+              mx2 = max3(mx2, sb[i], sb[i + 1]);
+              mx3 = max3(mx3, sb[16 + i], sb[17 + i]);
             }
-            float mx = fmaxf(mx0, mx1) * sl2;
+            mx0 = max3(mx0, sa[15], sa[31]);
+            mx1 = max3(mx1, sb[15], sb[31]);
+            float mx = fmaxf(max3(mx0, mx1, mx2), mx3) * sl2;
             if (sl2 == 0.f) mx = 0.f;
             const bool up = mx > m + kRescale || (m == -INFINITY && mx > m);
             if (__any_sync(0xffffffffu, up)) {
@@ -497,14 +522,18 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (up) m = mx;
             }
             const float nb = m == -INFINITY ? 0.f : -m;
-            float sum0 = 0.f, sum1 = 0.f;
+            const uint64_t scale2 = pair32(sl2, sl2), base2 = pair32(nb, nb);
+            uint64_t sum0 = 0, sum1 = 0;  // pairs of sums
             auto put = [&](int c, const float(&s)[32]) {  // P of keys 32 c .. 32 c + 31 of the half
               uint32_t u[16];
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
-                const float p0 = ex2f(fmaf(s[2 * e], sl2, nb)), p1 = ex2f(fmaf(s[2 * e + 1], sl2, nb));
-                sum0 += p0;
-                sum1 += p1;
+                float p0, p1;
+                split32(fma2(pair32(s[2 * e], s[2 * e + 1]), scale2, base2), p0, p1);
+                p0 = ex2f(p0);
+                p1 = ex2f(p1);
+                uint64_t& sum = e & 1 ? sum1 : sum0;
+                sum = add2(sum, pair32(p0, p1));
                 const __nv_bfloat162 two = __floats2bfloat162_rn(p0, p1);
                 u[e] = *reinterpret_cast<const uint32_t*>(&two);
               }
@@ -514,7 +543,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             put(0, sa);
             put(1, sb);
             your_turn(pair);
-            l += sum0 + sum1;
+            float l0, l1;
+            split32(add2(sum0, sum1), l0, l1);
+            l += l0 + l1;
             tmem_wait_st_();
           } else {
             my_turn(pair);
