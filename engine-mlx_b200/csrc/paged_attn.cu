@@ -23,7 +23,6 @@ namespace emx {
 
 namespace {
 
-constexpr int kKT = 16;     // keys of one step of a warp
 constexpr int kWarps = 4;   // of a CTA
 constexpr int kStages = 3;  // tiles a worker keeps, two of them in flight
 // Units of a segment's set-up (q, its pieces): a worker's share of 14 one-tile
@@ -176,40 +175,46 @@ struct Rows {
     for (int x = 16; x > 0; x >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, x));
   }
 
-  // Sixteen keys, key0 of the part the first, rows r0 .. r0 + 15 of the tiles at K and V; bit j of `there`: key j is.
-  __device__ __forceinline__ void keys16(float sl2, uint32_t K, uint32_t V, int r0, int key0, uint32_t there) {
+  // 16 G keys, key0 of the part the first, rows r0 .. r0 + 16 G - 1 of the tiles at K and V; bit j of `there`: key j is.
+  template <int G>
+  __device__ __forceinline__ void keys(float sl2, uint32_t K, uint32_t V, int r0, int key0, uint32_t there) {
+    constexpr uint32_t kAll = G == 2 ? 0xffffffffu : 0xffffu;
     const int lane = threadIdx.x & 31, col = (lane & 3) * 2;
     const float nothing = sl2 < 0.f ? INFINITY : -INFINITY;  // the score of a key that is not seen
-    float s[2][4];
+    float s[2 * G][4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 2 * G; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks) {
-      uint32_t kf[4];  // keys 0-7 (dims lo, hi), keys 8-15 (dims lo, hi)
-      ldsm4(kf, K + at<HD>(r0 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
-      mma_bf16_16816(s[0], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], kf[0], kf[1]);
-      mma_bf16_16816(s[1], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], kf[2], kf[3]);
-    }
+    for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        uint32_t kf[4];  // keys 0-7 (dims lo, hi), keys 8-15 (dims lo, hi)
+        ldsm4(kf, K + at<HD>(r0 + 16 * g + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
+        mma_bf16_16816(s[2 * g], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], kf[0], kf[1]);
+        mma_bf16_16816(s[2 * g + 1], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], kf[2], kf[3]);
+      }
     // m is the maximum of s * scale * log2 e.  Masks only where a key is missing
     // or some row does not see the whole tile.
-    const bool masked = there != 0xffffu || key0 + kKT > least;
-    uint32_t pf[4];
+    const bool cut = key0 + 16 * G > least, masked = there != kAll || cut;
+    uint32_t pf[G][4];
     bool moved = false;
     float alpha[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       if (masked) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2 * G; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int key = j * 8 + col + e;
             if (!(key0 + key < vis[b] && ((there >> key) & 1u))) s[j][2 * b + e] = nothing;
           }
       }
-      float mx = fmaxf(fmaxf(s[0][2 * b] * sl2, s[0][2 * b + 1] * sl2), fmaxf(s[1][2 * b] * sl2, s[1][2 * b + 1] * sl2));
+      float mx = fmaxf(s[0][2 * b] * sl2, s[0][2 * b + 1] * sl2);
+#pragma unroll
+      for (int j = 1; j < 2 * G; ++j) mx = fmaxf(mx, fmaxf(s[j][2 * b] * sl2, s[j][2 * b + 1] * sl2));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const float to = fmaxf(m[b], mx);
@@ -221,11 +226,11 @@ struct Rows {
       // itself, and l sums the rounded ones, so a constant V comes out exact
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 2 * G; ++j) {
         const __nv_bfloat162 two =
             __floats2bfloat162_rn(ex2f(fmaf(s[j][2 * b], sl2, -from)), ex2f(fmaf(s[j][2 * b + 1], sl2, -from)));
         const uint32_t u = *reinterpret_cast<const uint32_t*>(&two);
-        pf[b + 2 * j] = u;
+        pf[j >> 1][b + 2 * (j & 1)] = u;
         sum += __uint_as_float(u << 16) + __uint_as_float(u & 0xffff0000u);
       }
       l[b] = l[b] * alpha[b] + sum;
@@ -240,9 +245,9 @@ struct Rows {
     // some rows see further than others and V holds something not finite, the
     // products are taken one visible key at a time.
     bool odd = false;
-    if (!SHARED && key0 + kKT > least) {
+    if (!SHARED && cut) {
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i) {
+      for (int i = 0; i < G * HD / 16; ++i) {
         const uint4 u = *reinterpret_cast<const uint4*>(__cvta_shared_to_generic(V + r0 * HD * 2 + (i * 32 + lane) * 16));
         const uint32_t x[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -250,29 +255,32 @@ struct Rows {
       }
       odd = __any_sync(0xffffffffu, odd);
     }
-    if (!odd) {
 #pragma unroll
-      for (int d = 0; d < HD / 16; ++d) {
-        uint32_t vf[4];  // dims lo (keys lo, hi), dims hi (keys lo, hi)
-        ldsm4t(vf, V + at<HD>(r0 + (lane & 7) + (((lane >> 3) & 1) << 3), d * 2 + (lane >> 4)));
-        mma_bf16_16816(o[2 * d], pf[0], pf[1], pf[2], pf[3], vf[0], vf[1]);
-        mma_bf16_16816(o[2 * d + 1], pf[0], pf[1], pf[2], pf[3], vf[2], vf[3]);
-      }
-    } else {
-      for (int key = 0; key < kKT; ++key) {
-        const int from = (lane & ~3) | ((key & 7) >> 1);
+    for (int g = 0; g < G; ++g) {
+      if (!odd) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const uint32_t u = __shfl_sync(0xffffffffu, key < 8 ? pf[b] : pf[b + 2], from);
-          const float pw = (key & 1) ? __uint_as_float(u & 0xffff0000u) : __uint_as_float(u << 16);
-          const bool on = key0 + key < vis[b] && ((there >> key) & 1u);
+        for (int d = 0; d < HD / 16; ++d) {
+          uint32_t vf[4];  // dims lo (keys lo, hi), dims hi (keys lo, hi)
+          ldsm4t(vf, V + at<HD>(r0 + 16 * g + (lane & 7) + (((lane >> 3) & 1) << 3), d * 2 + (lane >> 4)));
+          mma_bf16_16816(o[2 * d], pf[g][0], pf[g][1], pf[g][2], pf[g][3], vf[0], vf[1]);
+          mma_bf16_16816(o[2 * d + 1], pf[g][0], pf[g][1], pf[g][2], pf[g][3], vf[2], vf[3]);
+        }
+      } else {
+        for (int key = 0; key < 16; ++key) {
+          const int from = (lane & ~3) | ((key & 7) >> 1);
 #pragma unroll
-          for (int d = 0; d < HD / 8; ++d) {
-            const uint32_t x =
-                *reinterpret_cast<const uint32_t*>(__cvta_shared_to_generic(V + at<HD>(r0 + key, d) + (lane & 3) * 4));
-            if (on) {
-              o[d][2 * b] = fmaf(pw, __uint_as_float(x << 16), o[d][2 * b]);
-              o[d][2 * b + 1] = fmaf(pw, __uint_as_float(x & 0xffff0000u), o[d][2 * b + 1]);
+          for (int b = 0; b < 2; ++b) {
+            const uint32_t u = __shfl_sync(0xffffffffu, key < 8 ? pf[g][b] : pf[g][b + 2], from);
+            const float pw = (key & 1) ? __uint_as_float(u & 0xffff0000u) : __uint_as_float(u << 16);
+            const bool on = key0 + 16 * g + key < vis[b] && ((there >> (16 * g + key)) & 1u);
+#pragma unroll
+            for (int d = 0; d < HD / 8; ++d) {
+              const uint32_t x = *reinterpret_cast<const uint32_t*>(
+                  __cvta_shared_to_generic(V + at<HD>(r0 + 16 * g + key, d) + (lane & 3) * 4));
+              if (on) {
+                o[d][2 * b] = fmaf(pw, __uint_as_float(x << 16), o[d][2 * b]);
+                o[d][2 * b + 1] = fmaf(pw, __uint_as_float(x & 0xffff0000u), o[d][2 * b + 1]);
+              }
             }
           }
         }
@@ -391,7 +399,7 @@ struct WarpWorker {
       cp_wait<kStages - 1>();
       __syncwarp();
       const uint32_t K = ring + stage * 2 * kTileB;
-      rows.keys16(sl2, K, K + kTileB, 0, sh.cc.k * kKeys, there[stage]);
+      rows.template keys<1>(sl2, K, K + kTileB, 0, sh.cc.k * kKeys, there[stage]);
       __syncwarp();  // the stage may be filled again
       const bool last = sh.last(), more = sh.more(line);
       fresh = last || !more;
@@ -476,9 +484,9 @@ struct CtaWorker {
       const int key0 = sh.cc.k * kKeys;
       if (rows.base < rows.R) {
 #pragma unroll 1
-        for (int i = 0; i < kKeys / 16; ++i) {
-          const uint32_t mask = there[t % (kStages + 1)][i >> 1] >> ((i & 1) * 16) & 0xffffu;
-          if (mask) rows.keys16(sl2, K, K + kTileB, i * 16, key0 + i * 16, mask);
+        for (int i = 0; i < kKeys / 32; ++i) {  // two groups of 16 keys: one's latencies pass under the other's
+          const uint32_t mask = there[t % (kStages + 1)][i];
+          if (mask) rows.template keys<2>(sl2, K, K + kTileB, i * 32, key0 + i * 32, mask);
         }
       }
       const bool last = sh.last(), more = sh.more(line);

@@ -240,6 +240,7 @@ class PagedBatch:
     def __init__(self, indptr, lengths, table, n_seqs: int, n_rows: int, max_pages: int):
         self.indptr, self.lengths, self.table = indptr, lengths, table
         self.c = PagedBatchStruct(n_seqs, n_rows, max_pages, _ptr(indptr), _ptr(lengths), _ptr(table))
+        self._workspace = {}  # sdpa_paged's bytes, by what else they depend on
 
 
 class Ctx:
@@ -251,6 +252,7 @@ class Ctx:
         self.h = h.value
         self.device = device
         self._workspace = None  # sdpa_paged's, where the caller brings none
+        self._num_sms = None
 
     def close(self):
         if self.h:
@@ -265,9 +267,11 @@ class Ctx:
 
     @property
     def num_sms(self) -> int:
-        n = C.c_int()
-        _check(lib().emx_ctx_num_sms(self.h, C.byref(n)))
-        return n.value
+        if self._num_sms is None:
+            n = C.c_int()
+            _check(lib().emx_ctx_num_sms(self.h, C.byref(n)))
+            self._num_sms = n.value
+        return self._num_sms
 
     def synchronize(self):
         _check(lib().emx_synchronize(self.h))
@@ -448,7 +452,10 @@ class Ctx:
         if out is None:
             out = self.alloc(batch.c.n_rows * n_q * kv.c.head_dim * 2)
         if workspace is None:
-            need = self.sdpa_paged_workspace(kv, batch, n_q, shared_len)
+            what = (self.num_sms, batch.c.n_rows, n_q, kv.c.n_kv, kv.c.head_dim, shared_len)
+            need = batch._workspace.get(what)
+            if need is None:
+                need = batch._workspace[what] = self.sdpa_paged_workspace(kv, batch, n_q, shared_len)
             if self._workspace is None or self._workspace.nbytes < need:
                 if self._workspace is not None:
                     self._workspace.free()
