@@ -714,9 +714,9 @@ size_t lay_out(PagedWork& w, int num_sms, unsigned char* base) {
 template <int HD, bool SHARED, template <int, bool> class W>
 cudaError_t launch_part(const PagedWork& w, int ctas, cudaStream_t st) {
   constexpr int smem = W<HD, SHARED>::kSmem;
-  static cudaError_t once =
-      cudaFuncSetAttribute(paged_attn_kernel<HD, SHARED, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (once != cudaSuccess) return once;
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = attribute(done, paged_attn_kernel<HD, SHARED, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute at;
   overlapped(cfg, at, (unsigned)ctas, kWarps * 32, smem, st);

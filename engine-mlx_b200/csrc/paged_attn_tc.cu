@@ -675,13 +675,13 @@ cudaError_t encode(CUtensorMap* map, const PagedArgs& p, const void* base, int b
 
 template <int HD>
 cudaError_t launch(const PagedWork& w, int num_sms, cudaStream_t st) {
-  static cudaError_t once = cudaFuncSetAttribute(paged_shared_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 Smem<HD>::kBytes);
-  if (once != cudaSuccess) return once;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = attribute(done, paged_shared_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD>::kBytes);
+  if (e != cudaSuccess) return e;
   int box = kTcKeys;
   while (w.a.p.page_size % box) box /= 2;
   CUtensorMap tk, tv;
-  cudaError_t e = encode(&tk, w.a.p, w.a.p.k, box);
+  e = encode(&tk, w.a.p, w.a.p.k, box);
   if (e == cudaSuccess) e = encode(&tv, w.a.p, w.a.p.v, box);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg;

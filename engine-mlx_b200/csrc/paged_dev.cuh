@@ -39,6 +39,14 @@ __device__ __forceinline__ int warp_find_seq(const int* indptr, int n_seqs, int 
   return lo;
 }
 
+// An attribute of a kernel, before its launch on the current device.
+template <typename K>
+inline cudaError_t attribute(std::atomic<uint64_t>& done, K kernel, cudaFuncAttribute which, int value) {
+  int device = -1;
+  const cudaError_t e = cudaGetDevice(&device);
+  return e != cudaSuccess ? e : once_a_device(done, device, [&] { return cudaFuncSetAttribute(kernel, which, value); });
+}
+
 // A launch that may begin while the kernel before it in the stream still runs:
 // the kernel waits (pdl_wait) before it reads or writes anything but its own
 // shared and tensor memory.

@@ -6,6 +6,8 @@
 #pragma once
 #include <stdint.h>
 
+#include <atomic>
+
 #ifdef __CUDACC__
 #define EMX_HD __host__ __device__ __forceinline__
 #else
@@ -38,6 +40,17 @@ EMX_HD SeqInfo seq_info(int a, int b, int len, int n_rows, int shared, int64_t r
   s.len = len;
   if (s.rows > 0 && (len < 0 || (int64_t)len < (int64_t)shared + s.rows || (int64_t)len > room)) s.ok = false;
   return s;
+}
+
+// What `set` sets (a kernel's attributes: 0 or an error) holds for one device,
+// so it is called until it has gone well on each; `done` has a bit for a device.
+template <typename F>
+inline auto once_a_device(std::atomic<uint64_t>& done, int device, F set) -> decltype(set()) {
+  const uint64_t bit = device >= 0 && device < 64 ? 1ull << device : 0;  // a 65th is set every time
+  if (done.load(std::memory_order_acquire) & bit) return {};
+  const auto e = set();
+  if (e == decltype(e){}) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 EMX_HD int ceil_div(int a, int b) { return (int)(((int64_t)a + b - 1) / b); }

@@ -22,7 +22,7 @@
 // the run of the warp that does, all its threads together, out of L2.
 #include <cooperative_groups.h>
 
-#include "paged.cuh"
+#include "paged_dev.cuh"
 
 namespace emx {
 
@@ -279,9 +279,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
 
 template <typename T, int VEC, int THREADS>
 cudaError_t run(const VerifyArgs& a, int parts, cudaStream_t st) {
-  static cudaError_t once =
-      cudaFuncSetAttribute(verify_kernel<T, VEC, THREADS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (once != cudaSuccess) return once;
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = attribute(done, verify_kernel<T, VEC, THREADS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.n_seqs * parts));
   cfg.blockDim = dim3(THREADS);

@@ -101,6 +101,14 @@ HARNESS = r"""
 #include "paged_plan.h"
 #include <stdio.h>
 using namespace emx;
+// The calls that once_a_device makes of `set`, which fails the first `fails` times, for devices[0..n).
+extern "C" int once(const int* devices, int n, int fails, int* made) {
+  std::atomic<uint64_t> done{0};
+  int errors = 0;
+  for (int i = 0; i < n; ++i)
+    errors += once_a_device(done, devices[i], [&] { ++made[i]; return fails-- > 0 ? 7 : 0; }) != 0;
+  return errors;
+}
 // Walks every worker's share of the line the way the kernel does.  seen[] counts the tiles in line order, pieces[] (at a
 // segment's first tile) the pieces written of it; returns 0, or where an index left its range.
 extern "C" int walk(int own, int n_seqs, int n_rows, int n_kv, int hpg, int shared, int mt, int keys, int setup, long room,
@@ -164,13 +172,26 @@ extern "C" int walk(int own, int n_seqs, int n_rows, int n_kv, int hpg, int shar
 
 
 @pytest.fixture(scope="module")
-def walk(tmp_path_factory):
+def plan(tmp_path_factory):
     d = tmp_path_factory.mktemp("plan")
     src, lib = d / "walk.cc", d / "walk.so"
     src.write_text(HARNESS)
     subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", os.path.join(ROOT, "engine-mlx_b200", "csrc"),
                     str(src), "-o", str(lib)], check=True)
-    f = C.CDLL(str(lib)).walk
+    return C.CDLL(str(lib))
+
+
+@pytest.mark.parametrize("devices,fails,made", [([0, 0, 0], 0, [1, 0, 0]), ([0, 1, 0, 1, 7], 0, [1, 1, 0, 0, 1]),
+                                                ([3, 3, 3], 1, [1, 1, 0]), ([63, 64, 64, 63], 0, [1, 1, 1, 0])])
+def test_attributes_are_set_on_every_device(plan, devices, fails, made):
+    got = (C.c_int * len(devices))()
+    assert plan.once((C.c_int * len(devices))(*devices), len(devices), fails, got) == fails
+    assert list(got) == made
+
+
+@pytest.fixture(scope="module")
+def walk(plan):
+    f = plan.walk
     f.restype = C.c_int
     f.argtypes = [C.c_int] * 9 + [C.c_long] + [C.c_void_p] * 3 + [C.c_int, C.c_int, C.c_void_p, C.c_long, C.c_void_p]
 
