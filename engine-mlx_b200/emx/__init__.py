@@ -448,7 +448,8 @@ class Ctx:
 
     def sdpa_paged(self, q, kv, batch, n_q, scale, shared_len=0, shared_pages=None, out=None, workspace=None):
         """Attention of the batch's rows, the first shared_len positions read once for all; `workspace` is a
-        Buffer of sdpa_paged_workspace bytes (by default one that the context keeps and grows)."""
+        Buffer of sdpa_paged_workspace bytes (by default one that the context keeps and grows).  Graphs that can
+        run at the same time as another call take one of their own."""
         if out is None:
             out = self.alloc(batch.c.n_rows * n_q * kv.c.head_dim * 2)
         if workspace is None:
@@ -457,10 +458,8 @@ class Ctx:
             if need is None:
                 need = batch._workspace[what] = self.sdpa_paged_workspace(kv, batch, n_q, shared_len)
             if self._workspace is None or self._workspace.nbytes < need:
-                if self._workspace is not None:
-                    self._workspace.free()
-                    self._workspace = None
-                self._workspace = self.alloc(need)
+                # the one before stays allocated until the context closes: a captured graph may hold its address
+                self._workspace = self.alloc(need if self._workspace is None else max(need, 2 * self._workspace.nbytes))
             workspace = self._workspace
         _check(lib().emx_sdpa_paged(self.h, _ptr(q), kv.c, batch.c, n_q, scale, shared_len, _ptr(shared_pages), _ptr(out),
                                     workspace.ptr, workspace.nbytes))

@@ -248,9 +248,10 @@ int emx_sdpa_paged_workspace(emx_ctx* ctx, const emx_paged_kv* kv, const emx_pag
                              size_t* bytes);
 /* Attention of a batch's rows over the paged cache: q bf16[n_rows, n_q,
  * head_dim], the row at position p attends positions 0..p of its sequence;
- * out likewise.  The first shared_len positions of every sequence with rows
- * are the pages shared_pages[shared_len / page_size] (device): they are read
- * once for the whole batch, and the tables' entries for them are not read.
+ * out likewise (it may be q itself).  The first shared_len positions of every
+ * sequence with rows are the pages shared_pages[shared_len / page_size]
+ * (device): they are read once for the whole batch, and the tables' entries
+ * for them are not read.
  * shared_len: whole pages, 0 for none; a sequence with rows has at least
  * shared_len + its rows positions.  Rows of a sequence not in order become
  * zeros, as do rows that see no page inside the cache (such a page's positions

@@ -373,3 +373,283 @@ def test_append_norm_of_large_and_zero_heads(ctx):
     x[1, 1] = emx.bf16(np.full(128, 1e18, np.float32))  # squares near fp32's end
     x[1, 4] = emx.bf16(np.full(128, 1e-18, np.float32))
     check_append(ctx, c.device(ctx))
+
+
+# ------------------------------------------------------------------------------------------- sizes and uses at the ends
+def want_without(c, hole):
+    """The definition where the positions in hole[i] of sequence i are in no page of the cache."""
+    want, size = np.zeros((c.n, c.n_q, c.hd)), np.zeros((c.n, c.n_q, c.hd))
+    each = c.n_q // c.n_kv
+    for i in range(c.n_seqs):
+        keep = np.array([p for p in range(c.lens[i]) if p not in hole[i]], int)
+        k, v = (emx.f32(x[c.table[i, keep // c.page], :, keep % c.page]).astype(np.float64) for x in (c.k, c.v))
+        for j, p in enumerate(c.positions(i)):
+            row, m = c.indptr[i] + j, keep <= p
+            if not m.any():
+                continue
+            q = emx.f32(c.q[row]).astype(np.float64).reshape(c.n_kv, each, c.hd)
+            s = np.einsum("hgd,shd->hgs", q, k[m]) * c.scale
+            w = np.exp(s - s.max(-1, keepdims=True))
+            w /= w.sum(-1, keepdims=True)
+            want[row] = np.einsum("hgs,shd->hgd", w, v[m]).reshape(c.n_q, c.hd)
+            size[row] = np.einsum("hgs,shd->hgd", w, np.abs(v[m])).reshape(c.n_q, c.hd)
+    return want, size
+
+
+def near(got, want, size):
+    return np.abs(emx.f32(got).astype(np.float64) - want) <= H * np.abs(want) + (H + 2.0 ** -11) * (size + np.abs(want))
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("page", [1, 5, 8, 20, 24, 40, 128, 256])
+@pytest.mark.parametrize("seqs", [20, 45])
+def test_many_rows_over_a_prefix_of_any_pages(ctx, page, hd, seqs):
+    """80 and 180 rows a KV head (one and two row tiles), with pages that the tiles' copies take and others."""
+    r = np.random.default_rng(page)
+    shared = page * max(1, round(400 / page))
+    rows = np.ones(seqs, int)
+    c = Case(page, rows, shared + rows + r.integers(0, 50, seqs), 8, 2, hd, page, shared, pad=1).device(ctx)
+    check_attend(c, attend(ctx, c))
+    assert c.status == 0
+
+
+@pytest.mark.parametrize("shared", [128, 320, 1040])
+def test_more_segments_than_workers(ctx, shared):
+    """64 KV heads of three row tiles: a worker goes from tiles of two rows' groups to those of one and back."""
+    r = np.random.default_rng(3)
+    c = Case(30, [1] * 300, shared + 1 + r.integers(0, 20, 300), 128, 64, 64, shared=shared).device(ctx)
+    check_attend(c, attend(ctx, c))
+
+
+@pytest.mark.parametrize("shared", [0, 48])
+def test_as_many_sequences_as_there_may_be(ctx, shared):
+    r = np.random.default_rng(4)
+    rows = r.choice([0, 1, 1, 2, 20], 1024, p=[0.2, 0.4, 0.2, 0.19, 0.01])
+    c = Case(31, rows, shared + rows + r.integers(0, 90, 1024), 4, 2, shared=shared, pad=5).device(ctx)
+    check_attend(c, attend(ctx, c))
+    assert c.status == 0
+
+
+@pytest.mark.parametrize("shared", [0, 32])
+@pytest.mark.parametrize("n_q,n_kv", [(1024, 1), (1024, 1024), (1023, 11)])
+def test_as_many_heads_as_there_may_be(ctx, n_q, n_kv, shared):
+    c = Case(32, [2, 0, 1], [shared + 40, 0, shared + 3], n_q, n_kv, 64, shared=shared, pad=1).device(ctx)
+    check_attend(c, attend(ctx, c))
+    check_append(ctx, c)
+
+
+@pytest.mark.parametrize("seqs", [1, 12, 60])
+def test_a_page_may_stand_for_several(ctx, seqs):
+    """The same page twice in a table, and twice in the prefix."""
+    c = Case(33, [1] * seqs, [200 + i for i in range(seqs)], 8, 2, shared=64)
+    c.shared_pages[2] = c.shared_pages[0]
+    c.table[:, 2] = c.shared_pages[0]
+    c.table[0, 6] = c.table[0, 5]
+    c.device(ctx)
+    check_attend(c, attend(ctx, c))
+
+
+@pytest.mark.parametrize("shared", [0, 32])
+def test_rows_before_the_first_sequence(ctx, shared):
+    """indptr may begin behind row 0."""
+    c = Case(34, [3, 2, 1], [shared + 40, shared + 21, shared + 9], 4, 2, shared=shared).device(ctx)
+    every = attend(ctx, c)
+    b = emx.PagedBatch(ctx.put(c.indptr[1:].copy()), ctx.put(np.array(c.lens[1:], np.int32)), ctx.put(c.table[1:].copy()), 2,
+                       c.n_rows, c.max_pages)
+    out = ctx.put(np.full((c.n_rows, 4, 128), 9, np.uint16))
+    ctx.sdpa_paged(c.dq, c.kv, b, 4, c.scale, shared, c.d_shared, out=out)
+    got = out.read(np.uint16, (c.n_rows, 4, 128))
+    assert ctx.device_status() == 0 and (got[:3] == 9).all()
+    assert near(got[3:], *(x[3:] for x in c.attend())).all() and near(every[:c.n], *c.attend()).all()
+    q = ctx.put(np.full((c.n_rows, 4, 128), 9, np.uint16))
+    ctx.paged_append(c.dqkv, c.kv, b, 4, out=q)
+    got = q.read(np.uint16, (c.n_rows, 4, 128))
+    assert ctx.device_status() == 0 and (got[:3] == 9).all()
+    assert np.allclose(emx.f32(got[3:]), c.append()[0][3:], rtol=H, atol=1e-4)
+
+
+@pytest.mark.parametrize("page", [16, 20])
+@pytest.mark.parametrize("seqs", [3, 20, 45])
+def test_bad_pages_of_the_prefix(ctx, seqs, page):
+    """A page of the prefix outside the cache is left out; a prefix, and then a whole batch, without a page gives zeros."""
+    c = Case(35, [1] * seqs, [20 * page + 1 + i for i in range(seqs)], 8, 2, page=page, shared=20 * page).device(ctx)
+    pages = c.shared_pages.copy()
+    pages[7], pages[19] = c.n_pages, -1
+    c.d_shared.write(pages)
+    hole = set(range(7 * page, 8 * page)) | set(range(19 * page, 20 * page))
+    got = attend(ctx, c)
+    assert c.status == 5 and near(got[:c.n], *want_without(c, [hole] * seqs)).all()
+    c.d_shared.write(np.full(20, 1 << 30, np.int32))
+    got = attend(ctx, c)
+    assert c.status == 5 and near(got[:c.n], *want_without(c, [set(range(20 * page))] * seqs)).all()
+    c.kv.c.n_pages = 0
+    got = attend(ctx, c)
+    assert c.status == 5 and (got[:c.n] == 0).all()
+
+
+def test_output_over_q(ctx):
+    for seqs, shared in ((1, 0), (40, 0), (5, 64), (40, 64)):
+        c = Case(36, [1] * seqs, [shared + 30 + 9 * i for i in range(seqs)], 8, 2, shared=shared).device(ctx)
+        want = attend(ctx, c)[:c.n]
+        ctx.sdpa_paged(c.dq, c.kv, c.batch, 8, c.scale, shared, c.d_shared, out=c.dq)
+        assert (c.dq.read(np.uint16, want.shape) == want).all()
+
+
+def test_calls_of_all_kinds_one_after_another(ctx):
+    """Nothing waits between them and one workspace serves them all: each call's kernels begin while the last one's end."""
+    cases = [Case(37, [1] * 45, [400 + i for i in range(45)], 8, 2, shared=320), Case(38, [1], [3000], 8, 2),
+             Case(39, [40, 1, 70], [60, 700, 90], 8, 2), Case(40, [1] * 3, [600, 300, 290], 8, 2, shared=256),
+             Case(41, [1] * 20, [130] * 20, 8, 2, page=20, shared=120)]
+    for c in cases:
+        c.device(ctx)
+    ws = ctx.alloc(max(ctx.sdpa_paged_workspace(c.kv, c.batch, 8, c.shared) for c in cases))
+    want = [attend(ctx, c, ws=ws) for c in cases]
+    for c, w in zip(cases, want):
+        check_attend(c, w)
+    outs = [[ctx.put(np.full(w.shape, NAN, np.uint16)) for w in want] for _ in range(6)]
+    for turn, out in enumerate(outs):
+        for i in np.random.default_rng(turn).permutation(len(cases)):
+            c = cases[i]
+            ctx.sdpa_paged(c.dq, c.kv, c.batch, 8, c.scale, c.shared, c.d_shared, out=out[i], workspace=ws)
+    for out in outs:
+        for o, w in zip(out, want):
+            assert (o.read(np.uint16, w.shape) == w).all()
+
+
+def test_two_contexts_in_two_threads(ctx):
+    import threading
+    other = emx.Ctx(0)
+    made, wrong = [], []
+    for cx, seed in ((ctx, 42), (other, 43)):
+        c = Case(seed, [1] * 40, [300 + 7 * i for i in range(40)], 16, 4, shared=160).device(cx)
+        made.append((cx, c, attend(cx, c)))
+
+    def work(cx, c, want):
+        for _ in range(30):
+            if not (attend(cx, c) == want).all():
+                wrong.append(c)
+
+    threads = [threading.Thread(target=work, args=m) for m in made]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    other.close()
+
+
+def test_offsets_past_32_bits(ctx):
+    """A cache of more than 2^32 elements, of which only some pages at both ends and in between hold anything."""
+    c = Case(44, [1, 3] + [1] * 20, [300, 90] + [70 + i for i in range(20)], 8, 2, page=128, shared=0)
+    s = Case(45, [1] * 24, [400 + i for i in range(24)], 8, 2, page=128, shared=256)
+    pages = (2 ** 32) // (2 * 128 * 128) + 64  # of 2 x 128 x 128 elements
+    k, v = (ctx.alloc(pages * 2 * 128 * 128 * 2) for _ in range(2))
+    for x in (c, s):
+        x.device(ctx)
+        assert x.n_pages <= 64
+        far = np.concatenate([np.arange(pages - 40, pages), pages // 2 + np.arange(24)])[:x.n_pages]  # page j of the case
+        for j, to in enumerate(far):
+            k.write(x.k[j], int(to) * 65536)
+            v.write(x.v[j], int(to) * 65536)
+        move = lambda t: np.where((t >= 0) & (t < x.n_pages), far[np.clip(t, 0, x.n_pages - 1)], -7).astype(np.int32)  # noqa: E731
+        x.kv = emx.PagedKV(k, v, pages, 128, 2, 128)
+        x.batch = emx.PagedBatch(x.d_indptr, x.d_lens, ctx.put(move(x.table)), x.n_seqs, x.n_rows, x.max_pages)
+        if x.shared:
+            x.d_shared = ctx.put(move(x.shared_pages))
+        check_attend(x, attend(ctx, x))
+        assert x.status == 0
+        # appended rows arrive there too
+        q = ctx.paged_append(x.dqkv, x.kv, x.batch, 8)
+        _, k_, v_ = x.append()
+        i, p = 1, x.positions(1)
+        at = far[x.table[1, p // 128]]
+        for row, pg, off in zip(range(x.indptr[1], x.indptr[2]), at, p % 128):
+            import ctypes
+            page = np.empty((2, 128, 128), np.uint16)
+            for buf, w in ((k, k_), (v, v_)):
+                assert emx.lib().emx_memcpy_d2h(ctx.h, page.ctypes.data_as(ctypes.c_void_p), buf.ptr + int(pg) * 65536, page.nbytes) == 0
+                assert np.allclose(emx.f32(page[:, off]), w[row], rtol=H, atol=1e-4)
+        q.free()
+    k.free()
+    v.free()
+
+
+def test_a_graph_keeps_the_default_workspace(ctx):
+    """A call without a workspace is captured; a larger one then makes the context's grow; the graph is replayed."""
+    torch = pytest.importorskip("torch")
+    own = emx.Ctx(0)
+    a = Case(46, [1] * 3, [300, 200, 100], 8, 2, shared=64).device(own)
+    b = Case(47, [1] * 200, [100] * 200, 32, 2, shared=64).device(own)
+    want = attend(own, a)
+    out = own.put(np.zeros(want.shape, np.uint16))
+    st, g = torch.cuda.ExternalStream(stream_of(own)), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st, capture_error_mode="thread_local"):
+        own.sdpa_paged(a.dq, a.kv, a.batch, 8, a.scale, 64, a.d_shared, out=out)
+    first = attend(own, b)
+    for _ in range(3):
+        with torch.cuda.stream(st):
+            g.replay()
+        assert (attend(own, b) == first).all()
+    own.synchronize()
+    assert (out.read(np.uint16, want.shape)[:a.n] == want[:a.n]).all()
+    del g
+    own.close()
+
+
+FIRST_IN_A_GRAPH = """
+import sys
+sys.path[:0] = sys.argv[1:]
+import ctypes as C, numpy as np, torch, emx
+from paged_case import Case, verify
+from test_verify_gpu import inputs
+ctx = emx.Ctx(0)
+c = Case(50, [2] * 30, [300 + i for i in range(30)], 8, 2, shared=64).device(ctx)
+t, d, x, u = inputs(51, 4, 3, 1000)
+buf = [ctx.put(y) for y in (t, d, x, u)]
+q = ctx.put(np.zeros((c.n, 8, 128), np.uint16))
+o = ctx.put(np.zeros((c.n, 8, 128), np.uint16))
+ws = ctx.alloc(ctx.sdpa_paged_workspace(c.kv, c.batch, 8, 64))
+out, acc = ctx.put(np.zeros((4, 4), np.int32)), ctx.put(np.zeros(4, np.int32))
+ctx.synchronize()
+def step():
+    ctx.paged_append(c.dqkv, c.kv, c.batch, 8, out=q)
+    ctx.sdpa_paged(q, c.kv, c.batch, 8, c.scale, 64, c.d_shared, out=o, workspace=ws)
+    ctx.verify_draft(*buf, 4, 3, 1000, out=out, accepted=acc)
+p = C.c_void_p()
+assert emx.lib().emx_ctx_stream(ctx.h, C.byref(p)) == 0
+st, g = torch.cuda.ExternalStream(p.value), torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=st, capture_error_mode="thread_local"):
+    step()
+read = lambda: (q.read(np.uint16, c.n * 1024), o.read(np.uint16, c.n * 1024), out.read(np.int32, (4, 4)), acc.read(np.int32, 4))
+for turn in range(3):
+    if turn:
+        r = np.random.default_rng(turn)
+        c.lens = [int(k) for k in r.integers(70, 300, 30)]
+        x, u = r.integers(0, 1000, (4, 3)).astype(np.int32), r.random((4, 4)).astype(np.float32)
+        c.d_lens.write(np.array(c.lens, np.int32)), buf[2].write(x), buf[3].write(u)
+        c.dqkv.write(c.qkv[::-1].copy() if turn == 2 else c.qkv)
+        ctx.synchronize()
+    with torch.cuda.stream(st):
+        g.replay()
+    got = read()
+    assert ctx.device_status() == 0
+    step()
+    assert all((a == b).all() for a, b in zip(got, read())) and got[1].any()
+    want = verify(t, d, x, u)
+    assert (got[2] == want[0]).all() and (got[3] == want[1]).all()
+del g
+print("as eager")
+"""
+
+
+def test_a_step_whose_first_calls_are_captured():
+    """In a process of its own, where no kernel has been launched before; then replayed as lengths, rows, drafts and
+    uniform numbers change, and compared with the same calls outside of the graph."""
+    pytest.importorskip("torch")
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_A_GRAPH, here, os.path.join(os.path.dirname(here), "engine-mlx_b200")],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "as eager" in r.stdout, r.stdout + r.stderr

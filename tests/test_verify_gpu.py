@@ -171,6 +171,41 @@ def test_tokens_are_distributed_as_the_target(ctx):
     assert (np.abs(share - p) <= 0.018).all() and share[3] == 0
 
 
+@pytest.mark.parametrize("kind", [emx.F32, emx.BF16])
+@pytest.mark.parametrize("n,m,v", [(65535, 1, 5), (2, 4096, 7), (1, 0, 1), (600, 2, 1000)])
+def test_as_many_sequences_and_drafts_as_there_may_be(ctx, n, m, v, kind):
+    t, d, x, u = inputs(n + m, n, m, v, near=0.0 if m > 100 else 0.7)
+    same(ctx, t, d if m else None, x, u, kind=kind)
+
+
+def test_rows_past_32_bits(ctx):
+    """A vocabulary of 2^30: rows of 2 GB that begin beyond 2^31 elements."""
+    torch = pytest.importorskip("torch")
+    V = 1 << 30
+    t, d = (torch.zeros(2, k, V, dtype=torch.bfloat16, device="cuda") for k in (2, 1))
+    # sequence 0: refused, and of p - q one index is left; sequence 1: accepted, and two have mass
+    t[0, 0, V // 2], t[0, 0, V - 3], d[0, 0, V // 2], d[0, 0, 5] = 0.5, 0.5, 0.5, 0.5
+    t[1, 0, V - 1], d[1, 0, V - 1], t[1, 1, V - 7], t[1, 1, V - 2] = 0.5, 0.5, 0.5, 0.5
+    x, u = torch.tensor([[5], [V - 1]], dtype=torch.int32, device="cuda"), torch.tensor([[0.1, 0.9], [0.3, 0.6]], device="cuda")
+    torch.cuda.synchronize()
+    out, acc = ctx.verify_draft(t, d, x, u, 2, 1, V, dtype=emx.BF16)
+    assert ctx.device_status() == 0
+    assert out.read(np.int32, (2, 2)).tolist() == [[V - 3, -1], [V - 1, V - 2]] and acc.read(np.int32, 2).tolist() == [0, 1]
+
+
+def test_two_contexts_verify_at_once(ctx):
+    other = emx.Ctx(0)
+    runs = []
+    for cx, seed in ((ctx, 11), (other, 12)):
+        t, d, x, u = inputs(seed, 40, 3, 20000)
+        runs.append((cx, [cx.put(y) for y in (t, d, x, u)], verify(t, d, x, u)))
+    outs = [[cx.verify_draft(*b, 40, 3, 20000) for cx, b, _ in runs] for _ in range(20)]
+    for pair in outs:
+        for (out, acc), (_, _, want) in zip(pair, runs):
+            assert (out.read(np.int32, (40, 4)) == want[0]).all() and (acc.read(np.int32, 40) == want[1]).all()
+    other.close()
+
+
 # ------------------------------------------------------------------------------------------- a step, all of it together
 def test_speculative_steps_over_a_shared_prompt(ctx):
     """Three sequences with a common prompt take four steps of speculative decoding: the drafted rows are appended
