@@ -54,6 +54,9 @@ constexpr int kValid = 4;        // tiles whose key masks are kept: a tile's V s
 template <int HD>
 struct Smem {
   static constexpr int kTile = HD / 64 * kBlk;  // 128 rows of HD
+  // K and V lie in groups of 8 rows, a group's 64-column blocks (8 rows of 128 bytes, swizzled) one after another, so
+  // that one copy brings whole rows.
+  static constexpr int kGroup = HD / 64 * 1024;
   static constexpr int kQ = 0;                  // [2]
   static constexpr int kRing = 2 * kTile;       // [kSlots]
   static constexpr int kBar = kRing + kSlots * kTile;
@@ -76,11 +79,12 @@ constexpr uint32_t idesc(int n, bool b_mn) {
          ((uint32_t)(128 >> 4) << 24);
 }
 
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar, uint64_t policy) {
+// A box of 8-row groups from group `y` of the cache on.
+__device__ __forceinline__ void tma_groups(uint32_t dst, const CUtensorMap* map, int y, uint64_t* bar, uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(
-          dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar)), "l"(policy)
+      "cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %2, %2, %3}], [%4], %5;" ::
+          "r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(y), "r"(smem_u32(bar)), "l"(policy)
       : "memory");
 }
 
@@ -279,9 +283,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive_expect_tx(&B.full[at.s], (uint32_t)L::kTile);
         __syncwarp();
         if (lane < boxes) {
-          const uint32_t dst = smem_u32(smem + L::kRing + at.s * L::kTile) + (uint32_t)(lane * box * 128);
-#pragma unroll
-          for (int b = 0; b < HD / 64; ++b) tma_2d(dst + b * kBlk, kv ? &tv : &tk, b * 64, row, &B.full[at.s], policy);
+          const uint32_t dst = smem_u32(smem + L::kRing + at.s * L::kTile) + (uint32_t)(lane * (box / 8) * L::kGroup);
+          tma_groups(dst, kv ? &tv : &tk, row / 8, &B.full[at.s], policy);
         }
         at.step(1);
       }
@@ -331,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int g = warp - kMmaWarp;
       constexpr uint32_t id_s = idesc(64, false), id_pv = idesc(HD, true);
       // operand descriptors: the low word holds the address in 16-byte units, the high word is the same for all tiles
-      const uint64_t k0 = desc_kmajor(smem), mn0 = desc_mnmajor(smem);
+      const uint64_t q0 = desc_kmajor(smem), k0 = desc_kmajor(smem, L::kGroup), v0 = desc_mnmajor(smem, 1024, L::kGroup);
       auto at16 = [](uint64_t d, uint32_t bytes) {
         return (d & 0xffffffff00000000ull) | (uint32_t)((uint32_t)d + (bytes >> 4));
       };
@@ -340,13 +343,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (mbar_test_wait(bar, parity)) return;
         wait(bar, parity);
       };
-      const uint64_t Q = at16(k0, L::kQ + g * L::kTile);
+      const uint64_t Q = at16(q0, L::kQ + g * L::kTile);
       const uint32_t tS = tmem + 128 * g, tO = tmem + 256 + 128 * g;
       auto qk = [&](int s, int half) {
-        const uint64_t K = at16(k0, L::kRing + s * L::kTile + half * 64 * 128);  // its 64 rows
+        const uint64_t K = at16(k0, L::kRing + s * L::kTile + half * 8 * L::kGroup);  // its 64 rows
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)  // 16 head dims a step: 32 bytes along the rows of a 64-column block
-          umma(tS + 64 * half, at16(Q, (k >> 2) * kBlk + 32 * (k & 3)), at16(K, (k >> 2) * kBlk + 32 * (k & 3)), id_s,
+          umma(tS + 64 * half, at16(Q, (k >> 2) * kBlk + 32 * (k & 3)), at16(K, (k >> 2) * 1024 + 32 * (k & 3)), id_s,
                k > 0 ? 1u : 0u);
         umma_commit(&B.s_full[g][half]);
         mbar_arrive(&B.s_full[g][half]);  // and the key masks, which the wait for K has seen
@@ -355,10 +358,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto pv = [&](int s, int half, bool first) {
         soon(&B.p_full[g][half], p_parity);
         tfence_after();
-        const uint64_t V = at16(mn0, L::kRing + s * L::kTile + half * 64 * 128);
+        const uint64_t V = at16(v0, L::kRing + s * L::kTile + half * 8 * L::kGroup);
 #pragma unroll
         for (int k = 0; k < 4; ++k)  // 16 keys a step: 8 columns of P, 16 rows of V
-          umma_ta(tO, tS + 64 * half + 8 * k, at16(V, k * 2048), id_pv, (k > 0 || half > 0 || !first) ? 1u : 0u);
+          umma_ta(tO, tS + 64 * half + 8 * k, at16(V, k * 2 * L::kGroup), id_pv, (k > 0 || half > 0 || !first) ? 1u : 0u);
         umma_commit(&B.pv_done[g][half]);
       };
       Slot ks{0, 0}, vs{1, 0};
@@ -653,7 +656,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
 
-// The cache's rows [n_pages * n_kv * page_size][head_dim] in boxes of 64 columns x `box` rows, 128-byte swizzle.
+// The cache's rows [n_pages * n_kv * page_size][head_dim] as [8-row groups][64-column blocks][8][64], in boxes of `box`
+// rows, 128-byte swizzle.
 cudaError_t encode(CUtensorMap* map, const PagedArgs& p, const void* base, int box) {
   std::call_once(g_encode_once, [] {
     void* fn = nullptr;
@@ -663,10 +667,11 @@ cudaError_t encode(CUtensorMap* map, const PagedArgs& p, const void* base, int b
       g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
   });
   if (!g_encode) return cudaErrorNotSupported;
-  const cuuint64_t dims[2] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.n_pages * p.n_kv * p.page_size};
-  const cuuint64_t strides[1] = {(cuuint64_t)p.head_dim * 2};
-  const cuuint32_t size[2] = {64, (cuuint32_t)box}, one[2] = {1, 1};
-  return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, size, one,
+  const cuuint64_t row = (cuuint64_t)p.head_dim * 2, blocks = p.head_dim / 64;
+  const cuuint64_t dims[4] = {64, 8, blocks, (cuuint64_t)p.n_pages * p.n_kv * p.page_size / 8};
+  const cuuint64_t strides[3] = {row, 128, 8 * row};
+  const cuuint32_t size[4] = {64, 8, (cuuint32_t)blocks, (cuuint32_t)box / 8}, one[4] = {1, 1, 1, 1};
+  return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, size, one,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
              ? cudaSuccess

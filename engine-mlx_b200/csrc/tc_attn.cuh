@@ -8,16 +8,17 @@ namespace emx {
 
 constexpr int kBlk = 128 * 64 * 2;  // 128 rows x 64 columns (128 B rows, swizzled): 16 KB
 
-__device__ __forceinline__ uint64_t desc_kmajor(const void* p) {
+// 8-row groups `group` bytes apart (SBO).
+__device__ __forceinline__ uint64_t desc_kmajor(const void* p, uint32_t group = 1024) {
   const uint64_t a = (smem_u32(p) >> 4) & 0x3FFFu;
-  return a | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+  return a | (1ull << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// MN-major operand with 128-byte swizzle: 64-element MN blocks kBlk bytes
-// apart (LBO), 8-row K groups 1024 bytes apart (SBO).
-__device__ __forceinline__ uint64_t desc_mnmajor(const void* p) {
+// MN-major operand with 128-byte swizzle: 64-element MN blocks `block` bytes
+// apart (LBO), 8-row K groups `group` bytes apart (SBO).
+__device__ __forceinline__ uint64_t desc_mnmajor(const void* p, uint32_t block = kBlk, uint32_t group = 1024) {
   const uint64_t a = (smem_u32(p) >> 4) & 0x3FFFu;
-  return a | ((uint64_t)(kBlk >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+  return a | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
 __device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
