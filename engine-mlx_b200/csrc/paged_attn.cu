@@ -30,6 +30,9 @@ constexpr int kStages = 3;  // tiles a worker keeps, two of them in flight
 constexpr int kSetup = 1;
 constexpr int kMaxSeqs = 1024;
 constexpr int kCtasPerSm = 2;
+// ns of a tcgen05 tile of 256 rows and of 128, and of an own part's unit by a
+// warp and by a CTA, of those that run beside them.
+constexpr int kPairNs = 1850, kHalfNs = 1450, kWarpNs = 1450, kCtaNs = 4000;
 
 // `policy`: first out of L2.  K and V are read once or, by a sequence's next row
 // tile, soon again; the pieces, which the join reads, are to stay.
@@ -519,13 +522,23 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const __grid_co
   } else {
     plan_starts<kWarps * 32>(w.a, line, starts, blockIdx.x == 0);
     total = starts[w.a.p.n_seqs];
-    if (blockIdx.x == 0)
-      for (int i = threadIdx.x; i <= w.a.p.n_seqs; i += kWarps * 32) w.starts[i] = starts[i];
   }
-  const int workers = gridDim.x * Worker::kPerCta;
   const int worker = Worker::kPerCta == 1 ? blockIdx.x : blockIdx.x * Worker::kPerCta + (threadIdx.x >> 5);
-  const int64_t per = SHARED ? w.shared_per : share_size(total, workers, 1);
-  if (worker * per < total) Worker::run(w, line, smem, worker, worker * per, min(total, (worker + 1) * per));
+  int64_t x0, x1;
+  if (SHARED) {
+    x0 = (int64_t)worker * w.shared_per;
+    x1 = x0 + w.shared_per;
+  } else {
+    const Shares shares = deal(total, w.own_workers, w.own_early, w.own_each);
+    x0 = shares.begin(worker);
+    x1 = shares.begin(worker + 1);
+    if (blockIdx.x == 0) {
+      for (int i = threadIdx.x; i <= w.a.p.n_seqs; i += kWarps * 32) w.starts[i] = starts[i];
+      if (threadIdx.x == 0) *w.shares = shares;
+    }
+  }
+  x1 = min(x1, total);
+  if (x0 < x1) Worker::run(w, line, smem, worker, x0, x1);
   if (!first) pdl_wait();
 }
 
@@ -565,28 +578,29 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     else s = own.seq(seq);
     const bool ok = item >= 0 && s.ok;
     // pieces of the row's segment in each part, and the slot of its second worker's
-    auto place = [&](int mt, int kt, int64_t each, int64_t per, int64_t begin, int r, uint32_t& slot) {
-      const int64_t x0 = begin + (int64_t)(r / mt) * each;
-      const int c0 = share_of(x0, per), c1 = share_of(x0 + kt - 1, per);
-      slot = (uint32_t)((c0 + 1) * mt + r % mt);
-      return c1 - c0 + 1;
-    };
     int n_all = 0, n_own = 0;
     uint32_t slot_all = 0, slot_own = 0;
     if (ok && a.shared_len > 0) {
       const SeqInfo every = all.seq(0);
-      const int kt = all.key_tiles(every);
+      const int kt = all.key_tiles(every), r = row * hpg + g, tile = share_of(r, w.shared_mt);
       // with workers of their own, shared segments are as long as those workers' shares
       const int64_t each = w.shared_split ? (int64_t)w.shared_split * w.shared_per : kt;
-      n_all = place(w.shared_mt, kt, each, w.shared_per, (int64_t)h * all.row_tiles(every) * each, row * hpg + g, slot_all);
+      const int64_t x0 = ((int64_t)h * all.row_tiles(every) + tile) * each;
+      const int c0 = share_of(x0, w.shared_per), c1 = share_of(x0 + kt - 1, w.shared_per);
+      slot_all = (uint32_t)((c0 + 1) * w.shared_mt + r - tile * w.shared_mt);
+      n_all = c1 - c0 + 1;
     }
+    const int r_own = ok ? (row - s.row0) * hpg + g : 0, tile_own = share_of(r_own, w.own_mt);
     const int kt_own = ok ? own.key_tiles(s) : 1;
-    const int64_t x_own = ok ? (int64_t)h * own.row_tiles(s) * (kt_own + kSetup) + kSetup : 0;
+    const int64_t x_own = ok ? ((int64_t)h * own.row_tiles(s) + tile_own) * (kt_own + kSetup) + kSetup : 0;
     if (!waited) pdl_wait();
     waited = true;
     if (ok) {
-      const int64_t per = share_size(w.starts[a.p.n_seqs], w.own_workers, 1);
-      n_own = place(w.own_mt, kt_own, kt_own + kSetup, per, w.starts[seq] + x_own, (row - s.row0) * hpg + g, slot_own);
+      const Shares shares = *w.shares;
+      const int64_t x0 = w.starts[seq] + x_own;
+      const int c0 = shares.of(x0), c1 = shares.of(x0 + kt_own - 1);
+      slot_own = (uint32_t)((c0 + 1) * w.own_mt + r_own - tile_own * w.own_mt);
+      n_own = c1 - c0 + 1;
       if (a.shared_len == 0 && n_own == 1) item = -1;  // one worker had the segment whole and wrote it
     }
     // ---- item by item
@@ -697,6 +711,7 @@ size_t lay_out(PagedWork& w, int num_sms, unsigned char* base) {
     return q;
   };
   w.starts = static_cast<int64_t*>(take(sizeof(int64_t) * (kMaxSeqs + 1)));
+  w.shares = static_cast<Shares*>(take(sizeof(Shares)));
   auto pieces = [&](Pieces& pc, size_t rows) {
     pc.first_o = static_cast<float*>(take(heads * p.head_dim * sizeof(float)));
     pc.first_ml = static_cast<float2*>(take(heads * sizeof(float2)));
@@ -730,40 +745,46 @@ cudaError_t launch(PagedWork& w, int num_sms, cudaStream_t st) {
   const PagedArgs& p = w.a.p;
   const int64_t rows = (int64_t)p.n_rows * (p.n_q / p.n_kv);  // of a KV head
   const int ctas = num_sms * kCtasPerSm;
+  // The own part by warps up to 16 rows a sequence and KV head, on average;
+  // beyond that a warp's 16 keys would be loaded again for every 16 rows.
+  const bool by_warp = rows <= Few::kRows * (int64_t)p.n_seqs;
+  w.own_mt = by_warp ? Few::kRows : Many::kRows;
+  w.own_keys = by_warp ? Few::kKeys : Many::kKeys;
+  const int own_per_sm = kCtasPerSm * (by_warp ? Few::kPerCta : 1);
+  w.own_workers = num_sms * own_per_sm;
   cudaError_t e = cudaSuccess;
   if (w.a.shared_len > 0) {
     // tcgen05 from 17 rows a head on, where it takes the pages
     const bool few = rows <= Few::kRows, tc = !few && paged_shared_tc_takes(p);
     w.shared_mt = few ? Few::kRows : tc ? kTcRows : Many::kRows;
     w.shared_keys = few ? Few::kKeys : tc ? kTcKeys : Many::kKeys;
-    w.shared_workers = few ? ctas * Few::kPerCta : tc ? num_sms : ctas;
+    const int workers = few ? ctas * Few::kPerCta : tc ? num_sms : ctas;
     const int kt = ceil_div(w.a.shared_len, w.shared_keys);
-    const int64_t segments = (int64_t)p.n_kv * ((rows + w.shared_mt - 1) / w.shared_mt);
-    w.shared_per = (int)share_size(segments * kt, w.shared_workers, 1);
-    w.shared_split = 0;
-    if (tc && segments <= w.shared_workers) {
-      // A worker that goes from one segment to the next stores one's rows and
-      // loads the other's Q with nothing to compute meanwhile: about four
-      // tiles' time.  Whole workers to a segment where the tiles that costs are
-      // fewer (64 rows a head on 32768: 15 tiles against 14 and a change).
-      const int split = (int)(w.shared_workers / segments), per = ceil_div(kt, split);
-      if (per <= w.shared_per + 4) {
-        w.shared_split = split;
-        w.shared_per = per;
+    const int64_t segments = (int64_t)p.n_kv * ceil_div(rows, w.shared_mt);
+    w.shared_per = ceil_div(segments * kt, workers);
+    if (tc) {
+      if (segments <= workers) {
+        // A worker that goes from one segment to the next stores one's rows and
+        // loads the other's Q with nothing to compute meanwhile: about four
+        // tiles' time.  Whole workers to a segment where the tiles that costs are
+        // fewer (64 rows a head on 32768: 15 tiles against 14 and a change).
+        const int split = (int)(workers / segments), per = ceil_div(kt, split);
+        if (per <= w.shared_per + 4) {
+          w.shared_split = split;
+          w.shared_per = per;
+        }
       }
+      // SMs without a share go to the own part's first workers, for as long as the others have theirs.
+      const int used = w.shared_split ? ceil_div(kt, w.shared_per) * (int)segments : ceil_div(segments * kt, w.shared_per);
+      w.own_early = (num_sms - used) * own_per_sm;
+      w.own_each = share_of((int64_t)w.shared_per * (rows > kTcRows / 2 ? kPairNs : kHalfNs), by_warp ? kWarpNs : kCtaNs);
     }
     e = few  ? launch_part<HD, true, WarpWorker>(w, ctas, st)
         : tc ? paged_shared_tc_launch(w, num_sms, st)
              : launch_part<HD, true, CtaWorker>(w, ctas, st);
     if (e != cudaSuccess) return e;
   }
-  // The own part by warps up to 16 rows a sequence and KV head, on average;
-  // beyond that a warp's 16 keys would be loaded again for every 16 rows.
-  const bool few = rows <= Few::kRows * (int64_t)p.n_seqs;
-  w.own_mt = few ? Few::kRows : Many::kRows;
-  w.own_keys = few ? Few::kKeys : Many::kKeys;
-  w.own_workers = few ? ctas * Few::kPerCta : ctas;
-  e = few ? launch_part<HD, false, WarpWorker>(w, ctas, st) : launch_part<HD, false, CtaWorker>(w, ctas, st);
+  e = by_warp ? launch_part<HD, false, WarpWorker>(w, ctas, st) : launch_part<HD, false, CtaWorker>(w, ctas, st);
   if (e != cudaSuccess) return e;
   // five CTAs an SM fit beside what the own part's have not left yet; fewer
   // items than their warps are shared by two or four

@@ -19,7 +19,8 @@ struct PagedWork {
   PagedAttnArgs a;
   Pieces own, shared;
   int64_t* starts;  // [n_seqs + 1] tiles before each sequence (own part)
-  int own_workers, shared_workers;
+  Shares* shares;   // the own part's, for the join
+  int own_workers, own_early, own_each;  // (see deal)
   int own_mt, shared_mt;      // rows of a tile
   int own_keys, shared_keys;  // positions of a tile
   // Shares of the shared part (its sizes are known to the host): `shared_per`

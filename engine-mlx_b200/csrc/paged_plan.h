@@ -53,7 +53,11 @@ inline auto once_a_device(std::atomic<uint64_t>& done, int device, F set) -> dec
   return e;
 }
 
-EMX_HD int ceil_div(int a, int b) { return (int)(((int64_t)a + b - 1) / b); }
+// x / per, by the short 32-bit division wherever both fit it.
+EMX_HD int share_of(int64_t x, int64_t per) {
+  return (x | per) >> 32 ? (int)(x / per) : (int)((uint32_t)x / (uint32_t)per);
+}
+EMX_HD int ceil_div(int64_t a, int b) { return share_of(a + b - 1, b); }
 
 // Row (in units of head_dim elements) of the cache [n_pages, n_kv, page_size]
 // that holds position `off` of page `page` for KV head h; the host refuses a
@@ -65,17 +69,34 @@ EMX_HD uint32_t cache_row(int page, int n_kv, int h, int page_size, int off) {
 // Segments: (KV head, row tile) pairs of one sequence, row tiles innermost,
 // each of `kt` key tiles and, before them, `setup` units for what a segment
 // costs its worker besides its tiles.  Units of sequence i are [start_i,
-// start_{i+1}) of the batch's T; worker c takes the tiles among units [c per,
-// (c + 1) per), so the tile at unit x is worker x / per's, and the workers of a
-// segment's tiles follow one another.
-EMX_HD int64_t share_size(int64_t T, int workers, int least) {
-  const int64_t up = T + workers - 1;
-  const int64_t per = up >> 32 ? up / workers : (int64_t)((uint32_t)up / (uint32_t)workers);
-  return per > least ? per : least;
-}
-// x / per, by the short 32-bit division wherever both fit it.
-EMX_HD int share_of(int64_t x, int64_t per) {
-  return (x | per) >> 32 ? (int)(x / per) : (int)((uint32_t)x / (uint32_t)per);
+// start_{i+1}) of the batch's T.  Workers take the units in order, so those of a
+// segment's tiles follow one another: the first `early` workers early_per units
+// each up to unit `cut`, the others late_per each from there on.
+struct Shares {
+  int64_t cut, early_per, late_per;
+  int early;
+  EMX_HD int64_t begin(int worker) const {
+    if (worker >= early) return cut + (int64_t)(worker - early) * late_per;
+    const int64_t x = (int64_t)worker * early_per;
+    return x < cut ? x : cut;
+  }
+  // the worker of a unit
+  EMX_HD int of(int64_t x) const { return x < cut ? share_of(x, early_per) : early + share_of(x - cut, late_per); }
+};
+
+// Even shares of a line of `units`, but for the first `early` workers, where they
+// have time for more than that, `each` units, before the others begin.
+EMX_HD Shares deal(int64_t units, int workers, int early, int each) {
+  Shares s;
+  s.early = (int64_t)each * workers > units ? early : 0;
+  s.cut = (int64_t)s.early * each;
+  s.early_per = each;
+  if (s.early > 0 && s.cut >= units) {  // they have time for all
+    s.cut = units;
+    s.early_per = share_of(units + early - 1, early);
+  }
+  s.late_per = share_of(units - s.cut + workers - s.early - 1, workers - s.early);
+  return s;
 }
 
 // The line of key tiles of one part of a batch's positions: the common prefix
@@ -99,7 +120,7 @@ struct Line {
     s.ok = true;
     return s;
   }
-  EMX_HD int row_tiles(const SeqInfo& s) const { return (int)(((int64_t)s.rows * hpg + mt - 1) / mt); }
+  EMX_HD int row_tiles(const SeqInfo& s) const { return ceil_div((int64_t)s.rows * hpg, mt); }
   EMX_HD int key_tiles(const SeqInfo& s) const { return ceil_div(own ? s.len - shared_len : s.len, keys); }
   EMX_HD int64_t units(const SeqInfo& s) const {
     if (!s.ok || s.rows == 0) return 0;

@@ -109,10 +109,10 @@ extern "C" int once(const int* devices, int n, int fails, int* made) {
     errors += once_a_device(done, devices[i], [&] { ++made[i]; return fails-- > 0 ? 7 : 0; }) != 0;
   return errors;
 }
-// Walks every worker's share of the line the way the kernel does.  seen[] counts the tiles in line order, pieces[] (at a
+// Walks every worker's share of the line the way the kernel does.  `choice` units are the first workers' shares; seen[] counts the tiles in line order, pieces[] (at a
 // segment's first tile) the pieces written of it; returns 0, or where an index left its range.
 extern "C" int walk(int own, int n_seqs, int n_rows, int n_kv, int hpg, int shared, int mt, int keys, int setup, long room,
-                    const int* indptr, const int* lengths, int64_t* starts, int workers, int least, int* seen, long n_seen,
+                    const int* indptr, const int* lengths, int64_t* starts, int workers, int choice, int* seen, long n_seen,
                     int* pieces) {
   Line line{own != 0, n_seqs, n_rows, n_kv, hpg, shared, mt, keys, setup, room, indptr, lengths, starts};
   int64_t T = 0, tiles = 0;
@@ -126,11 +126,14 @@ extern "C" int walk(int own, int n_seqs, int n_rows, int n_kv, int hpg, int shar
   if (own) starts[n_seqs] = T;
   if (tiles != n_seen) return 1;
   if (T == 0) return 0;
-  const int64_t per = share_size(T, workers, least);
-  if ((T + per - 1) / per > workers) return 13;
+  const int early = choice > 0 ? choice * workers / 40 : 0;
+  const Shares sh = deal(T, workers, early, choice);
+  if (sh.begin(0) != 0 || sh.begin(workers) < T || sh.begin(sh.early) != sh.cut) return 13;
+  if (sh.early && (sh.early != early || sh.early_per > choice || (sh.cut < T && sh.early_per != choice))) return 16;
+  if (!sh.early && sh.late_per > (T + workers - 1) / workers) return 17;
   int64_t at = 0;  // tiles seen: workers follow the line
   for (int c = 0; c < workers; ++c) {
-    const int64_t x0 = c * per, x1 = x0 + per < T ? x0 + per : T;
+    const int64_t x0 = sh.begin(c), x1 = sh.begin(c + 1) < T ? sh.begin(c + 1) : T;
     if (x0 >= T) continue;
     Cursor cur;
     cur.seek(line, x0);
@@ -154,7 +157,7 @@ extern "C" int walk(int own, int n_seqs, int n_rows, int n_kv, int hpg, int shar
       const bool last = cur.k + 1 == cur.kt, more = cur.x + 1 + (last ? setup : 0) < x1;
       if (last || !more) {
         // what the join will look for: the worker of the segment's first tile has the first piece
-        const int c0 = share_of(seg0, per), c1 = share_of(seg0 + cur.kt - 1, per);
+        const int c0 = sh.of(seg0), c1 = sh.of(seg0 + cur.kt - 1);
         if (whole ? c != c0 : !(c > c0 && c <= c1)) return 9;
         if (!whole && ++more_pieces > 1) return 10;  // one slot a worker
         pieces[at - cur.k] += 1;
@@ -195,7 +198,7 @@ def walk(plan):
     f.restype = C.c_int
     f.argtypes = [C.c_int] * 9 + [C.c_long] + [C.c_void_p] * 3 + [C.c_int, C.c_int, C.c_void_p, C.c_long, C.c_void_p]
 
-    def run(own, indptr, lengths, n_rows, n_kv, hpg, shared, mt, keys, room, workers, least=1, setup=0):
+    def run(own, indptr, lengths, n_rows, n_kv, hpg, shared, mt, keys, room, workers, choice=0, setup=0):
         indptr, lengths = np.asarray(indptr, np.int32), np.asarray(lengths, np.int32)
         n = len(lengths)
         total = 0
@@ -210,7 +213,7 @@ def walk(plan):
         seen, pieces = np.zeros(total + 1, np.int32), np.zeros(total + 1, np.int32)
         starts = np.zeros(n + 1, np.int64)
         rc = f(own, n, n_rows, n_kv, hpg, shared, mt, keys, setup, room, indptr.ctypes.data, lengths.ctypes.data, starts.ctypes.data,
-               workers, least, seen.ctypes.data, total, pieces.ctypes.data)
+               workers, choice, seen.ctypes.data, total, pieces.ctypes.data)
         assert rc == 0, rc
         assert (seen[:total] == 1).all()
         return total
@@ -230,7 +233,7 @@ def test_every_tile_has_one_worker_and_every_piece_is_joined(walk, seed):
     for own in (0, 1):
         if own or (shared and indptr[-1]):
             walk(own, indptr, lens, int(indptr[-1]) + 3, n_kv, hpg, shared, int(r.choice([16, 32, 128])),
-                 int(r.choice([16, 64, 128])), 8192, int(r.choice([1, 7, 148, 1184])), int(r.choice([1, 4])), int(r.choice([0, 1, 3])))
+                 int(r.choice([16, 64, 128])), 8192, int(r.choice([1, 7, 148, 1184])), int(r.choice([0, 0, 1, 4, 9, 39])), int(r.choice([0, 1, 3])))
 
 
 @pytest.mark.parametrize("seed", range(40))
@@ -240,5 +243,5 @@ def test_batches_out_of_order_stay_in_range(walk, seed):
     n = int(r.integers(1, 12))
     indptr = r.integers(-3, 20, n + 1)
     lens = r.choice([-5, 0, 1, 20, 64, 100, 513, 2**31 - 1], n)
-    walk(1, indptr, lens, 15, 2, int(r.choice([1, 4])), int(r.choice([0, 64])), 16, 16, 512, int(r.choice([1, 148])), 1, int(r.choice([0, 1])))
+    walk(1, indptr, lens, 15, 2, int(r.choice([1, 4])), int(r.choice([0, 64])), 16, 16, 512, int(r.choice([1, 148])), int(r.choice([0, 3])), int(r.choice([0, 1])))
     walk(1, [0] * (n + 1), lens, 15, 2, 1, 0, 16, 16, 512, 148)
