@@ -93,16 +93,23 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const PagedAp
     const bool store = page >= 0 && page < p.n_pages;
     if (!store && lane == 0) report_status(p.status, kDevBadPage);
     const size_t at = store ? (size_t)cache_row(page, p.n_kv, 0, p.page_size, pos % p.page_size) * HD + d0 : 0;
-    float sn[4], cs[4];
+    // a lane's four angles are those of the lanes with the same columns of the step's other heads: each works out its part
+    constexpr int kMine = 4 / HPI;
+    float sn[4], cs[4], my_sn[kMine], my_cs[kMine];
+#pragma unroll
+    for (int x = 0; x < kMine; ++x) {
+      my_sn[x] = 0.f;
+      my_cs[x] = 1.f;
+      if (a.rotate) {
+        double t = (double)pos * turns[d0 + sub * kMine + x];
+        t -= rint(t);
+        sincospif((float)(2.0 * t), &my_sn[x], &my_cs[x]);
+      }
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      sn[e] = 0.f;
-      cs[e] = 1.f;
-      if (a.rotate) {
-        double t = (double)pos * turns[d0 + e];
-        t -= rint(t);
-        sincospif((float)(2.0 * t), &sn[e], &cs[e]);
-      }
+      sn[e] = __shfl_sync(0xffffffffu, my_sn[e % kMine], e / kMine * LPH + lane % LPH);
+      cs[e] = __shfl_sync(0xffffffffu, my_cs[e % kMine], e / kMine * LPH + lane % LPH);
     }
     // y_d = inv (x_d c0 - x_{d+D/2} s1), y_{d+D/2} = inv (x_d s0 + x_{d+D/2} c1), the weights in c and s
     float c0[4], s0[4], c1[4], s1[4];
