@@ -14,12 +14,13 @@
 // 1e-2 rad), so turns p * theta^(-2d/D) / 2pi are taken in fp64, their whole
 // part is dropped there, and only the rest, in [-1/2, 1/2], goes to fp32.
 //
-// One warp per item, an item being some heads of one row, in steps of two heads
-// (four at D = 64) of one kind.  A lane holds elements 4d..4d+3 of both halves of
-// a head (two 8-byte loads, 128 contiguous bytes a half at D = 128): the pair
-// that a rotation mixes sits in one lane, and its four angles, multiplied into
-// the norm's weights once a row, serve every head of the row.  Four steps' loads
-// are in flight together, and 32 warps an SM.
+// One warp per item, an item being some heads of one row, in batches of four
+// steps: of q, or two of k and the same two of v; a step is two heads (four at
+// D = 64).  A lane holds elements 4d..4d+3 of both halves of a head (two 8-byte
+// loads, 128 contiguous bytes a half at D = 128): the pair that a rotation mixes
+// sits in one lane, and its four angles, multiplied into the norm's weights once a
+// row, serve every head of the row.  A batch's loads are in flight together, and 32
+// warps an SM.  The fp32 steps go two to an instruction (f32x2).
 #include "paged_dev.cuh"
 
 namespace emx {
@@ -27,22 +28,23 @@ namespace emx {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSteps = 4;  // whose loads are in flight together
+constexpr int kSteps = 4;  // of a batch
 
-__device__ __forceinline__ void unpack(const uint2& u, float (&f)[4]) {
-  f[0] = __uint_as_float(u.x << 16);
-  f[1] = __uint_as_float(u.x & 0xffff0000u);
-  f[2] = __uint_as_float(u.y << 16);
-  f[3] = __uint_as_float(u.y & 0xffff0000u);
+__device__ __forceinline__ uint64_t unpack(uint32_t u) { return pair32(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
+__device__ __forceinline__ uint32_t pack(uint64_t v) {
+  float a, b;
+  split32(v, a, b);
+  const __nv_bfloat162 two = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&two);
 }
 
-__device__ __forceinline__ uint2 pack(const float (&f)[4]) {
-  const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
-  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-}
+// The norm's weights (w, or 1) times the row's cosines and sines.
+struct Turn {
+  uint64_t c_lo[2], s_lo[2], c_hi[2], s_hi[2];  // s_hi negated
+};
 
-template <int HD>
-__global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const PagedAppendArgs a, int parts, int iters) {
+template <int HD, bool TURN>
+__global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const PagedAppendArgs a, int parts, int each) {
   constexpr int LPH = HD / 8;    // lanes a head
   constexpr int HPI = 32 / LPH;  // heads a step
   __shared__ double turns[HD / 2];  // theta^(-2d/D) / 2pi
@@ -50,8 +52,8 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const PagedAp
   const int lane = threadIdx.x & 31;
   const int d0 = 4 * (lane % LPH), sub = lane / LPH;
   const int n_heads = p.n_q + 2 * p.n_kv;
-  const int q_steps = (p.n_q + HPI - 1) / HPI, k_steps = (p.n_kv + HPI - 1) / HPI, steps = q_steps + 2 * k_steps;
-  if (threadIdx.x < HD / 2) turns[threadIdx.x] = exp2(a.log2_theta * (-2.0 * threadIdx.x / HD)) * 0.15915494309189533577;
+  const int q_batches = ceil_div(p.n_q, HPI * kSteps), batches = q_batches + ceil_div(p.n_kv, HPI * kSteps / 2);
+  if (TURN && threadIdx.x < HD / 2) turns[threadIdx.x] = exp2(a.log2_theta * (-2.0 * threadIdx.x / HD)) * 0.15915494309189533577;
   __syncthreads();
   pdl_wait();
   pdl_trigger();
@@ -59,28 +61,29 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const PagedAp
   const int64_t items = (int64_t)p.n_rows * parts;
   const int64_t warps = (int64_t)gridDim.x * (kThreads / 32);
   for (int64_t item = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); item < items; item += warps) {
-    const int row = (int)(item / parts);
-    const int it0 = (int)(item - (int64_t)row * parts) * iters, it1 = min(it0 + iters, steps);
+    const int row = share_of(item, parts);
+    const int b0 = (int)(item - (int64_t)row * parts) * each, b1 = min(b0 + each, batches);
     const bf16* src = a.qkv + (size_t)row * n_heads * HD + d0;
-    // the head of this lane in step `it` (in q | k | v), and whether there is one
-    auto head_of = [&](int it, bool& on) {
-      const int kind = it < q_steps ? 0 : it < q_steps + k_steps ? 1 : 2;
-      const int h = (it - (kind == 0 ? 0 : q_steps + (kind - 1) * k_steps)) * HPI + sub;
-      on = it < it1 && h < (kind == 0 ? p.n_q : p.n_kv);
-      return h + (kind == 0 ? 0 : p.n_q + (kind - 1) * p.n_kv);
-    };
     uint2 x[kSteps][2];
-    auto load = [&](int it) {
+    // head of slot u in batch b: of q, or of k (slots 0, 1) and v (2, 3)
+    auto q_head = [&](int b, int u) { return (b * kSteps + u) * HPI + sub; };
+    auto kv_head = [&](int b, int u) { return ((b - q_batches) * (kSteps / 2) + (u & 1)) * HPI + sub; };
+    auto load = [&](int b) {
 #pragma unroll
       for (int u = 0; u < kSteps; ++u) {
-        bool on;
-        const int h = head_of(it + u, on);
+        int h = q_head(b, u);
+        bool on = h < p.n_q;
+        if (b >= q_batches) {
+          h = kv_head(b, u);
+          on = h < p.n_kv;
+          h += p.n_q + (u >> 1) * p.n_kv;
+        }
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-          x[u][b] = on ? __ldcs(reinterpret_cast<const uint2*>(src + (size_t)h * HD + b * (HD / 2))) : make_uint2(0u, 0u);
+        for (int y = 0; y < 2; ++y)
+          x[u][y] = on ? __ldcs(reinterpret_cast<const uint2*>(src + h * HD + y * (HD / 2))) : make_uint2(0u, 0u);
       }
     };
-    load(it0);
+    load(b0);
     const int i = warp_find_seq(p.indptr, p.n_seqs, row);
     if (i >= p.n_seqs || row < p.indptr[i]) continue;  // behind the last sequence: left as it was
     const SeqInfo s = load_seq(p, i, 0);
@@ -89,119 +92,130 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const PagedAp
       continue;
     }
     const int pos = s.len - s.rows + (row - s.row0);
-    const int page = p.table[(size_t)i * p.max_pages + pos / p.page_size];
+    const int pg = pos / p.page_size, page = p.table[(size_t)i * p.max_pages + pg];
     const bool store = page >= 0 && page < p.n_pages;
     if (!store && lane == 0) report_status(p.status, kDevBadPage);
-    const size_t at = store ? (size_t)cache_row(page, p.n_kv, 0, p.page_size, pos % p.page_size) * HD + d0 : 0;
-    // a lane's four angles are those of the lanes with the same columns of the step's other heads: each works out its part
-    constexpr int kMine = 4 / HPI;
-    float sn[4], cs[4], my_sn[kMine], my_cs[kMine];
+    const size_t at = store ? (size_t)cache_row(page, p.n_kv, 0, p.page_size, pos - pg * p.page_size) * HD + d0 : 0;
+    float sn[4], cs[4];
+    if (TURN) {
+      // a lane's four angles are those of the lanes with the same columns of the step's other heads: each works out its part
+      constexpr int kMine = 4 / HPI;
+      float my_sn[kMine], my_cs[kMine];
 #pragma unroll
-    for (int x = 0; x < kMine; ++x) {
-      my_sn[x] = 0.f;
-      my_cs[x] = 1.f;
-      if (a.rotate) {
-        double t = (double)pos * turns[d0 + sub * kMine + x];
+      for (int e = 0; e < kMine; ++e) {
+        double t = (double)pos * turns[d0 + sub * kMine + e];
         t -= rint(t);
-        sincospif((float)(2.0 * t), &my_sn[x], &my_cs[x]);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      sn[e] = __shfl_sync(0xffffffffu, my_sn[e % kMine], e / kMine * LPH + lane % LPH);
-      cs[e] = __shfl_sync(0xffffffffu, my_cs[e % kMine], e / kMine * LPH + lane % LPH);
-    }
-    // y_d = inv (x_d c0 - x_{d+D/2} s1), y_{d+D/2} = inv (x_d s0 + x_{d+D/2} c1), the weights in c and s
-    float c0[4], s0[4], c1[4], s1[4];
-    auto weigh = [&](const bf16* w) {
-      float w0[4] = {1.f, 1.f, 1.f, 1.f}, w1[4] = {1.f, 1.f, 1.f, 1.f};
-      if (w) {
-        unpack(*reinterpret_cast<const uint2*>(w + d0), w0);
-        unpack(*reinterpret_cast<const uint2*>(w + d0 + HD / 2), w1);
+        sincospif((float)(2.0 * t), &my_sn[e], &my_cs[e]);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        c0[e] = cs[e] * w0[e];
-        s0[e] = sn[e] * w0[e];
-        c1[e] = cs[e] * w1[e];
-        s1[e] = sn[e] * w1[e];
+        sn[e] = __shfl_sync(0xffffffffu, my_sn[e % kMine], e / kMine * LPH + lane % LPH);
+        cs[e] = __shfl_sync(0xffffffffu, my_cs[e % kMine], e / kMine * LPH + lane % LPH);
+      }
+    }
+    // y_d = inv (x_d c_lo + x_{d+D/2} s_hi), y_{d+D/2} = inv (x_d s_lo + x_{d+D/2} c_hi)
+    Turn t;
+    auto weigh = [&](const bf16* w) {
+      uint2 lo = make_uint2(0x3f803f80u, 0x3f803f80u), hi = lo;  // ones
+      if (w) {
+        lo = *reinterpret_cast<const uint2*>(w + d0);
+        hi = *reinterpret_cast<const uint2*>(w + d0 + HD / 2);
+      }
+      const uint64_t l[2] = {unpack(lo.x), unpack(lo.y)}, h[2] = {unpack(hi.x), unpack(hi.y)};
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        t.c_lo[e] = TURN ? mul2(pair32(cs[2 * e], cs[2 * e + 1]), l[e]) : l[e];
+        t.c_hi[e] = TURN ? mul2(pair32(cs[2 * e], cs[2 * e + 1]), h[e]) : h[e];
+        if (TURN) {
+          t.s_lo[e] = mul2(pair32(sn[2 * e], sn[2 * e + 1]), l[e]);
+          t.s_hi[e] = mul2(pair32(-sn[2 * e], -sn[2 * e + 1]), h[e]);
+        }
       }
     };
-    int weighed = -1;
-    for (int it = it0; it < it1; it += kSteps) {
-      if (it != it0) load(it);
+    // a head: its norm (w given) and rotation
+    auto turn = [&](uint2 (&v)[2], bool norm) {
+      const uint64_t lo[2] = {unpack(v[0].x), unpack(v[0].y)}, hi[2] = {unpack(v[1].x), unpack(v[1].y)};
+      float inv = 1.f;
+      if (norm) {
+        float s0, s1;
+        split32(fma2(lo[0], lo[0], fma2(lo[1], lo[1], fma2(hi[0], hi[0], mul2(hi[1], hi[1])))), s0, s1);
+        float ss = s0 + s1;
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        inv = rsqrtf(fmaf(ss, 1.0f / HD, a.eps));  // 2 ulp of fp32
+      }
+      const uint64_t by = pair32(inv, inv);
+      uint32_t u[4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        // without a rotation x passes untouched: 0 * inf would not be 0
+        uint64_t y0 = mul2(lo[e], t.c_lo[e]), y1 = mul2(hi[e], t.c_hi[e]);
+        if (TURN) {
+          y0 = fma2(hi[e], t.s_hi[e], y0);
+          y1 = fma2(lo[e], t.s_lo[e], y1);
+        }
+        u[e] = pack(mul2(y0, by));
+        u[2 + e] = pack(mul2(y1, by));
+      }
+      v[0] = make_uint2(u[0], u[1]);
+      v[1] = make_uint2(u[2], u[3]);
+    };
+    auto put = [&](bf16* dst, const uint2 (&v)[2]) {
+      *reinterpret_cast<uint2*>(dst) = v[0];
+      *reinterpret_cast<uint2*>(dst + HD / 2) = v[1];
+    };
+    int b = b0;
+    if (b < q_batches) {
+      bf16* dst = a.q_out + (size_t)row * p.n_q * HD + d0;
+      weigh(a.q_norm);
+      for (; b < min(b1, q_batches); ++b) {
+        if (b != b0) load(b);
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u) {
+          turn(x[u], a.q_norm != nullptr);
+          const int h = q_head(b, u);
+          if (h < p.n_q) put(dst + h * HD, x[u]);
+        }
+      }
+    }
+    if (b >= b1) continue;
+    weigh(a.k_norm);
+    for (; b < b1; ++b) {
+      if (b != b0) load(b);
 #pragma unroll
       for (int u = 0; u < kSteps; ++u) {
-        if (it + u >= it1) break;
-        bool on;
-        const int h = head_of(it + u, on), kind = it + u < q_steps ? 0 : it + u < q_steps + k_steps ? 1 : 2;
-        if (kind < 2) {
-          const bf16* w = kind == 0 ? a.q_norm : a.k_norm;
-          if (weighed != kind) weigh(w);
-          weighed = kind;
-          float f[2][4], y[2][4];
-          unpack(x[u][0], f[0]);
-          unpack(x[u][1], f[1]);
-          float inv = 1.f;
-          if (w) {
-            float ss = 0.f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) ss = fmaf(f[0][e], f[0][e], fmaf(f[1][e], f[1][e], ss));
-#pragma unroll
-            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            inv = rsqrtf(fmaf(ss, 1.0f / HD, a.eps));  // 2 ulp of fp32
-          }
-          const bool norm = w != nullptr, turn = a.rotate != 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            // without a rotation x passes untouched: 0 * inf would not be 0
-            const float r0 = turn ? fmaf(f[0][e], c0[e], -(f[1][e] * s1[e])) : f[0][e] * c0[e];
-            const float r1 = turn ? fmaf(f[0][e], s0[e], f[1][e] * c1[e]) : f[1][e] * c1[e];
-            y[0][e] = norm ? r0 * inv : r0;
-            y[1][e] = norm ? r1 * inv : r1;
-          }
-          x[u][0] = pack(y[0]);
-          x[u][1] = pack(y[1]);
-        }
-        if (!on || (kind > 0 && !store)) continue;
-        bf16* dst;
-        if (kind == 0) {
-          dst = a.q_out + ((size_t)row * p.n_q + h) * HD + d0;
-        } else {
-          const int hk = h - p.n_q - (kind - 1) * p.n_kv;
-          dst = (kind == 1 ? p.k : p.v) + at + (size_t)hk * p.page_size * HD;
-        }
-#pragma unroll
-        for (int b = 0; b < 2; ++b) *reinterpret_cast<uint2*>(dst + b * (HD / 2)) = x[u][b];
+        if (u < kSteps / 2) turn(x[u], a.k_norm != nullptr);
+        const int h = kv_head(b, u);
+        if (store && h < p.n_kv) put((u < kSteps / 2 ? p.k : p.v) + at + (size_t)h * p.page_size * HD, x[u]);
       }
     }
   }
 }
 
-}  // namespace
-
-cudaError_t paged_append_launch(const PagedAppendArgs& a, int num_sms, cudaStream_t st) {
+template <int HD, bool TURN>
+cudaError_t launch(const PagedAppendArgs& a, int num_sms, cudaStream_t st) {
   const PagedArgs& p = a.p;
-  const int hpi = 32 / (p.head_dim / 8);
-  const int steps = (p.n_q + hpi - 1) / hpi + 2 * ((p.n_kv + hpi - 1) / hpi);
+  constexpr int kHeads = 256 / HD * kSteps;  // of a batch of q
+  const int batches = ceil_div(p.n_q, kHeads) + ceil_div(p.n_kv, kHeads / 2);
   // a row to a warp when the rows alone fill the SMs' warps; below that its
-  // heads are spread over more warps, four steps (one batch of loads) at
-  // least each, so that a few rows are not one warp's serial work
-  const int64_t want = (int64_t)num_sms * 32;
-  int parts = (int)((want + p.n_rows - 1) / p.n_rows);
-  const int most = (steps + kSteps - 1) / kSteps;
-  if (parts > most) parts = most;
-  const int iters = (steps + parts - 1) / parts;
-  parts = (steps + iters - 1) / iters;
-  const int64_t items = (int64_t)p.n_rows * parts;
-  int64_t grid = (items + kThreads / 32 - 1) / (kThreads / 32);
-  const int64_t cap = (int64_t)num_sms * 8;  // two rounds of four CTAs an SM: beyond that a warp takes further items
-  if (grid > cap) grid = cap;
+  // batches are spread over more warps, so that a few rows are not one warp's
+  // serial work
+  int parts = min(batches, ceil_div((int64_t)num_sms * 32, p.n_rows));
+  const int each = ceil_div(batches, parts);
+  parts = ceil_div(batches, each);
+  // two rounds of four CTAs an SM: beyond that a warp takes further items
+  const int64_t grid = min(((int64_t)p.n_rows * parts + kThreads / 32 - 1) / (kThreads / 32), (int64_t)num_sms * 8);
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute at;
   overlapped(cfg, at, (unsigned)grid, kThreads, 0, st);
-  return p.head_dim == 128 ? cudaLaunchKernelEx(&cfg, paged_append_kernel<128>, a, parts, iters)
-                           : cudaLaunchKernelEx(&cfg, paged_append_kernel<64>, a, parts, iters);
+  return cudaLaunchKernelEx(&cfg, paged_append_kernel<HD, TURN>, a, parts, each);
+}
+
+}  // namespace
+
+cudaError_t paged_append_launch(const PagedAppendArgs& a, int num_sms, cudaStream_t st) {
+  if (a.p.head_dim == 128) return a.rotate ? launch<128, true>(a, num_sms, st) : launch<128, false>(a, num_sms, st);
+  return a.rotate ? launch<64, true>(a, num_sms, st) : launch<64, false>(a, num_sms, st);
 }
 
 }  // namespace emx
