@@ -745,20 +745,28 @@ cudaError_t launch(PagedWork& w, int num_sms, cudaStream_t st) {
   const PagedArgs& p = w.a.p;
   const int64_t rows = (int64_t)p.n_rows * (p.n_q / p.n_kv);  // of a KV head
   const int ctas = num_sms * kCtasPerSm;
-  // The own part by warps up to 16 rows a sequence and KV head, on average;
-  // beyond that a warp's 16 keys would be loaded again for every 16 rows.
-  const bool by_warp = rows <= Few::kRows * (int64_t)p.n_seqs;
+  // The own part by warps up to 32 rows a sequence and KV head, on average;
+  // beyond that a warp's 16 keys are loaded once too often, again for every 16
+  // rows (32 sequences of 500 to 2500 positions, 32 heads on 4: 8, 24 and 32 rows
+  // 27, 42 and 43 us, by CTAs 41, 46 and 46; 64 rows 72 us, by CTAs 51).
+  const bool by_warp = rows <= 2 * Few::kRows * (int64_t)p.n_seqs;
   w.own_mt = by_warp ? Few::kRows : Many::kRows;
   w.own_keys = by_warp ? Few::kKeys : Many::kKeys;
   const int own_per_sm = kCtasPerSm * (by_warp ? Few::kPerCta : 1);
   w.own_workers = num_sms * own_per_sm;
   cudaError_t e = cudaSuccess;
   if (w.a.shared_len > 0) {
-    // tcgen05 from 17 rows a head on, where it takes the pages
-    const bool few = rows <= Few::kRows, tc = !few && paged_shared_tc_takes(p);
-    w.shared_mt = few ? Few::kRows : tc ? kTcRows : Many::kRows;
-    w.shared_keys = few ? Few::kKeys : tc ? kTcKeys : Many::kKeys;
-    const int workers = few ? ctas * Few::kPerCta : tc ? num_sms : ctas;
+    // tcgen05 where it takes the pages and the prefix is more than two of a CTA's
+    // 64 x 64 tiles to each of those (592): below, its start and end cost more than
+    // its tiles save (8 KV heads of 8 rows: 512 positions, 64 tiles, 15.5 us against
+    // 12.1; 4096, 512 tiles, 17.5 against 19.0; 8192, 1024 tiles, 20.9 against 24.7.
+    // 4 heads of 512 rows: 1024 positions, 512 tiles, 26.2 against 25.0; 2048, 1024
+    // tiles, 28.6 against 31.3; 8192 33.8 against 61.1).
+    const int64_t tiles = (int64_t)p.n_kv * ceil_div(rows, Many::kRows) * ceil_div(w.a.shared_len, Many::kKeys);
+    const bool tc = paged_shared_tc_takes(p) && tiles > 2 * ctas;
+    w.shared_mt = tc ? kTcRows : Many::kRows;
+    w.shared_keys = tc ? kTcKeys : Many::kKeys;
+    const int workers = tc ? num_sms : ctas;
     const int kt = ceil_div(w.a.shared_len, w.shared_keys);
     const int64_t segments = (int64_t)p.n_kv * ceil_div(rows, w.shared_mt);
     w.shared_per = ceil_div(segments * kt, workers);
@@ -779,9 +787,7 @@ cudaError_t launch(PagedWork& w, int num_sms, cudaStream_t st) {
       w.own_early = (num_sms - used) * own_per_sm;
       w.own_each = share_of((int64_t)w.shared_per * (rows > kTcRows / 2 ? kPairNs : kHalfNs), by_warp ? kWarpNs : kCtaNs);
     }
-    e = few  ? launch_part<HD, true, WarpWorker>(w, ctas, st)
-        : tc ? paged_shared_tc_launch(w, num_sms, st)
-             : launch_part<HD, true, CtaWorker>(w, ctas, st);
+    e = tc ? paged_shared_tc_launch(w, num_sms, st) : launch_part<HD, true, CtaWorker>(w, ctas, st);
     if (e != cudaSuccess) return e;
   }
   e = by_warp ? launch_part<HD, false, WarpWorker>(w, ctas, st) : launch_part<HD, false, CtaWorker>(w, ctas, st);

@@ -653,3 +653,103 @@ def test_a_step_whose_first_calls_are_captured():
     r = subprocess.run([sys.executable, "-c", FIRST_IN_A_GRAPH, here, os.path.join(os.path.dirname(here), "engine-mlx_b200")],
                        capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "as eager" in r.stdout, r.stdout + r.stderr
+
+
+# ------------------------------------------------------------------- a prefix long enough for the tensor-memory kernel
+def long_prefix(seed, page, hd, seqs, n_q=64, n_kv=8, **k):
+    """More than 592 tiles of 64 rows and 64 positions: 12, 20 and 45 sequences have one half, one and two row tiles."""
+    r = np.random.default_rng(seed)
+    shared = page * -(-2500 // page)
+    rows = np.ones(seqs, int)
+    assert n_kv * -(-seqs * (n_q // n_kv) // 64) * (shared // 64) > 592
+    return Case(seed, rows, shared + rows + r.integers(0, 50, seqs), n_q, n_kv, hd, page, shared, **k)
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("page", [8, 16, 24, 40, 64, 128, 256, 20])
+@pytest.mark.parametrize("seqs", [12, 20, 45])
+def test_a_long_prefix(ctx, seqs, page, hd):
+    c = long_prefix(page, page, hd, seqs, pad=1).device(ctx)
+    check_attend(c, attend(ctx, c))
+    assert c.status == 0
+
+
+@pytest.mark.parametrize("seqs", [3, 12, 45])
+def test_a_long_prefix_of_large_scores(ctx, seqs):
+    """Scores of a standard deviation of six: maxima move, and few weights count.  Their fp32 errors (128 products, 2^-24 of
+    scores up to 40) stay below the 2^-11 that the bound has for them."""
+    c = long_prefix(50, 16, 128, seqs) if seqs > 3 else Case(50, [1] * 3, [5000] * 3, 64, 8, shared=4992)
+    c.q = emx.bf16(emx.f32(c.q) * 6)
+    ramp = np.linspace(0.2, 1.0, c.shared // 16)  # later pages have larger keys
+    for j, p in enumerate(c.shared_pages):
+        c.k[p] = emx.bf16(emx.f32(c.k[p]) * ramp[j])
+    check_attend(c, attend(ctx, c.device(ctx)))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+@pytest.mark.parametrize("seqs", [12, 45])
+def test_a_long_prefix_and_scales_that_are_not_positive(ctx, scale, seqs):
+    c = long_prefix(51, 16, 128, seqs)
+    c.scale = scale
+    check_attend(c, attend(ctx, c.device(ctx)))
+
+
+@pytest.mark.parametrize("seqs", [12, 45])
+def test_bad_pages_of_a_long_prefix(ctx, seqs):
+    c = long_prefix(52, 16, 128, seqs).device(ctx)
+    pages = c.shared_pages.copy()
+    pages[7], pages[20], pages[-1] = c.n_pages, -1, 1 << 30
+    c.d_shared.write(pages)
+    hole = {p * 16 + x for p in (7, 20, len(pages) - 1) for x in range(16)}
+    got = attend(ctx, c)
+    assert c.status == 5 and near(got[:c.n], *want_without(c, [hole] * seqs)).all()
+    c.d_shared.write(np.full(len(pages), -1, np.int32))
+    got = attend(ctx, c)
+    assert c.status == 5 and near(got[:c.n], *want_without(c, [set(range(c.shared))] * seqs)).all()
+
+
+@pytest.mark.parametrize("seqs", [12, 45])
+def test_what_is_not_finite_in_a_long_prefix(ctx, seqs):
+    """A row of q that is NaN spoils no other; NaN in one dimension of V reaches that dimension of all rows."""
+    c = long_prefix(53, 16, 128, seqs)
+    want, size = c.attend()
+    q = c.q.copy()
+    q[5, 9] = NAN
+    d = long_prefix(53, 16, 128, seqs)
+    d.q = q
+    got = attend(ctx, d.device(ctx))
+    g = emx.f32(got[:c.n])
+    assert np.isnan(g[5, 9]).all() and np.isnan(g).sum() == 128
+    g[5, 9] = want[5, 9]
+    assert near(emx.bf16(g), want, size).all()
+    d = long_prefix(53, 16, 128, seqs)
+    d.v[d.shared_pages[3], 2, 7, 11] = NAN
+    g = emx.f32(attend(ctx, d.device(ctx))[:c.n])
+    assert np.isnan(g[:, 16:24, 11]).all() and np.isnan(g).sum() == c.n * 8
+
+
+@pytest.mark.parametrize("seqs,n_q,n_kv", [(12, 64, 8), (20, 64, 8), (45, 64, 8), (135, 64, 8)])
+def test_a_long_prefix_gives_the_same_bits(ctx, seqs, n_q, n_kv):
+    c = long_prefix(54, 16, 128, seqs, n_q, n_kv).device(ctx)
+    first = attend(ctx, c)
+    for _ in range(20):
+        assert (attend(ctx, c) == first).all()
+    ctx.sdpa_paged(c.dq, c.kv, c.batch, n_q, c.scale, c.shared, c.d_shared, out=c.dq)  # over q
+    assert (c.dq.read(np.uint16, c.q.shape) == first[:c.n_rows]).all()
+
+
+def test_long_and_short_prefixes_one_after_another(ctx):
+    cases = [long_prefix(55, 16, 128, 45), Case(56, [1] * 45, [400 + i for i in range(45)], 64, 8, shared=320),
+             long_prefix(57, 64, 128, 12), long_prefix(58, 20, 128, 12), Case(59, [1] * 30, [70] * 30, 64, 8)]
+    for c in cases:
+        c.device(ctx)
+    ws = ctx.alloc(max(ctx.sdpa_paged_workspace(c.kv, c.batch, 64, c.shared) for c in cases))
+    want = [attend(ctx, c, ws=ws) for c in cases]
+    outs = [[ctx.put(np.full(w.shape, NAN, np.uint16)) for w in want] for _ in range(4)]
+    for turn, out in enumerate(outs):
+        for i in np.random.default_rng(turn).permutation(len(cases)):
+            c = cases[i]
+            ctx.sdpa_paged(c.dq, c.kv, c.batch, 64, c.scale, c.shared, c.d_shared, out=out[i], workspace=ws)
+    for out in outs:
+        for o, w in zip(out, want):
+            assert (o.read(np.uint16, w.shape) == w).all()
