@@ -4,9 +4,12 @@
 // All rows of the batch that use one KV head (n_rows * n_q / n_kv of them)
 // attend the same S keys without a mask, so the prefix is two dense products
 // around a softmax: S = Q K^T, O = P V, rows in tiles of 128, keys in tiles of
-// 128.  K and V are read from HBM once per KV head and 256 rows; with up to
-// 128 rows a head that stream (64 KB a tile) bounds the kernel, with more the
-// exponentials (128 x 128 a tile, 16 an SM and clock) and the tensor pipe.
+// 128.  K and V are read from HBM once per KV head and 256 rows.  A tile of 256
+// rows and 128 keys takes 1.82 us (1.65 with K and V in L2): 9.2 TFLOP/s an SM, of
+// the 11.4 that the library's measured rate comes to; the exponentials alone (128 x
+// 128 twice, 16 an SM and clock) 1.1.  A tile of up to 128 rows takes 1.35 us, the
+// time of its 64 KB on all SMs (7 TB/s out of L2 and HBM together).  A worker's start
+// (barriers, Q, the first keys) takes 4 us, the end (pieces to memory) 4.
 //
 // One CTA an SM, each with an even share of the (KV head, 256 rows, 128 keys)
 // tiles in line order; twelve warps:
@@ -20,8 +23,11 @@
 //              rows, the largest power of two that divides the page size),
 //              into a ring of five 128-row slots (K, V, K, V, ...).  Boxes
 //              behind the prefix and pages outside the cache start beyond the
-//              tensor and read as zeros.  (16-byte asynchronous copies by two or
-//              three warps, which take any page size, reached 30 GB/s an SM.)
+//              tensor and read as zeros.  A copy takes 20 to 30 ns of the SM's copy
+//              engine, so it brings whole rows: with two for the two 64-column
+//              blocks a tile of 16-position pages took 2.2 us.  (16-byte
+//              asynchronous copies by two or three warps, which take any page size,
+//              reached 30 KB/us an SM.)
 // Each group is a stream of its own — S, P and O in tensor memory, its Q tile
 // in shared memory: two row tiles against the same keys where the segment has
 // more than 128 rows, else the same rows against alternate key tiles (then the
@@ -32,7 +38,7 @@
 //
 // The maximum that the exponentials use moves only when a tile's exceeds it by
 // more than 2^8 (then O and l are rescaled); O / l does not depend on it.  P is
-// rounded to bf16 for its product (off by at most 2^-9 of each weight).
+// rounded to bf16 for its product (off by at most 2^-8 of each weight).
 #include <cudaTypedefs.h>
 
 #include <mutex>
