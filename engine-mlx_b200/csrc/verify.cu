@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
     const bool minus = turn == 0 && q, certain = turn == 0 && one >= 0;
     constexpr int U = 4;  // steps whose loads are in flight together
     double sums[U] = {};  // one chain of additions would take longer than the loads
+    float rests[U] = {};
     for (int at0 = b + lane * VEC; at0 < e; at0 += U * kTile) {
       Raw<T, VEC> x[U], y[U];
 #pragma unroll
@@ -191,11 +192,23 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
       for (int k = 0; k < U; ++k)
         if (at0 + k * kTile < e)
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) sums[k] += r_of(x[k], y[k], minus, certain, at0 + k * kTile, v);
+          for (int v = 0; v < VEC; ++v) {
+            // An SM converts 16 values to fp64 a clock, so p - q goes there once: rounded to fp32, and what the
+            // rounding left (exact: a - b = d + e for a > b) is summed beside, 2^-24 of it in 24 bits.
+            if (minus) {
+              const float f = mass(x[k].get(v)), g = mass(y[k].get(v)), d = f - g;
+              if (d > 0.f) {
+                sums[k] += (double)d;
+                rests[k] += (f - d) - g;
+              }
+            } else {
+              sums[k] += r_of(x[k], y[k], minus, certain, at0 + k * kTile, v);
+            }
+          }
     }
     double sum = 0.0;
 #pragma unroll
-    for (int k = 0; k < U; ++k) sum += sums[k];
+    for (int k = 0; k < U; ++k) sum += sums[k] + (double)rests[k];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) S.warp_sum[warp] = sum;
