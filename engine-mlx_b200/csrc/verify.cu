@@ -84,11 +84,12 @@ struct Shared {
   int found;
 };
 
-// Inclusive sum over the lanes.
+// Inclusive sum over the lanes, right in the first N.
+template <int N = 32>
 __device__ __forceinline__ double warp_scan(double v) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
+  for (int o = 1; o < N; o <<= 1) {
     const double x = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += x;
   }
@@ -214,14 +215,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
     if (lane == 0) S.warp_sum[warp] = sum;
     __syncthreads();
     // every warp has the CTA's warps' running sums in its lanes
-    const double w_sum = lane < kWarps ? S.warp_sum[lane] : 0.0, w_incl = warp_scan(w_sum);
+    const double w_sum = lane < kWarps ? S.warp_sum[lane] : 0.0, w_incl = warp_scan<kWarps>(w_sum);
     const double cta = __shfl_sync(0xffffffffu, w_incl, kWarps - 1);
     if (turn == 0) all_began();
     if (tid < parts) *cluster.map_shared_rank(&S.cta_sum[turn & 1][part], tid) = cta;
     cluster.sync();
     // ... and, in the same way, the cluster's CTAs'
-    const double c_sum = lane < parts ? S.cta_sum[turn & 1][lane] : 0.0, c_incl = warp_scan(c_sum);
-    const double total = __shfl_sync(0xffffffffu, c_incl, 31);
+    const double c_sum = lane < parts ? S.cta_sum[turn & 1][lane] : 0.0, c_incl = warp_scan<kMost>(c_sum);
+    const double total = __shfl_sync(0xffffffffu, c_incl, kMost - 1);
     if (!(total > 0.0)) {
       if (minus || certain) continue;  // nothing left of p - q: p itself
       if (part == 0 && tid == 0) out[n] = -1;  // no mass at all
@@ -259,7 +260,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
       const double incl = warp_scan(own);
       if (lane == 31) S.scan[warp] = incl;
       __syncthreads();
-      const double ws = lane < kWarps ? S.scan[lane] : 0.0, wi = warp_scan(ws);
+      const double ws = lane < kWarps ? S.scan[lane] : 0.0, wi = warp_scan<kWarps>(ws);
       double s = base + __shfl_sync(0xffffffffu, wi - ws, warp) + (incl - own);
       int hit = -1, last = -1;
 #pragma unroll
