@@ -21,7 +21,7 @@
 // remote is touched behind it; the CTA whose slice holds the token then walks
 // the run of the warp that does, all its threads together, out of L2.
 //
-// 64 sequences over 151936 fp32 values, p and q (78 MB): 24.6 us, 3.2 TB/s, half of
+// 64 sequences over 151936 fp32 values, p and q (78 MB): 23.5 us, 3.3 TB/s, half of
 // which are the chain's other links (7.0 us for one sequence: the drafts' two
 // dependent loads, the row, two reductions, the walk).
 #include <cooperative_groups.h>
@@ -35,6 +35,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMost = 16;  // CTAs of a cluster
+constexpr int kLoads = 4;  // steps whose loads are in flight together
 
 template <typename T>
 __device__ __forceinline__ float val(T v);
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
   };
   for (int turn = 0;; ++turn) {
     const bool minus = turn == 0 && q, certain = turn == 0 && one >= 0;
-    constexpr int U = 4;  // steps whose loads are in flight together
+    constexpr int U = kLoads;
     double sums[U] = {};  // one chain of additions would take longer than the loads
     float rests[U] = {};
     for (int at0 = b + lane * VEC; at0 < e; at0 += U * kTile) {
@@ -317,14 +318,17 @@ cudaError_t run(const VerifyArgs& a, int parts, cudaStream_t st) {
 
 template <typename T, int VEC>
 cudaError_t run(const VerifyArgs& a, int num_sms, cudaStream_t st) {
-  // As many threads as there is room for, so that a thread's share of the row is
-  // a load or two: sixteen CTAs of 512 a sequence while each has an SM of its own
-  // (one sequence of 151936: 7.2 us, with eight 9.4), then eight (16 sequences:
-  // 12.2 us, of 256 threads 13.5).  Beyond that eight of 256, four on an SM, so
-  // that one's chain of latencies passes under the others' streams (64 sequences:
-  // 24.7 us, of 512 threads 29.1).
+  // As many threads as there is room for, so that a thread's share of the row is a
+  // load or two: sixteen CTAs of 512 a sequence while each has an SM of its own (one
+  // sequence of 151936: 7.2 us, with eight 9.3), then eight, of 512 threads where
+  // 256 would take more than one round of loads (24 and 32 sequences of 151936: 14.7
+  // and 16.0 us, of 256 17.8 and 18.1; of 32000 8.4 and 8.9 against 7.8).  Beyond seven
+  // quarters of an SM's worth each eight of 256, four on an SM, so that one's
+  // chain of latencies passes under the others' streams (37 sequences: 22.5 us, of
+  // 512 threads 23.2; 64: 23.5 and 28.4).
   if (a.n_seqs * 16 <= num_sms) return run<T, VEC, 512>(a, 16, st);
-  if (a.n_seqs * 8 <= num_sms) return run<T, VEC, 512>(a, 8, st);
+  const bool rounds = a.vocab > 8 * 256 * VEC * kLoads;
+  if (rounds && a.n_seqs * 8 <= num_sms * 7 / 4) return run<T, VEC, 512>(a, 8, st);
   return run<T, VEC, 256>(a, 8, st);
 }
 
