@@ -75,6 +75,7 @@ struct Bars {
   uint64_t q_full[2];
   uint64_t s_full[2][2], p_full[2][2];  // by group and half
   uint64_t pv_done[2][2];               // a half's products (and all before) are in O
+  uint64_t all_done[2];                 // all of a group's products and commits
   uint32_t tmem;
   alignas(16) unsigned char valid[kValid][16];  // by tile of the share, bit j: key j is there
 };
@@ -202,6 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int g = 0; g < 2; ++g) {
         mbar_init(&B.q_full[g], 128);
+        mbar_init(&B.all_done[g], 1);
         for (int x = 0; x < 2; ++x) {
           mbar_init(&B.s_full[g][x], 2);
           mbar_init(&B.p_full[g][x], x == 0 ? 129 : 128);  // the first half's with its keys
@@ -229,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int worker = blockIdx.x;
   Walk wk;
   const bool any = wk.begin(line, worker, w.shared_per, w.shared_split);
-  // a wait that gave up leaves `ok` false: later waits are skipped, the work runs out on whatever is there
+  // a wait that gave up leaves `ok` false: later waits are skipped and no more copies and MMAs are begun
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && mbar_wait_bounded(bar, parity, status); };
 
@@ -245,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       return lane < boxes && pos < a.shared_len ? a.shared_pages[pos / a.p.page_size] : -1;
     };
     Slot at{0, 1};  // `empty`: the first round waits for nothing
-    int page = look_up(wk.c.k), tile = 0;
+    int page = look_up(wk.c.k), tile = 0, copies = 0;  // `copies`: slots filled
     bool more = true;
     for (int t = 0; more;) {
       const int pos = (wk.c.k + t) * kTcKeys + lane * box;
@@ -263,6 +265,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int kv = 0; kv < 2; ++kv) {
         wait(&B.empty[at.s], at.parity);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         if (kv == 0 && lane < boxes)
           for (int g = 0; g < box / 8; ++g) B.valid[tile % kValid][lane * (box / 8) + g] = on ? 0xff : 0;
         __syncwarp();
@@ -273,16 +277,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           tma_groups(dst, kv ? &tv : &tk, row / 8, &B.full[at.s], policy);
         }
         at.step(1);
+        ++copies;
       }
+      if (!ok) break;
       ++tile;
     }
     // copies still on their way (after a wait that gave up) have landed before the CTA ends
-    const int last = 2 * tile < kSlots ? 2 * tile : kSlots;
-    for (int i = 0; i < last; ++i) {
-      at.s = at.s == 0 ? kSlots - 1 : at.s - 1;
-      const uint32_t use = (uint32_t)((2 * tile - 1 - i) / kSlots);
-      mbar_wait_bounded(&B.full[at.s], use & 1, status);
-    }
+    for (int i = copies; i-- > 0 && i >= copies - kSlots;) mbar_wait_bounded(&B.full[i % kSlots], (i / kSlots) & 1, status);
   } else if (any && warp == kKeyWarp) {
     if (lane == 0) {
       Slot ks{0, 0}, vs{1, 0};
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return (d & 0xffffffff00000000ull) | (uint32_t)((uint32_t)d + (bytes >> 4));
       };
       auto soon = [&](uint64_t* bar, uint32_t parity) {  // polls closely before the bounded wait's longer steps
-        for (int i = 0; i < 2000; ++i)
+        for (int i = 0; i < 2000 && ok; ++i)
           if (mbar_test_wait(bar, parity)) return;
         wait(bar, parity);
       };
@@ -333,10 +334,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t tS = tmem + 128 * g, tO = tmem + 256 + 128 * g;
       auto qk = [&](int s, int half) {
         const uint64_t K = at16(k0, L::kRing + s * L::kTile + half * 8 * L::kGroup);  // its 64 rows
+        if (ok) {
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k)  // 16 head dims a step: 32 bytes along the rows of a 64-column block
-          umma(tS + 64 * half, at16(Q, (k >> 2) * kBlk + 32 * (k & 3)), at16(K, (k >> 2) * 1024 + 32 * (k & 3)), id_s,
-               k > 0 ? 1u : 0u);
+          for (int k = 0; k < HD / 16; ++k)  // 16 head dims a step: 32 bytes along the rows of a 64-column block
+            umma(tS + 64 * half, at16(Q, (k >> 2) * kBlk + 32 * (k & 3)), at16(K, (k >> 2) * 1024 + 32 * (k & 3)), id_s,
+                 k > 0 ? 1u : 0u);
+        }
         umma_commit(&B.s_full[g][half]);
         mbar_arrive(&B.s_full[g][half]);  // and the key masks, which the wait for K has seen
       };
@@ -345,9 +348,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         soon(&B.p_full[g][half], p_parity);
         tfence_after();
         const uint64_t V = at16(v0, L::kRing + s * L::kTile + half * 8 * L::kGroup);
+        if (ok) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)  // 16 keys a step: 8 columns of P, 16 rows of V
-          umma_ta(tO, tS + 64 * half + 8 * k, at16(V, k * 2 * L::kGroup), id_pv, (k > 0 || half > 0 || !first) ? 1u : 0u);
+          for (int k = 0; k < 4; ++k)  // 16 keys a step: 8 columns of P, 16 rows of V
+            umma_ta(tO, tS + 64 * half + 8 * k, at16(V, k * 2 * L::kGroup), id_pv, (k > 0 || half > 0 || !first) ? 1u : 0u);
+        }
         umma_commit(&B.pv_done[g][half]);
       };
       Slot ks{0, 0}, vs{1, 0};
@@ -398,6 +403,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       } while (wk.next(line));
+      // nothing of this thread's is on its way when the CTA ends, whatever waits gave up
+      umma_commit(&B.all_done[g]);
+      mbar_wait_bounded(&B.all_done[g], 0, status);
     }
   } else if (any) {
     // ---- softmax: group g, row r of its tile
