@@ -19,12 +19,12 @@
 // pieces of each row (and a segment that one worker has whole is written by it).
 //
 // The own part reads every K and V once and for few rows: memory bounds it where
-// there is enough of it (32 sequences of 17 to 8192 positions, 269 MB: 49 us
-// alone, 5.5 TB/s; 53.5 us with the join), and a warp's own chain of latencies
+// there is enough of it (32 sequences of 17 to 8192 positions, 269 MB: 50 us
+// alone, 5.4 TB/s; 54.3 us with the join), and a warp's own chain of latencies
 // elsewhere: a 16-key tile takes it 1.3 to 1.45 us, whether or not the SM's other
 // warps want memory.  Twelve warps an SM with two tiles each (against eight with
 // three) took 55.3 us, fewer instructions for the copies nothing off.  A short
-// sequence alone (132 positions) takes 9.3 us: three dependent loads (rows,
+// sequence alone (132 positions) takes 8.7 us: three dependent loads (rows,
 // page, keys) and two kernels.
 #include "paged_attn.cuh"
 
@@ -41,8 +41,8 @@ constexpr int kMaxSeqs = 1024;
 constexpr int kCtasPerSm = 2;
 // ns of a tcgen05 tile of 256 rows and of 128, and of an own part's unit by a
 // warp and by a CTA, of those that run beside them (with the longer shares 128 rows
-// on 16384 take 65.1 us, with even ones 66.7).
-constexpr int kPairNs = 1850, kHalfNs = 1450, kWarpNs = 1450, kCtaNs = 4000;
+// on 16384 take 75.5 us, with even ones 75.9; 24 drafted sequences on 8192 83.0 and 83.7).
+constexpr int kPairNs = 2480, kHalfNs = 1610, kWarpNs = 1450, kCtaNs = 4000;
 
 // `policy`: first out of L2.  K and V are read once or, by a sequence's next row
 // tile, soon again; the pieces, which the join reads, are to stay.
@@ -147,7 +147,7 @@ __device__ __forceinline__ void copy_kv(const PagedAttnArgs& a, uint32_t to_k, u
 
 // Sixteen rows of one segment, by a warp: q as MMA operands, the running
 // maximum and sum of each row and its O.
-template <int HD, bool SHARED>
+template <int HD, bool SHARED, bool FEW_ROWS>
 struct Rows {
   uint32_t qf[HD / 16][4];
   float o[HD / 8][4];
@@ -188,10 +188,14 @@ struct Rows {
     for (int x = 16; x > 0; x >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, x));
   }
 
+  // Up to eight rows: the other eight of the operands hold the low parts of the weights.
+  __device__ __forceinline__ bool few() const { return R - base <= 8; }
+
   // 16 G keys, key0 of the part the first, rows r0 .. r0 + 16 G - 1 of the tiles at K and V; bit j of `there`: key j is.
-  template <int G>
+  template <int G, bool FEW>
   __device__ __forceinline__ void keys(float sl2, uint32_t K, uint32_t V, int r0, int key0, uint32_t there) {
     constexpr uint32_t kAll = G == 2 ? 0xffffffffu : 0xffffu;
+    constexpr int B = FEW ? 1 : 2;  // rows of a thread
     const int lane = threadIdx.x & 31, col = (lane & 3) * 2;
     const float nothing = sl2 < 0.f ? INFINITY : -INFINITY;  // the score of a key that is not seen
     float s[2 * G][4];
@@ -211,11 +215,11 @@ struct Rows {
     // m is the maximum of s * scale * log2 e.  Masks only where a key is missing
     // or some row does not see the whole tile.
     const bool cut = key0 + 16 * G > least, masked = there != kAll || cut;
-    uint32_t pf[G][4];
+    uint32_t ph[G][4], pl[G][4];
     bool moved = false;
-    float alpha[2];
+    float alpha[B];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < B; ++b) {
       if (masked) {
 #pragma unroll
         for (int j = 0; j < 2 * G; ++j)
@@ -235,16 +239,14 @@ struct Rows {
       alpha[b] = ex2f(m[b] - from);
       moved |= to > m[b];
       m[b] = to;
-      // weights go to the products in bf16: each is off by at most 2^-8 of
-      // itself, and l sums the rounded ones, so a constant V comes out exact
+      // weights go to the products as two bf16 (split_weights), which takes twice the MMAs of more than eight rows
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 2 * G; ++j) {
-        const __nv_bfloat162 two =
-            __floats2bfloat162_rn(ex2f(fmaf(s[j][2 * b], sl2, -from)), ex2f(fmaf(s[j][2 * b + 1], sl2, -from)));
-        const uint32_t u = *reinterpret_cast<const uint32_t*>(&two);
-        pf[j >> 1][b + 2 * (j & 1)] = u;
-        sum += __uint_as_float(u << 16) + __uint_as_float(u & 0xffff0000u);
+        const float p0 = ex2f(fmaf(s[j][2 * b], sl2, -from)), p1 = ex2f(fmaf(s[j][2 * b + 1], sl2, -from));
+        sum += p0 + p1;
+        const int at = b + 2 * (j & 1);
+        split_weights(p0, p1, ph[j >> 1][at], FEW ? ph[j >> 1][at + 1] : pl[j >> 1][at]);
       }
       l[b] = l[b] * alpha[b] + sum;
     }
@@ -252,7 +254,7 @@ struct Rows {
 #pragma unroll
       for (int d = 0; d < HD / 8; ++d)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[d][e] *= alpha[e >> 1];
+        for (int e = 0; e < 4; ++e) o[d][e] *= alpha[FEW ? 0 : e >> 1];
     }
     // A row that does not see a key gives it weight 0, and 0 * inf is NaN: where
     // some rows see further than others and V holds something not finite, the
@@ -271,20 +273,33 @@ struct Rows {
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       if (!odd) {
+        // high parts of four 16-column blocks, then their low parts: a product does not wait for the one before
 #pragma unroll
-        for (int d = 0; d < HD / 16; ++d) {
-          uint32_t vf[4];  // dims lo (keys lo, hi), dims hi (keys lo, hi)
-          ldsm4t(vf, V + at<HD>(r0 + 16 * g + (lane & 7) + (((lane >> 3) & 1) << 3), d * 2 + (lane >> 4)));
-          mma_bf16_16816(o[2 * d], pf[g][0], pf[g][1], pf[g][2], pf[g][3], vf[0], vf[1]);
-          mma_bf16_16816(o[2 * d + 1], pf[g][0], pf[g][1], pf[g][2], pf[g][3], vf[2], vf[3]);
+        for (int d0 = 0; d0 < HD / 16; d0 += 4) {
+          uint32_t vf[4][4];  // dims lo (keys lo, hi), dims hi (keys lo, hi)
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            ldsm4t(vf[d], V + at<HD>(r0 + 16 * g + (lane & 7) + (((lane >> 3) & 1) << 3), (d0 + d) * 2 + (lane >> 4)));
+#pragma unroll
+          for (int part = 0; part < B; ++part) {
+            const uint32_t(&p)[4] = part ? pl[g] : ph[g];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              mma_bf16_16816(o[2 * (d0 + d)], p[0], p[1], p[2], p[3], vf[d][0], vf[d][1]);
+              mma_bf16_16816(o[2 * (d0 + d) + 1], p[0], p[1], p[2], p[3], vf[d][2], vf[d][3]);
+            }
+          }
         }
       } else {
         for (int key = 0; key < 16; ++key) {
           const int from = (lane & ~3) | ((key & 7) >> 1);
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const uint32_t u = __shfl_sync(0xffffffffu, key < 8 ? pf[g][b] : pf[g][b + 2], from);
-            const float pw = (key & 1) ? __uint_as_float(u & 0xffff0000u) : __uint_as_float(u << 16);
+          for (int b = 0; b < B; ++b) {
+            const uint32_t(&rest)[4] = FEW ? ph[g] : pl[g];
+            const uint32_t hi = __shfl_sync(0xffffffffu, key < 8 ? ph[g][b] : ph[g][b + 2], from);
+            const uint32_t lo = __shfl_sync(0xffffffffu, key < 8 ? rest[b + FEW] : rest[b + 2 + FEW], from);
+            const float pw = (key & 1) ? __uint_as_float(hi & 0xffff0000u) + __uint_as_float(lo & 0xffff0000u)
+                                       : __uint_as_float(hi << 16) + __uint_as_float(lo << 16);
             const bool on = key0 + 16 * g + key < vis[b] && ((there >> (16 * g + key)) & 1u);
 #pragma unroll
             for (int d = 0; d < HD / 8; ++d) {
@@ -307,6 +322,12 @@ struct Rows {
     const PagedAttnArgs& a = w.a;
     const Pieces& pc = SHARED ? w.shared : w.own;
     const int lane = threadIdx.x & 31, quad = lane >> 2, col = (lane & 3) * 2;
+    if (FEW_ROWS && few()) {
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) o[d][e] += o[d][e + 2];
+    }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       float ls = l[b];
@@ -401,7 +422,7 @@ struct WarpWorker {
 #pragma unroll 1
     for (int i = 0; i < kStages - 1; ++i) load();
     const float sl2 = a.scale * kLog2e;
-    Rows<HD, SHARED> rows;
+    Rows<HD, SHARED, true> rows;
     bool fresh = true, first = false;
     for (int stage = 0;; stage = stage + 1 == kStages ? 0 : stage + 1) {
       if (fresh) {
@@ -412,7 +433,8 @@ struct WarpWorker {
       cp_wait<kStages - 1>();
       __syncwarp();
       const uint32_t K = ring + stage * 2 * kTileB;
-      rows.template keys<1>(sl2, K, K + kTileB, 0, sh.cc.k * kKeys, there[stage]);
+      if (rows.few()) rows.template keys<1, true>(sl2, K, K + kTileB, 0, sh.cc.k * kKeys, there[stage]);
+      else rows.template keys<1, false>(sl2, K, K + kTileB, 0, sh.cc.k * kKeys, there[stage]);
       __syncwarp();  // the stage may be filled again
       const bool last = sh.last(), more = sh.more(line);
       fresh = last || !more;
@@ -482,7 +504,7 @@ struct CtaWorker {
       load();
     }
     const float sl2 = a.scale * kLog2e;
-    Rows<HD, SHARED> rows;
+    Rows<HD, SHARED, false> rows;
     bool fresh = true, first = false;
     for (int t = 0;; ++t) {
       if (fresh) {
@@ -499,7 +521,7 @@ struct CtaWorker {
 #pragma unroll 1
         for (int i = 0; i < kKeys / 32; ++i) {  // two groups of 16 keys: one's latencies pass under the other's
           const uint32_t mask = there[t % (kStages + 1)][i];
-          if (mask) rows.template keys<2>(sl2, K, K + kTileB, i * 32, key0 + i * 32, mask);
+          if (mask) rows.template keys<2, false>(sl2, K, K + kTileB, i * 32, key0 + i * 32, mask);
         }
       }
       const bool last = sh.last(), more = sh.more(line);
@@ -759,7 +781,7 @@ cudaError_t launch(PagedWork& w, int num_sms, cudaStream_t st) {
   // The own part by warps up to 32 rows a sequence and KV head, on average;
   // beyond that a warp's 16 keys are loaded once too often, again for every 16
   // rows (32 sequences of 500 to 2500 positions, 32 heads on 4: 8, 24 and 32 rows
-  // 27, 42 and 43 us, by CTAs 41, 46 and 46; 64 rows 72 us, by CTAs 51).
+  // 28, 47 and 49 us, by CTAs 44, 51 and 51; 64 rows 85 us, by CTAs 56).
   const bool by_warp = rows <= 2 * Few::kRows * (int64_t)p.n_seqs;
   w.own_mt = by_warp ? Few::kRows : Many::kRows;
   w.own_keys = by_warp ? Few::kKeys : Many::kKeys;
@@ -769,10 +791,12 @@ cudaError_t launch(PagedWork& w, int num_sms, cudaStream_t st) {
   if (w.a.shared_len > 0) {
     // tcgen05 where it takes the pages and the prefix is more than two of a CTA's
     // 64 x 64 tiles to each of those (592): below, its start and end cost more than
-    // its tiles save (8 KV heads of 8 rows: 512 positions, 64 tiles, 15.5 us against
-    // 12.1; 4096, 512 tiles, 17.5 against 19.0; 8192, 1024 tiles, 20.9 against 24.7.
-    // 4 heads of 512 rows: 1024 positions, 512 tiles, 26.2 against 25.0; 2048, 1024
-    // tiles, 28.6 against 31.3; 8192 33.8 against 61.1).
+    // its tiles save (8 KV heads of 8 rows: 512 positions, 64 tiles, 16.1 us against
+    // 11.8; 4096, 512 tiles, 18.4 against 17.3; 8192, 1024 tiles, 22.3 against 22.4.
+    // 4 heads of 512 rows: 1024 positions, 512 tiles, 27.6 against 24.9; 2048, 1024
+    // tiles, 29.4 against 31.0; 8192 36.4 against 61.6).  Near the border the tiles
+    // alone do not tell: 4 heads of 64 rows on 8192, 512 tiles, take 23.2 us by CTAs
+    // and would take 21.1; 8 heads of one row on 8192, 1024 tiles, 21.4 and 20.2.
     const int64_t tiles = (int64_t)p.n_kv * ceil_div(rows, Many::kRows) * ceil_div(w.a.shared_len, Many::kKeys);
     const bool tc = paged_shared_tc_takes(p) && tiles > 2 * ctas;
     w.shared_mt = tc ? kTcRows : Many::kRows;

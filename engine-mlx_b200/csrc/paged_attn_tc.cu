@@ -5,10 +5,10 @@
 // attend the same S keys without a mask, so the prefix is two dense products
 // around a softmax: S = Q K^T, O = P V, rows in tiles of 128, keys in tiles of
 // 128.  K and V are read from HBM once per KV head and 256 rows.  A tile of 256
-// rows and 128 keys takes 1.82 us (1.65 with K and V in L2): 9.2 TFLOP/s an SM, of
-// the 11.4 that the library's measured rate comes to; the exponentials alone (128 x
-// 128 twice, 16 an SM and clock) 1.1.  A tile of up to 128 rows takes 1.35 us, the
-// time of its 64 KB on all SMs (7 TB/s out of L2 and HBM together).  A worker's start
+// rows and 128 keys takes 2.48 us (2.13 with K and V in L2): 10.1 TFLOP/s of MMAs an
+// SM, of the 11.4 that the library's measured rate comes to; the exponentials alone
+// (128 x 128 twice, 16 an SM and clock) 1.1.  A tile of up to 128 rows takes 1.61 us,
+// its 64 KB on all SMs 1.35 (7 TB/s out of L2 and HBM together).  A worker's start
 // (barriers, Q, the first keys) takes 4 us, the end (pieces to memory) 4.
 //
 // One CTA an SM, each with an even share of the (KV head, 256 rows, 128 keys)
@@ -37,8 +37,11 @@
 // place, so the group finds its next S ready.
 //
 // The maximum that the exponentials use moves only when a tile's exceeds it by
-// more than 2^8 (then O and l are rescaled); O / l does not depend on it.  P is
-// rounded to bf16 for its product (off by at most 2^-8 of each weight).
+// more than 2^8 (then O and l are rescaled); O / l does not depend on it.  P goes
+// to its product as the sum of two bf16 (off by at most 2^-14 of each weight, see
+// split_weights), which takes another half of the two products' MMAs: with one
+// bf16, off by 2^-8, a tile took 1.8 us, and the output's error was 1.4 times its own
+// rounding.
 #include <cudaTypedefs.h>
 
 #include <mutex>
@@ -54,7 +57,7 @@ constexpr int kThreads = 384;
 constexpr int kSlots = 5;
 constexpr int kMmaWarp = 8, kLoadWarp = 10, kKeyWarp = 11;
 constexpr float kRescale = 8.0f;
-constexpr uint32_t kCols = 512;  // S of the groups at 0 and 128 (P of a half over its first 32 columns), O at 256 and 384
+constexpr uint32_t kCols = 512;  // S of the groups at 0 and 128 (P of a half over it, high parts and low parts 32 columns each), O at 256 and 384
 constexpr int kValid = 4;        // tiles whose key masks are kept: a tile's V slot is free before the ring holds 3 later ones
 
 template <int HD>
@@ -350,8 +353,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t V = at16(v0, L::kRing + s * L::kTile + half * 8 * L::kGroup);
         if (ok) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)  // 16 keys a step: 8 columns of P, 16 rows of V
+          for (int k = 0; k < 4; ++k) {  // 16 keys a step: 8 columns of P, high and low parts, 16 rows of V
             umma_ta(tO, tS + 64 * half + 8 * k, at16(V, k * 2 * L::kGroup), id_pv, (k > 0 || half > 0 || !first) ? 1u : 0u);
+            umma_ta(tO, tS + 64 * half + 32 + 8 * k, at16(V, k * 2 * L::kGroup), id_pv, 1u);
+          }
         }
         umma_commit(&B.pv_done[g][half]);
       };
@@ -522,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t scale2 = pair32(sl2, sl2), base2 = pair32(nb, nb);
             uint64_t sum0 = 0, sum1 = 0;  // pairs of sums
             auto put = [&](int c, const float(&s)[32]) {  // P of keys 32 c .. 32 c + 31 of the half
-              uint32_t u[16];
+              uint32_t hi[16], lo[16];
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
                 float p0, p1;
@@ -531,10 +536,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 p1 = ex2f(p1);
                 uint64_t& sum = e & 1 ? sum1 : sum0;
                 sum = add2(sum, pair32(p0, p1));
-                const __nv_bfloat162 two = __floats2bfloat162_rn(p0, p1);
-                u[e] = *reinterpret_cast<const uint32_t*>(&two);
+                split_weights(p0, p1, hi[e], lo[e]);
               }
-              tst16u(tS + 64 * half + 16 * c, u);
+              tst16u(tS + 64 * half + 16 * c, hi);
+              tst16u(tS + 64 * half + 32 + 16 * c, lo);
             };
             my_turn(pair);
             put(0, sa);

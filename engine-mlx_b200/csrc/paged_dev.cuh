@@ -29,6 +29,19 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return d;
 }
 
+// Two weights, each as the sum of two bf16: hi below the weight, lo what is left, rounded (off by at most 2^-14 of the
+// weight).  Both are positive where the weight is, so that an infinite V stays what it is.
+__device__ __forceinline__ void split_weights(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+  constexpr float kBelow = 1.f - 0x1p-20f;
+  const uint64_t p = pair32(p0, p1);
+  float h0, h1, l0, l1;
+  split32(mul2(p, pair32(kBelow, kBelow)), h0, h1);
+  hi = __byte_perm(__float_as_uint(h0), __float_as_uint(h1), 0x7632);  // truncated
+  split32(fma2(pair32(__uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u)), pair32(-1.f, -1.f), p), l0, l1);
+  const __nv_bfloat162 l = __floats2bfloat162_rn(l0, l1);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
 __device__ __forceinline__ SeqInfo load_seq(const PagedArgs& p, int i, int shared) {
   return seq_info(p.indptr[i], p.indptr[i + 1], p.lengths[i], p.n_rows, shared, (int64_t)p.max_pages * p.page_size);
 }

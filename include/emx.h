@@ -255,7 +255,9 @@ int emx_sdpa_paged_workspace(emx_ctx* ctx, const emx_paged_kv* kv, const emx_pag
  * shared_len: whole pages, 0 for none; a sequence with rows has at least
  * shared_len + its rows positions.  Rows of a sequence not in order become
  * zeros, as do rows that see no page inside the cache (such a page's positions
- * are left out).  The workspace (256-byte aligned) belongs to this call until
+ * are left out).  Scores, maxima and sums are fp32; a weight enters the
+ * product with v as two bf16 whose sum is off by at most 2^-14 of it, and the
+ * output is rounded to bf16 once.  The workspace (256-byte aligned) belongs to this call until
  * it has run: calls that can overlap, or graphs that do, take one each. */
 int emx_sdpa_paged(emx_ctx* ctx, const void* q, const emx_paged_kv* kv, const emx_paged_batch* batch, int n_q, float scale,
                    int shared_len, const int32_t* shared_pages, void* out, void* workspace, size_t workspace_bytes);

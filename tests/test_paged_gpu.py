@@ -753,3 +753,55 @@ def test_long_and_short_prefixes_one_after_another(ctx):
     for out in outs:
         for o, w in zip(out, want):
             assert (o.read(np.uint16, w.shape) == w).all()
+
+
+# ------------------------------------------------------------------------------------------------- the weights' precision
+@pytest.mark.parametrize("rows,n_q,n_kv,hd", [(1, 32, 4, 128), (1, 16, 8, 64), (40, 8, 2, 128), (40, 8, 2, 64)])
+def test_the_output_is_rounded_once(ctx, rows, n_q, n_kv, hd):
+    """Own parts by warps (one row a sequence) and by CTAs: the error's root mean square is that of one rounding to bf16.
+    What else there is of it: weights off by at most 2^-14, scores by 2^-13 of a weight (128 products of 2^-24, of sums
+    |q k| scale up to 8), and as V is drawn apart from q and k, an error e of every weight moves the output by e |o| in
+    the mean square; the sum of the weights adds as much again.  2^-11 in all, against 0.0016 |o| for the rounding."""
+    c = Case(61, [rows] * 6, [500 + 100 * i for i in range(6)], n_q, n_kv, hd).device(ctx)
+    want, _ = c.attend()
+    g = emx.f32(attend(ctx, c)[:c.n]).astype(np.float64)
+    rms = lambda x: np.sqrt((x * x).mean())  # noqa: E731
+    extra = 2.0 ** -11 * rms(want)
+    assert rms(g - want) <= np.hypot(rms(emx.f32(emx.bf16(want)) - want), extra)
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("seqs", [12, 20, 45])
+def test_the_output_over_a_long_prefix_is_rounded_once(ctx, seqs, hd):
+    c = long_prefix(62, 16, hd, seqs).device(ctx)
+    want, _ = c.attend()
+    g = emx.f32(attend(ctx, c)[:c.n]).astype(np.float64)
+    rms = lambda x: np.sqrt((x * x).mean())  # noqa: E731
+    extra = 2.0 ** -11 * rms(want)
+    assert rms(g - want) <= np.hypot(rms(emx.f32(emx.bf16(want)) - want), extra)
+
+
+@pytest.mark.parametrize("seqs,prefix", [(1, 0), (3, 64), (12, 2560), (45, 2560)])
+def test_a_constant_v_comes_out_as_it_is(ctx, seqs, prefix):
+    """Keys of one score below that of a single key, so that all their weights round the same way: the weights of the
+    products and those of the sum are the same to 2^-14 of each, well below the half step of 2^-9 that would show."""
+    for below in (0.3, 0.69, 1.1, 2.6):
+        c = Case(63, [1] * seqs, [prefix + 300] * seqs, 64, 8, page=16, shared=prefix)
+        c.q = emx.bf16(np.ones(c.q.shape))
+        c.k = emx.bf16(np.zeros(c.k.shape))
+        top = (c.shared_pages if prefix else c.table[0])[1]
+        c.k[top, :, 3] = emx.bf16(np.full((8, 128), below / (128 * c.scale)))
+        c.v = emx.bf16(np.broadcast_to(np.linspace(0.7, 1.4, 128), c.v.shape))
+        got = attend(ctx, c.device(ctx))
+        assert (got[:c.n] == c.v[0, 0, 0]).all()
+
+
+@pytest.mark.parametrize("seqs,prefix", [(1, 0), (12, 2560), (45, 2560)])
+def test_an_infinite_v_stays_infinite(ctx, seqs, prefix):
+    c = Case(64, [1] * seqs, [prefix + 40] * seqs, 64, 8, page=16, shared=prefix)
+    page = (c.shared_pages if prefix else c.table[0])[1]
+    c.v[page, 2, 7, 11], c.v[page, 2, 7, 12] = 0x7F80, 0xFF80
+    g = emx.f32(attend(ctx, c.device(ctx))[:c.n])
+    assert (g[:, 16:24, 11] == np.inf).all() and (g[:, 16:24, 12] == -np.inf).all()
+    g[:, 16:24, 11:13] = 0
+    assert np.isfinite(g).all()
