@@ -49,8 +49,9 @@ int check_shape(const char* op, const emx_paged_kv* kv, const emx_paged_batch* b
   PG_REQUIRE(b->n_seqs >= 0 && b->n_seqs <= kMaxSeqs, "%s: n_seqs %d outside [0, %d]", op, b->n_seqs, kMaxSeqs);
   PG_REQUIRE(b->n_rows >= 0 && (int64_t)b->n_rows * n_q <= 0x7fffffff, "%s: n_rows %d is negative or too large for %d heads",
              op, b->n_rows, n_q);
-  PG_REQUIRE(b->max_pages >= 1 && (int64_t)b->max_pages * kv->page_size <= 0x7fffffff,
-             "%s: max_pages %d of %d positions outside [1, 2^31)", op, b->max_pages, kv->page_size);
+  // the last key tile ends up to 127 positions behind a sequence, still in int32
+  PG_REQUIRE(b->max_pages >= 1 && (int64_t)b->max_pages * kv->page_size <= 0x7fffffff - 255,
+             "%s: max_pages %d of %d positions outside [1, 2^31 - 256]", op, b->max_pages, kv->page_size);
   return EMX_OK;
 }
 

@@ -218,7 +218,8 @@ typedef struct {
  * stands at position lengths[i] - c + j.  Position p is in page
  * table[i * max_pages + p / page_size], at row p % page_size of it.
  * indptr[0] >= 0, ascending; rows from indptr[n_seqs] to n_rows belong to
- * nobody and what would be written for them stays as it was.  n_seqs <= 1024.
+ * nobody and what would be written for them stays as it was.  n_seqs <= 1024,
+ * max_pages * page_size <= 2^31 - 256.
  * A sequence whose rows or length cannot be (rows outside [0, n_rows), fewer
  * positions than rows) reports EMX_DEV_BAD_BATCH, one longer than its table
  * EMX_DEV_KV_OVERFLOW, a page outside [0, n_pages) EMX_DEV_BAD_PAGE; nothing

@@ -96,6 +96,16 @@ def test_workspace_query_refuses():
     refused(f(None, kv(k=None, v=None), batch(indptr=None, lengths=None, table=None), 4, 0, C.byref(n)), "null context")
 
 
+@pytest.mark.parametrize("page_size,max_pages,fits", [(32767, 65538, False), (1, 2**31 - 1, False), (1, 2**31 - 255, False),
+                                                      (1, 2**31 - 256, True), (256, 2**23 - 1, True)])
+def test_the_last_key_tile_of_a_table_ends_in_int32(page_size, max_pages, fits):
+    """A tile of 64 positions behind a prefix that is no multiple of it may end beyond the table; its positions are int32."""
+    for call in (append, attend):
+        refused(call(kv_=kv(page_size=page_size), b=batch(max_pages=max_pages)), "null context" if fits else "max_pages")
+    refused(emx.lib().emx_sdpa_paged_workspace(None, kv(page_size=page_size), batch(max_pages=max_pages), 4, 0, C.byref(C.c_size_t())),
+            "null context" if fits else "max_pages")
+
+
 # ------------------------------------------------------------------------------------ the deal of tiles to workers
 HARNESS = r"""
 #include "paged_plan.h"
