@@ -375,10 +375,11 @@ struct Share {
   __device__ __forceinline__ bool more(const Line& line) const { return cc.x + 1 + (last() ? line.setup : 0) < x1; }
 };
 
-// Few rows (up to 16 a sequence and KV head): a warp is a worker, with 16 keys
+// Few rows (up to 32 a sequence and KV head): a warp is a worker, with 16 rows, 16 keys
 // a tile and three tiles in flight of its own, and never meets another.
 template <int HD, bool SHARED>
 struct WarpWorker {
+  static_assert(!SHARED, "a prefix has more rows");
   static constexpr int kRows = 16, kKeys = 16, kPerCta = kWarps;
   static constexpr int kTileB = kKeys * HD * 2;  // one tile of K (or V)
   static constexpr int kSmem = kWarps * kStages * 2 * kTileB;
@@ -394,7 +395,7 @@ struct WarpWorker {
     if (!sh.begin(line, x0, x1)) return;
     const uint64_t policy = l2_evict_first_policy();
     auto next_key = [&]() {
-      return key_at<SHARED>(a, sh.ld, (SHARED ? 0 : a.shared_len) + sh.ld.k * kKeys + (lane & 15));
+      return key_at<false>(a, sh.ld, a.shared_len + sh.ld.k * kKeys + (lane & 15));
     };
     Key key = next_key();
     int at_stage = 0;  // of the next load
@@ -422,7 +423,7 @@ struct WarpWorker {
 #pragma unroll 1
     for (int i = 0; i < kStages - 1; ++i) load();
     const float sl2 = a.scale * kLog2e;
-    Rows<HD, SHARED, true> rows;
+    Rows<HD, false, true> rows;
     bool fresh = true, first = false;
     for (int stage = 0;; stage = stage + 1 == kStages ? 0 : stage + 1) {
       if (fresh) {
@@ -438,7 +439,7 @@ struct WarpWorker {
       __syncwarp();  // the stage may be filled again
       const bool last = sh.last(), more = sh.more(line);
       fresh = last || !more;
-      if (fresh) rows.end(w, sh.cc, line.hpg, first && last && !SHARED && a.shared_len == 0, first, (size_t)worker * kRows);
+      if (fresh) rows.end(w, sh.cc, line.hpg, first && last && a.shared_len == 0, first, (size_t)worker * kRows);
       if (!more) break;
       sh.cc.next(line);
     }

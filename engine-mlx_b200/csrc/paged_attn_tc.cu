@@ -501,8 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             mx0 = max3(mx0, sa[15], sa[31]);
             mx1 = max3(mx1, sb[15], sb[31]);
-            float mx = fmaxf(max3(mx0, mx1, mx2), mx3) * sl2;
-            if (sl2 == 0.f) mx = 0.f;
+            const float mx = fmaxf(max3(mx0, mx1, mx2), mx3) * sl2;
             const bool up = mx > m + kRescale || (m == -INFINITY && mx > m);
             if (__any_sync(0xffffffffu, up)) {
               const float alpha = up ? ex2f(m - mx) : 1.f;  // 0 at the first tile
