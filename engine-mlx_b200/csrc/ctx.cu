@@ -123,6 +123,60 @@ using namespace emx;
     if (!(cond)) return fail(EMX_ERR_INVALID, __VA_ARGS__); \
   } while (0)
 
+namespace {
+
+void drop_stream(emx_ctx* c) {
+  if (c->own_stream) cudaStreamDestroy(c->stream);
+}
+
+// A context with a stream of its own, or on the caller's.
+int create_ctx(const char* what, int device, bool own_stream, cudaStream_t stream, emx_ctx** out) {
+  EMX_REQUIRE(out, "%s: out is null", what);
+  *out = nullptr;
+  int n = 0;
+  cudaError_t e = cudaGetDeviceCount(&n);
+  if (e != cudaSuccess || n == 0) {
+    cudaGetLastError();
+    return fail(EMX_ERR_CUDA, "%s: no CUDA device (%s)", what, cudaGetErrorString(e));
+  }
+  EMX_REQUIRE(device >= 0 && device < n, "%s: device %d out of range [0,%d)", what, device, n);
+  cudaDeviceProp prop;
+  EMX_CHECK_CUDA(cudaGetDeviceProperties(&prop, device), "cudaGetDeviceProperties");
+  if (prop.major != 10) return fail(EMX_ERR_CUDA, "%s: device %d is sm_%d%d; libemx is built for sm_100a", what, device,
+                                    prop.major, prop.minor);
+  EMX_CHECK_CUDA(cudaSetDevice(device), "cudaSetDevice");
+  emx_ctx* c = new emx_ctx();
+  c->device = device;
+  c->num_sms = prop.multiProcessorCount;
+  c->own_stream = own_stream;
+  c->stream = stream;
+  cudaError_t ce = own_stream ? cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking) : cudaSuccess;
+  if (ce != cudaSuccess) {
+    delete c;
+    return fail_cuda(ce, "cudaStreamCreate");
+  }
+  void* st = nullptr;
+  int rc = ctx_alloc(c, sizeof(int) * 4, &st);
+  if (rc) {
+    drop_stream(c);
+    delete c;
+    return rc;
+  }
+  c->status = static_cast<int*>(st);
+  cudaMemset(c->status, 0, sizeof(int) * 4);
+  c->gemm = gemm_ctx_create(0);
+  if (!c->gemm) {
+    ctx_free(c, c->status);
+    drop_stream(c);
+    delete c;
+    return fail(EMX_ERR_CUDA, "%s: cuBLAS handle creation failed", what);
+  }
+  *out = c;
+  return EMX_OK;
+}
+
+}  // namespace
+
 extern "C" {
 
 void emx_set_error_handler(emx_error_handler handler, void* data) {
@@ -135,47 +189,10 @@ const char* emx_last_error(void) { return g_last_error.c_str(); }
 
 const char* emx_version(void) { return "emx 0.1 (sm_100a)"; }
 
-int emx_ctx_create(int device, emx_ctx** out) {
-  EMX_REQUIRE(out, "emx_ctx_create: out is null");
-  *out = nullptr;
-  int n = 0;
-  cudaError_t e = cudaGetDeviceCount(&n);
-  if (e != cudaSuccess || n == 0) {
-    cudaGetLastError();
-    return fail(EMX_ERR_CUDA, "emx_ctx_create: no CUDA device (%s)", cudaGetErrorString(e));
-  }
-  EMX_REQUIRE(device >= 0 && device < n, "emx_ctx_create: device %d out of range [0,%d)", device, n);
-  cudaDeviceProp prop;
-  EMX_CHECK_CUDA(cudaGetDeviceProperties(&prop, device), "cudaGetDeviceProperties");
-  if (prop.major != 10) return fail(EMX_ERR_CUDA, "emx_ctx_create: device %d is sm_%d%d; libemx is built for sm_100a",
-                                    device, prop.major, prop.minor);
-  EMX_CHECK_CUDA(cudaSetDevice(device), "cudaSetDevice");
-  emx_ctx* c = new emx_ctx();
-  c->device = device;
-  c->num_sms = prop.multiProcessorCount;
-  cudaError_t ce = cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking);
-  if (ce != cudaSuccess) {
-    delete c;
-    return fail_cuda(ce, "cudaStreamCreate");
-  }
-  void* st = nullptr;
-  int rc = ctx_alloc(c, sizeof(int) * 4, &st);
-  if (rc) {
-    cudaStreamDestroy(c->stream);
-    delete c;
-    return rc;
-  }
-  c->status = static_cast<int*>(st);
-  cudaMemset(c->status, 0, sizeof(int) * 4);
-  c->gemm = gemm_ctx_create(0);
-  if (!c->gemm) {
-    ctx_free(c, c->status);
-    cudaStreamDestroy(c->stream);
-    delete c;
-    return fail(EMX_ERR_CUDA, "emx_ctx_create: cuBLAS handle creation failed");
-  }
-  *out = c;
-  return EMX_OK;
+int emx_ctx_create(int device, emx_ctx** out) { return create_ctx("emx_ctx_create", device, true, nullptr, out); }
+
+int emx_ctx_create_on_stream(int device, void* cuda_stream, emx_ctx** out) {
+  return create_ctx("emx_ctx_create_on_stream", device, false, static_cast<cudaStream_t>(cuda_stream), out);
 }
 
 int emx_ctx_destroy(emx_ctx* c) {
@@ -186,7 +203,7 @@ int emx_ctx_destroy(emx_ctx* c) {
   std::vector<void*> left;
   for (auto& kv : c->allocs) left.push_back(kv.first);
   for (void* p : left) ctx_free(c, p);
-  cudaStreamDestroy(c->stream);
+  drop_stream(c);
   delete c;
   return EMX_OK;
 }

@@ -15,6 +15,7 @@
 struct emx_ctx {
   int device = 0;
   cudaStream_t stream = nullptr;
+  bool own_stream = true;  // else the caller's
   int num_sms = 0;
   int* status = nullptr;  // device-side status word
   std::mutex mu;

@@ -58,6 +58,7 @@ _SIGS = {
     "emx_version": (C.c_char_p, []),
     "emx_set_error_handler": (None, [C.c_void_p, C.c_void_p]),
     "emx_ctx_create": (C.c_int, [C.c_int, C.POINTER(C.c_void_p)]),
+    "emx_ctx_create_on_stream": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(C.c_void_p)]),
     "emx_ctx_destroy": (C.c_int, [C.c_void_p]),
     "emx_ctx_stream": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "emx_ctx_num_sms": (C.c_int, [C.c_void_p, C.POINTER(C.c_int)]),
@@ -246,9 +247,15 @@ class PagedBatch:
 class Ctx:
     """MlxCtx equivalent: one device and one stream (crates/mlx-ffi/src/ops/real/mod.rs:4-41)."""
 
-    def __init__(self, device: int = 0):
+    def __init__(self, device: int = 0, stream=None):
+        """`stream`: a CUDA stream of the caller's to run on (a torch stream, or a handle as an int; 0 is the default
+        stream); else the context has one of its own."""
         h = C.c_void_p()
-        _check(lib().emx_ctx_create(int(device), C.byref(h)))
+        if stream is None:
+            _check(lib().emx_ctx_create(int(device), C.byref(h)))
+        else:
+            _check(lib().emx_ctx_create_on_stream(int(device), int(getattr(stream, "cuda_stream", stream)), C.byref(h)))
+        self.stream = stream  # kept alive
         self.h = h.value
         self.device = device
         self._workspace = None  # sdpa_paged's, where the caller brings none
@@ -430,8 +437,10 @@ class Ctx:
         return out
 
     # --- a batch of sequences over a paged cache; device arrays are Buffers or
-    # torch tensors, whose contents must be complete before the call: it runs
-    # on this context's stream
+    # torch tensors.  A call runs on this context's stream.  Tensors that are
+    # made and used on that stream (Ctx(stream=torch.cuda.current_stream()))
+    # need nothing more; else their contents must be complete before the call,
+    # and they must live, and not be read or written, until synchronize().
     def paged_append(self, qkv, kv, batch, n_q, q_norm=None, k_norm=None, eps=1e-6, theta=1e6, out=None):
         """Per-head norm and rotation of q and k, k and v to their pages; returns q bf16 [n_rows, n_q, head_dim]."""
         if out is None:

@@ -113,6 +113,15 @@ impl MlxCtx {
         check(unsafe { sys::emx_ctx_create(device, &mut raw) }, "emx_ctx_create")?;
         Ok(Self { raw })
     }
+    /// A context that runs on a CUDA stream of the caller's (null: the default stream).
+    ///
+    /// # Safety
+    /// `stream` must be a stream of `device` and outlive the context.
+    pub unsafe fn on_stream(device: i32, stream: *mut std::os::raw::c_void) -> Result<Self> {
+        let mut raw = std::ptr::null_mut();
+        check(sys::emx_ctx_create_on_stream(device, stream, &mut raw), "emx_ctx_create_on_stream")?;
+        Ok(Self { raw })
+    }
     pub fn raw(&self) -> *mut sys::emx_ctx {
         self.raw
     }

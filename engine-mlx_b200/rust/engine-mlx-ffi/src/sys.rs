@@ -112,6 +112,7 @@ extern "C" {
     pub fn emx_last_error() -> *const c_char;
     pub fn emx_version() -> *const c_char;
     pub fn emx_ctx_create(device: c_int, out: *mut *mut emx_ctx) -> c_int;
+    pub fn emx_ctx_create_on_stream(device: c_int, cuda_stream: *mut c_void, out: *mut *mut emx_ctx) -> c_int;
     pub fn emx_ctx_destroy(ctx: *mut emx_ctx) -> c_int;
     pub fn emx_ctx_stream(ctx: *mut emx_ctx, cuda_stream: *mut *mut c_void) -> c_int;
     pub fn emx_ctx_num_sms(ctx: *mut emx_ctx, n: *mut c_int) -> c_int;

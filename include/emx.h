@@ -63,6 +63,12 @@ typedef struct emx_ctx emx_ctx;
 /* MlxCtx::new / MlxCtx::gpu + mlx_default_gpu_stream_new
  * (crates/mlx-ffi/src/ops/real/mod.rs:19-33, crates/serve/src/engine.rs:69-80). */
 int emx_ctx_create(int device, emx_ctx** out);
+/* No reference counterpart: a context that runs on a stream of the caller's
+ * (of this device; null: the legacy default stream), in order with the
+ * caller's other work on it.  The stream outlives the context.  An engine
+ * whose steps are replayed as a graph needs a stream that can be captured,
+ * which the default one cannot. */
+int emx_ctx_create_on_stream(int device, void* cuda_stream, emx_ctx** out);
 int emx_ctx_destroy(emx_ctx* ctx);
 int emx_ctx_stream(emx_ctx* ctx, void** cuda_stream);
 int emx_ctx_num_sms(emx_ctx* ctx, int* n);
@@ -86,7 +92,11 @@ int emx_set_memory_limit(emx_ctx* ctx, size_t limit, size_t* previous);
 
 /* --------------------------------------------------------------------- ops
  * One entry per MlxCtx method on the Qwen3 path; all pointers are device
- * pointers, all work is enqueued on ctx's stream. */
+ * pointers, all work is enqueued on ctx's stream.  A context's own stream is
+ * ordered with no other, the default stream included: the caller waits, or
+ * orders them by events, before it calls on what another stream writes and
+ * before it reads or frees there what a call uses; or creates the context on
+ * that stream. */
 
 /* MlxCtx::quantized_matmul (crates/mlx-ffi/src/ops/real/transform.rs:77-89):
  * y[M,N] = x[M,K] . dequant(w)^T; transpose must be 1; bits 4|8; group 32|64|128.

@@ -76,3 +76,13 @@ def test_error_handler_receives_messages():
     finally:
         lib.emx_set_error_handler(None, None)
     assert got and "null" in got[0]
+
+
+def test_a_context_on_a_stream_wants_its_arguments():
+    lib = emx.lib()
+    assert lib.emx_ctx_create_on_stream(0, None, None) == emx.ERR_INVALID
+    assert "emx_ctx_create_on_stream" in lib.emx_last_error().decode()
+    if not _has_gpu():
+        with pytest.raises(emx.EmxError) as ei:
+            emx.Ctx(0, stream=0)
+        assert ei.value.code == emx.ERR_CUDA and "on_stream" in ei.value.msg

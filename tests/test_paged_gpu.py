@@ -805,3 +805,71 @@ def test_an_infinite_v_stays_infinite(ctx, seqs, prefix):
     assert (g[:, 16:24, 11] == np.inf).all() and (g[:, 16:24, 12] == -np.inf).all()
     g[:, 16:24, 11:13] = 0
     assert np.isfinite(g).all()
+
+
+# ------------------------------------------------------------------------------------------ on a stream of the caller's
+def tensor(torch, bits):
+    return torch.from_numpy(np.ascontiguousarray(bits).view(np.int16)).cuda().view(torch.bfloat16)
+
+
+@pytest.mark.parametrize("side", [False, True])
+def test_a_context_on_a_torch_stream(ctx, side):
+    """Inputs that are written behind long products, outputs that are read, and memory that is used again, all without a
+    wait: one stream orders them."""
+    torch = pytest.importorskip("torch")
+    c = Case(65, [1] * 40, [300 + 7 * i for i in range(40)], 16, 4, shared=160).device(ctx)
+    want = attend(ctx, c)[:c.n]
+    q0 = tensor(torch, c.q)
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream() if side else torch.cuda.default_stream()
+    on = emx.Ctx(0, stream=st)
+    assert stream_of(on) == (st.cuda_stream or None)
+    with torch.cuda.stream(st):
+        got = []
+        for _ in range(10):
+            x = torch.randn(4096, 4096, device="cuda")
+            for _ in range(6):
+                x = torch.tanh(x @ x)
+            q, out = torch.full_like(q0, float("nan")), torch.empty(c.n, 16, 128, dtype=torch.bfloat16, device="cuda")
+            q.copy_(torch.where(x[0, 0] > 2, q, q0))  # tanh: never
+            on.sdpa_paged(q, c.kv, c.batch, 16, c.scale, c.shared, c.d_shared, out=out)
+            del q
+            torch.full_like(q0, float("nan"))  # where q was
+            got.append(out.clone())
+            out.zero_()
+        torch.cuda.synchronize()
+    assert on.device_status() == 0
+    for g in got:
+        assert (g.cpu().view(torch.int16).numpy().view(np.uint16) == want).all()
+    on.close()
+    with torch.cuda.stream(st):  # still the caller's
+        assert float(torch.ones(8, device="cuda").sum()) == 8
+
+
+def test_a_context_on_a_torch_stream_is_captured_with_it(ctx):
+    torch = pytest.importorskip("torch")
+    c = Case(66, [1] * 20, [200 + 5 * i for i in range(20)], 8, 2, shared=64).device(ctx)
+    want = attend(ctx, c)[:c.n]
+    ctx.synchronize()
+    q0, st = tensor(torch, c.q), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    on = emx.Ctx(0, stream=st)
+    ws = on.alloc(on.sdpa_paged_workspace(c.kv, c.batch, 8, 64))
+    x = torch.zeros_like(q0)
+    out = torch.empty(c.n, 8, 128, dtype=torch.bfloat16, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st, capture_error_mode="thread_local"):
+        q = x * 0.5
+        on.sdpa_paged(q, c.kv, c.batch, 8, c.scale, 64, c.d_shared, out=out, workspace=ws)
+        twice = out * 2
+    with torch.cuda.stream(st):
+        x.copy_(q0 * 2)  # halved and doubled without rounding
+        g.replay()
+        x.zero_()
+        got = twice.clone()
+        g.replay()
+    torch.cuda.synchronize()
+    assert on.device_status() == 0
+    assert ((got * 0.5).cpu().view(torch.int16).numpy().view(np.uint16) == want).all()
+    del g
+    on.close()
