@@ -199,22 +199,26 @@ def _prepare_verify(case, g):
 
 
 # ---------------------------------------------------------------------------------------------------- the framework's
-_ctx = None
+_ctx = {}
 
 
 def _framework():
-    """The package and the program's context, made once."""
-    global _ctx
-    if _ctx is None:
-        sys.path.insert(0, os.path.join(os.getcwd(), "engine-mlx_b200"))
+    """The package and the program's context on the current device and stream, where the inputs are made and the outputs
+    used; made once for each."""
+    at = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
+    if at not in _ctx:
+        if not _ctx:
+            sys.path.insert(0, os.path.join(os.getcwd(), "engine-mlx_b200"))
         import emx
 
-        _ctx = emx, emx.Ctx(torch.cuda.current_device())
-    return _ctx
+        _ctx[at] = emx, emx.Ctx(at[0], stream=at[1])
+    return _ctx[at]
 
 
 def _run_own(s):
-    emx, ctx = _framework()
+    if "on" not in s:  # a program keeps its context, as it keeps to its stream
+        s["on"] = _framework()
+    emx, ctx = s["on"]
     if s["op"] == "verify":
         return ctx.verify_draft(s["target"], s["draft"], s["tokens"], s["uniforms"], s["n_seqs"], s["drafts"], s["vocab"],
                                 dtype=emx.F32 if s["target"].dtype == torch.float32 else emx.BF16, counts=s["counts"],
