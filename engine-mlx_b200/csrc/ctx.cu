@@ -163,7 +163,7 @@ int create_ctx(const char* what, int device, bool own_stream, cudaStream_t strea
     return rc;
   }
   c->status = static_cast<int*>(st);
-  cudaMemset(c->status, 0, sizeof(int) * 4);
+  cudaMemsetAsync(c->status, 0, sizeof(int) * 4, c->stream);
   c->gemm = gemm_ctx_create(0);
   if (!c->gemm) {
     ctx_free(c, c->status);
@@ -229,7 +229,8 @@ int emx_device_status(emx_ctx* c, int* status, int clear) {
   EMX_REQUIRE(c && status, "emx_device_status: null argument");
   EMX_CHECK_CUDA(cudaStreamSynchronize(c->stream), "emx_device_status");
   EMX_CHECK_CUDA(cudaMemcpy(status, c->status, sizeof(int), cudaMemcpyDeviceToHost), "status read");
-  if (clear) EMX_CHECK_CUDA(cudaMemset(c->status, 0, sizeof(int)), "status clear");
+  // on the stream: what comes next on it may report again
+  if (clear) EMX_CHECK_CUDA(cudaMemsetAsync(c->status, 0, sizeof(int), c->stream), "status clear");
   return EMX_OK;
 }
 

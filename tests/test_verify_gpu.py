@@ -206,6 +206,18 @@ def test_two_contexts_verify_at_once(ctx):
     other.close()
 
 
+def test_a_status_reported_after_another_was_cleared_is_kept(ctx):
+    """Clearing is ordered with what follows on the context's stream."""
+    t, d, x, u = (ctx.put(y) for y in inputs(12, 1, 1, 8))
+    bad = ctx.put(np.array([[8]], np.int32))
+    out, acc = ctx.put(np.zeros((1, 2), np.int32)), ctx.put(np.zeros(1, np.int32))
+    for _ in range(300):
+        ctx.verify_draft(t, d, bad, u, 1, 1, 8, out=out, accepted=acc)
+        assert ctx.device_status() == 3
+    ctx.verify_draft(t, d, x, u, 1, 1, 8, out=out, accepted=acc)
+    assert ctx.device_status() == 0
+
+
 # ------------------------------------------------------------------------------------------- a step, all of it together
 def test_speculative_steps_over_a_shared_prompt(ctx):
     """Three sequences with a common prompt take four steps of speculative decoding: the drafted rows are appended
