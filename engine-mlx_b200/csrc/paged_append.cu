@@ -91,10 +91,7 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const PagedAp
     const int i = warp_find_seq(p.indptr, p.n_seqs, row);
     if (i >= p.n_seqs || row < p.indptr[i]) continue;  // behind the last sequence: left as it was
     const SeqInfo s = load_seq(p, i, 0);
-    if (!s.ok) {
-      if (lane == 0) report_status(p.status, seq_status(p, i));
-      continue;
-    }
+    if (!s.ok) continue;
     const int pos = s.len - s.rows + (row - s.row0);
     const int pg = pos / p.page_size, page = p.table[(size_t)i * p.max_pages + pg];
     const bool store = page >= 0 && page < p.n_pages;
@@ -194,6 +191,10 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const PagedAp
       }
     }
   }
+  // sequences out of order report, those among them too that no row was found to belong to
+  if (blockIdx.x == gridDim.x - 1)
+    for (int i = threadIdx.x; i < p.n_seqs; i += kThreads)
+      if (!load_seq(p, i, 0).ok) report_status(p.status, seq_status(p, i));
 }
 
 template <int HD, bool TURN>

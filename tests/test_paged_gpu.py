@@ -873,3 +873,62 @@ def test_a_context_on_a_torch_stream_is_captured_with_it(ctx):
     assert ((got * 0.5).cpu().view(torch.int16).numpy().view(np.uint16) == want).all()
     del g
     on.close()
+
+
+# ------------------------------------------------------------------------- each thing that can be out of order, by itself
+OUT_OF_ORDER = [("lengths", 2, 1, 6), ("lengths", 1, 0, 6), ("lengths", 3, -1, 6), ("lengths", 0, -2**31, 6), ("lengths", 1, "room", 4),
+                ("lengths", 3, 2**31 - 1, 4), ("indptr", 4, 100, 6), ("indptr", 0, -1, 6), ("indptr", 2, 9, 6), ("indptr", 2, 0, 6),
+                ("table", (2, 1), "pages", 5), ("table", (0, 0), -1, 5), ("table", (3, 2), 2**31 - 1, 5), ("table", (1, 1), -2**31, 5)]
+
+
+@pytest.mark.parametrize("call", ["attend", "append"])
+@pytest.mark.parametrize("array,at,value,status", OUT_OF_ORDER)
+def test_each_input_out_of_order_has_its_status(ctx, array, at, value, status, call):
+    c = Case(67, [1, 2, 3, 1], [10, 20, 30, 48], 4, 2, pad=2)
+    c.max_pages = c.table.shape[1]
+    indptr, lens, table = c.indptr.copy(), np.array(c.lens, np.int32), c.table.copy()
+    {"indptr": indptr, "lengths": lens, "table": table}[array][at] = {"room": c.max_pages * 16 + 1, "pages": c.n_pages}.get(value, value)
+    c.device(ctx)
+    b = emx.PagedBatch(ctx.put(indptr), ctx.put(lens), ctx.put(table), 4, c.n_rows, c.max_pages)
+    out = ctx.alloc(c.n_rows * 4 * 128 * 2)
+    if call == "attend":
+        ctx.sdpa_paged(c.dq, c.kv, b, 4, c.scale, out=out)
+    else:
+        if array == "table":  # the page of a new row
+            row_page = {(2, 1): (27, 29), (0, 0): (9, 9), (3, 2): (47, 47), (1, 1): (18, 19)}[at]
+            assert row_page[0] // 16 == at[1] == row_page[1] // 16
+        ctx.paged_append(c.dqkv, c.kv, b, 4, out=out)
+    assert ctx.device_status() == status
+    attend(ctx, c)
+    assert c.status == 0
+
+
+@pytest.mark.parametrize("seqs,prefix", [(3, 64), (12, 2560)])
+@pytest.mark.parametrize("value", [-1, 1 << 30, "pages"])
+def test_a_bad_page_of_a_prefix_has_its_status(ctx, seqs, prefix, value):
+    c = Case(68, [1] * seqs, [prefix + 20] * seqs, 64, 8, page=16, shared=prefix).device(ctx)
+    attend(ctx, c)
+    assert c.status == 0
+    pages = c.shared_pages.copy()
+    pages[-1] = c.n_pages if value == "pages" else value
+    c.d_shared.write(pages)
+    attend(ctx, c)
+    assert c.status == 5
+
+
+def test_scores_of_any_size_where_one_key_decides(ctx):
+    """Scores of some thousands.  Their fp32 products are off by at most 130 * 2^-24 of sum |q k| scale: where the largest is
+    ahead of the next by that twice and 20 more, the others' weights come to less than 300 e^-20 = 2^-20."""
+    c = Case(9, [2, 1], [300, 160], 4, 2)
+    c.k, c.q = emx.bf16(emx.f32(c.k) * 60), emx.bf16(emx.f32(c.q) * 30)
+    want, size = c.attend()
+    ok = np.zeros((c.n, 4), bool)
+    for i in range(2):
+        k = c.keys(i)
+        for j, p in enumerate(c.positions(i)):
+            q = emx.f32(c.q[c.indptr[i] + j]).astype(np.float64).reshape(2, 2, 128)
+            s = np.sort(np.einsum("hgd,shd->hgs", q, k[:p + 1]).reshape(4, -1) * c.scale, -1)
+            off = np.einsum("hgd,shd->hgs", np.abs(q), np.abs(k[:p + 1])).reshape(4, -1).max(-1) * c.scale * 130 * 2.0 ** -24
+            ok[c.indptr[i] + j] = s[:, -1] - s[:, -2] > 20 + 2 * off
+    assert ok.mean() > 0.7
+    assert near(attend(ctx, c.device(ctx))[:c.n], want, size)[ok].all()
