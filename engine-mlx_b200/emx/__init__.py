@@ -217,11 +217,44 @@ class Buffer:
         return out
 
 
-def _ptr(x) -> Optional[int]:
-    """Device address of a Buffer, or of anything with data_ptr() (a torch tensor); None for None."""
+class _Kind:
+    """A type of array elements: torch's name for it, and torch's object once a tensor of it has been seen."""
+
+    def __init__(self, name: str):
+        self.name, self.dtype = name, None
+
+
+_BF16, _F32, _I32 = _Kind("bfloat16"), _Kind("float32"), _Kind("int32")
+
+
+def _ptr(x, kind: _Kind, device: Optional[int] = None) -> Optional[int]:
+    """Device address of a Buffer, or of a torch tensor (anything with data_ptr()); None for None.  A tensor is
+    contiguous, of type `kind`, and on a GPU, that one where `device` is given."""
     if x is None:
         return None
-    return x.ptr if isinstance(x, Buffer) else x.data_ptr()
+    if x.__class__ is Buffer:
+        return x.ptr
+    t = getattr(x, "dtype", None)
+    if t is None:
+        return x.data_ptr()
+    # first what a tensor in order is: a small call's time is the host's
+    if t is kind.dtype and x.get_device() == device and x.is_contiguous():
+        return x.data_ptr()
+    name, at = str(t).rsplit(".", 1)[-1], x.get_device()
+    if name != kind.name or at < 0 or (device is not None and at != device) or not x.is_contiguous():
+        raise EmxError(ERR_INVALID, "a contiguous %s tensor on %s is wanted, not a %s%s on %s" % (
+            kind.name, "a GPU" if device is None else "GPU %d" % device, "" if x.is_contiguous() else "strided ", name,
+            "GPU %d" % at if at >= 0 else "the host"))
+    kind.dtype = t
+    return x.data_ptr()
+
+
+def _device(*xs) -> Optional[int]:
+    """The GPU that Buffers and tensors are on (None: not known)."""
+    at = {x.ctx.device if isinstance(x, Buffer) else x.get_device() for x in xs if isinstance(x, Buffer) or hasattr(x, "get_device")}
+    if len(at) > 1:
+        raise EmxError(ERR_INVALID, "arrays on several GPUs: %s" % sorted(at))
+    return at.pop() if at else None
 
 
 class PagedKV:
@@ -230,7 +263,8 @@ class PagedKV:
 
     def __init__(self, k, v, n_pages: int, page_size: int, n_kv: int, head_dim: int):
         self.k, self.v = k, v
-        self.c = PagedKVStruct(_ptr(k), _ptr(v), n_pages, page_size, n_kv, head_dim)
+        self.c = PagedKVStruct(_ptr(k, _BF16), _ptr(v, _BF16), n_pages, page_size, n_kv, head_dim)
+        self.device = _device(k, v)
 
 
 class PagedBatch:
@@ -240,7 +274,8 @@ class PagedBatch:
 
     def __init__(self, indptr, lengths, table, n_seqs: int, n_rows: int, max_pages: int):
         self.indptr, self.lengths, self.table = indptr, lengths, table
-        self.c = PagedBatchStruct(n_seqs, n_rows, max_pages, _ptr(indptr), _ptr(lengths), _ptr(table))
+        self.c = PagedBatchStruct(n_seqs, n_rows, max_pages, *(_ptr(x, _I32) for x in (indptr, lengths, table)))
+        self.device = _device(indptr, lengths, table)
         self._workspace = {}  # sdpa_paged's bytes, by what else they depend on
 
 
@@ -441,12 +476,19 @@ class Ctx:
     # made and used on that stream (Ctx(stream=torch.cuda.current_stream()))
     # need nothing more; else their contents must be complete before the call,
     # and they must live, and not be read or written, until synchronize().
+    def _elsewhere(self, kv, batch):
+        if not {kv.device, batch.device} <= {self.device, None}:
+            raise EmxError(ERR_INVALID, "the context is on GPU %d, the cache or the batch on another" % self.device)
+
     def paged_append(self, qkv, kv, batch, n_q, q_norm=None, k_norm=None, eps=1e-6, theta=1e6, out=None):
         """Per-head norm and rotation of q and k, k and v to their pages; returns q bf16 [n_rows, n_q, head_dim]."""
+        if kv.device != self.device or batch.device != self.device:
+            self._elsewhere(kv, batch)
         if out is None:
             out = self.alloc(batch.c.n_rows * n_q * kv.c.head_dim * 2)
-        _check(lib().emx_paged_append(self.h, _ptr(qkv), _ptr(q_norm), _ptr(k_norm), eps, theta, n_q, kv.c, batch.c,
-                                      _ptr(out)))
+        at = self.device
+        _check(lib().emx_paged_append(self.h, _ptr(qkv, _BF16, at), _ptr(q_norm, _BF16, at), _ptr(k_norm, _BF16, at), eps, theta,
+                                      n_q, kv.c, batch.c, _ptr(out, _BF16, at)))
         return out
 
     def sdpa_paged_workspace(self, kv, batch, n_q, shared_len=0) -> int:
@@ -459,6 +501,8 @@ class Ctx:
         """Attention of the batch's rows, the first shared_len positions read once for all; `workspace` is a
         Buffer of sdpa_paged_workspace bytes (by default one that the context keeps and grows).  Graphs that can
         run at the same time as another call take one of their own."""
+        if kv.device != self.device or batch.device != self.device:
+            self._elsewhere(kv, batch)
         if out is None:
             out = self.alloc(batch.c.n_rows * n_q * kv.c.head_dim * 2)
         if workspace is None:
@@ -470,8 +514,9 @@ class Ctx:
                 # the one before stays allocated until the context closes: a captured graph may hold its address
                 self._workspace = self.alloc(need if self._workspace is None else max(need, 2 * self._workspace.nbytes))
             workspace = self._workspace
-        _check(lib().emx_sdpa_paged(self.h, _ptr(q), kv.c, batch.c, n_q, scale, shared_len, _ptr(shared_pages), _ptr(out),
-                                    workspace.ptr, workspace.nbytes))
+        at = self.device
+        _check(lib().emx_sdpa_paged(self.h, _ptr(q, _BF16, at), kv.c, batch.c, n_q, scale, shared_len, _ptr(shared_pages, _I32, at),
+                                    _ptr(out, _BF16, at), workspace.ptr, workspace.nbytes))
         return out
 
     def verify_draft(self, target, draft, tokens, uniforms, n_seqs, n_draft, vocab, dtype=F32, counts=None, out=None,
@@ -481,8 +526,10 @@ class Ctx:
             out = self.alloc(n_seqs * (n_draft + 1) * 4)
         if accepted is None:
             accepted = self.alloc(n_seqs * 4)
-        _check(lib().emx_verify_draft(self.h, _ptr(target), _ptr(draft), dtype, _ptr(tokens), _ptr(counts),
-                                      _ptr(uniforms), n_seqs, n_draft, vocab, _ptr(out), _ptr(accepted)))
+        kind, at = _F32 if dtype == F32 else _BF16, self.device
+        _check(lib().emx_verify_draft(self.h, _ptr(target, kind, at), _ptr(draft, kind, at), dtype, _ptr(tokens, _I32, at),
+                                      _ptr(counts, _I32, at), _ptr(uniforms, _F32, at), n_seqs, n_draft, vocab,
+                                      _ptr(out, _I32, at), _ptr(accepted, _I32, at)))
         return out, accepted
 
 

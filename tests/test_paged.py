@@ -106,6 +106,47 @@ def test_the_last_key_tile_of_a_table_ends_in_int32(page_size, max_pages, fits):
             "null context" if fits else "max_pages")
 
 
+class Tensor:
+    """What the binding looks at of a torch tensor."""
+
+    def __init__(self, dtype, device=0, contiguous=True):
+        self.dtype, self.device, self.contiguous = dtype, device, contiguous
+
+    def get_device(self):
+        return self.device
+
+    def is_contiguous(self):
+        return self.contiguous
+
+    def data_ptr(self):
+        return P
+
+
+def test_tensors_that_the_kernels_cannot_read_are_refused():
+    """On the host, on another GPU, strided, or of another type than the operator's."""
+    torch = pytest.importorskip("torch")
+    bf, i32, cpu = torch.bfloat16, torch.int32, torch.zeros
+    emx.PagedKV(Tensor(bf), Tensor(bf), 1, 1, 1, 64)
+    emx.PagedBatch(Tensor(i32), Tensor(i32), Tensor(i32), 1, 1, 1)
+    for bad, word in ((cpu(64, dtype=bf), "host"), (Tensor(bf, contiguous=False), "strided"), (Tensor(torch.float16), "float16"),
+                      (Tensor(bf, device=1), "several GPUs")):
+        for pair in ((bad, Tensor(bf)), (Tensor(bf), bad)):
+            with pytest.raises(emx.EmxError, match=word) as e:
+                emx.PagedKV(*pair, 1, 1, 1, 64)
+            assert e.value.code == emx.ERR_INVALID
+    for bad, word in ((cpu(2, dtype=i32), "host"), (Tensor(torch.int64), "int64"), (Tensor(i32, contiguous=False), "strided")):
+        for at in range(3):
+            arrays = [Tensor(i32) for _ in range(3)]
+            arrays[at] = bad
+            with pytest.raises(emx.EmxError, match=word):
+                emx.PagedBatch(*arrays, 1, 1, 1)
+    for _ in range(2):
+        for bad in (Tensor(torch.float32, device=1), Tensor(torch.float32, contiguous=False), cpu(3), Tensor(torch.int32)):
+            with pytest.raises(emx.EmxError, match="float32 tensor on GPU 0 is wanted, not a"):
+                emx._ptr(bad, emx._F32, 0)
+        assert emx._ptr(Tensor(torch.float32, device=1), emx._F32, 1) == P and emx._ptr(None, emx._F32, 1) is None
+
+
 # ------------------------------------------------------------------------------------ the deal of tiles to workers
 HARNESS = r"""
 #include "paged_plan.h"

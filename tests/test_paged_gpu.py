@@ -875,6 +875,28 @@ def test_a_context_on_a_torch_stream_is_captured_with_it(ctx):
     on.close()
 
 
+def test_tensors_of_other_types_and_places_are_refused(ctx):
+    """Before anything is launched."""
+    torch = pytest.importorskip("torch")
+    c = Case(72, [1, 2], [30, 20], 4, 2).device(ctx)
+    q, out = (torch.zeros(3, 4, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    qkv = torch.zeros(3, 8 * 128, dtype=torch.bfloat16, device="cuda")
+    t, u = torch.rand(2, 3, 50, device="cuda"), torch.rand(2, 3, device="cuda")
+    x = torch.zeros(2, 2, dtype=torch.int32, device="cuda")
+    for bad in (q.cpu(), q.half(), q.transpose(0, 1)):
+        for call in (lambda: ctx.sdpa_paged(bad, c.kv, c.batch, 4, c.scale, out=out), lambda: ctx.sdpa_paged(q, c.kv, c.batch, 4, c.scale, out=bad),
+                     lambda: ctx.paged_append(qkv, c.kv, c.batch, 4, out=bad)):
+            with pytest.raises(emx.EmxError, match="is wanted"):
+                call()
+    for args in ((t.double(), None, x, u), (t.cpu(), None, x, u), (t, t[:, :2], x, u), (t, None, x.long(), u), (t, None, x, u.bfloat16())):
+        with pytest.raises(emx.EmxError, match="is wanted"):
+            ctx.verify_draft(*args, 2, 2, 50)
+    with pytest.raises(emx.EmxError, match="is wanted"):
+        ctx.verify_draft(t, None, x, u, 2, 2, 50, dtype=emx.BF16)
+    ctx.verify_draft(t, t[:, :2].contiguous(), x, u, 2, 2, 50)
+    assert ctx.device_status() == 0
+
+
 # ------------------------------------------------------------------------- each thing that can be out of order, by itself
 OUT_OF_ORDER = [("lengths", 2, 1, 6), ("lengths", 1, 0, 6), ("lengths", 3, -1, 6), ("lengths", 0, -2**31, 6), ("lengths", 1, "room", 4),
                 ("lengths", 3, 2**31 - 1, 4), ("indptr", 4, 100, 6), ("indptr", 0, -1, 6), ("indptr", 2, 9, 6), ("indptr", 2, 0, 6),
@@ -932,3 +954,80 @@ def test_scores_of_any_size_where_one_key_decides(ctx):
             ok[c.indptr[i] + j] = s[:, -1] - s[:, -2] > 20 + 2 * off
     assert ok.mean() > 0.7
     assert near(attend(ctx, c.device(ctx))[:c.n], want, size)[ok].all()
+
+
+# ----------------------------------------------------------------- the tensor-memory kernel by the arithmetic of its choice
+def takes_tensor_memory(ctx, c):
+    """Whether the prefix has more than two 64 x 64 tiles to each of two CTAs an SM, in pages of whole 8-row groups."""
+    return c.page % 8 == 0 and c.n_kv * -(-c.n_rows * (c.n_q // c.n_kv) // 64) * -(-c.shared // 64) > 4 * ctx.num_sms
+
+
+def attend_64(c):
+    """Case.attend on the device."""
+    torch = pytest.importorskip("torch")
+    t = lambda x: torch.from_numpy(emx.f32(x)).cuda().double()  # noqa: E731
+    k, v, q = t(c.k), t(c.v), t(c.q)
+    out, size = (np.zeros((c.n, c.n_q, c.hd)) for _ in range(2))
+    for i in range(c.n_seqs):
+        p = torch.arange(c.lens[i], device="cuda")
+        pages, off = torch.from_numpy(c.table[i]).cuda().long()[p // c.page], p % c.page
+        ks, vs = k[pages, :, off], v[pages, :, off]
+        for j, pos in enumerate(c.positions(i)):
+            row = c.indptr[i] + j
+            s = torch.einsum("hgd,shd->hgs", q[row].view(c.n_kv, -1, c.hd), ks[:pos + 1]) * c.scale
+            w = torch.softmax(s, -1)
+            out[row] = torch.einsum("hgs,shd->hgd", w, vs[:pos + 1]).reshape(c.n_q, c.hd).cpu().numpy()
+            size[row] = torch.einsum("hgs,shd->hgd", w, vs[:pos + 1].abs()).reshape(c.n_q, c.hd).cpu().numpy()
+    return out, size
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("seqs,n_q,n_kv,shared", [(300, 128, 64, 128), (300, 128, 64, 1040), (15, 1000, 50, 2080), (17, 960, 48, 2048)])
+def test_workers_go_from_segment_to_segment(ctx, seqs, n_q, n_kv, shared, hd):
+    """More segments than SMs, and fewer where whole workers to each would take too long: a worker goes from tiles of two
+    groups' rows to those of one and back."""
+    r = np.random.default_rng(69)
+    c = Case(69, [1] * seqs, shared + 1 + r.integers(0, 20, seqs), n_q, n_kv, hd, shared=shared)
+    rows, kt = seqs * n_q // n_kv, -(-shared // 128)
+    segments = n_kv * -(-rows // 256)
+    per = -(-segments * kt // ctx.num_sms)
+    assert takes_tensor_memory(ctx, c) and (segments > ctx.num_sms or -(-kt // (ctx.num_sms // segments)) > per + 4)
+    got = attend(ctx, c.device(ctx))
+    assert c.status == 0 and near(got[:c.n], *attend_64(c)).all()
+
+
+@pytest.mark.parametrize("seqs", [12, 45])
+def test_a_page_may_stand_for_several_of_a_long_prefix(ctx, seqs):
+    c = long_prefix(70, 16, 128, seqs)
+    for a, b in ((2, 0), (9, 8), (40, 0)):
+        c.shared_pages[a] = c.shared_pages[b]
+    c.table[:, :len(c.shared_pages)] = c.shared_pages
+    assert takes_tensor_memory(ctx, c)
+    got = attend(ctx, c.device(ctx))
+    assert c.status == 0 and near(got[:c.n], *attend_64(c)).all()
+
+
+@pytest.mark.parametrize("seqs", [12, 45])
+def test_a_long_prefix_past_32_bits(ctx, seqs):
+    """Its pages at both ends and in the middle of a cache of more than 2^32 elements."""
+    c = long_prefix(71, 128, 128, seqs)
+    assert takes_tensor_memory(ctx, c)
+    page = 8 * 128 * 128
+    pages = 2 ** 32 // page + 128
+    want = attend_64(c)
+    k, v = (ctx.alloc(pages * page * 2) for _ in range(2))
+    assert c.n_pages <= 90
+    far = np.concatenate([np.arange(30), pages // 2 + np.arange(20), np.arange(pages - 40, pages)])[:c.n_pages]
+    far = np.random.default_rng(71).permutation(far).astype(np.int32)
+    c.device(ctx)
+    for j, to in enumerate(far):
+        k.write(c.k[j], int(to) * page * 2)
+        v.write(c.v[j], int(to) * page * 2)
+    move = lambda t: np.where((t >= 0) & (t < c.n_pages), far[np.clip(t, 0, c.n_pages - 1)], -7).astype(np.int32)  # noqa: E731
+    c.kv = emx.PagedKV(k, v, pages, 128, 8, 128)
+    c.batch = emx.PagedBatch(c.d_indptr, c.d_lens, ctx.put(move(c.table)), c.n_seqs, c.n_rows, c.max_pages)
+    c.d_shared = ctx.put(move(c.shared_pages))
+    got = attend(ctx, c)
+    k.free()
+    v.free()
+    assert c.status == 0 and near(got[:c.n], *want).all()
