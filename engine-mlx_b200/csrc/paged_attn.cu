@@ -543,11 +543,14 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const __grid_co
   using Worker = W<HD, SHARED>;
   const Line line = make_line(w.a.p, w.a.shared_len, !SHARED, Worker::kRows, Worker::kKeys, SHARED ? 0 : kSetup, starts);
   // The first kernel of a call waits for what ran before it.  An own part that
-  // follows a shared one has been let go by it after such a wait; it needs
-  // nothing of that one, but the join waits for this kernel alone, so it ends
-  // after the other.
+  // follows a shared one has been let go by it after such a wait, so what ran before
+  // is complete and in memory, but only a grid's own wait is promised to show it to
+  // that grid: here a fence drops what L1 may hold from earlier.  It needs nothing of
+  // the shared part, but the join waits for this kernel alone, so it ends after the
+  // other.
   const bool first = SHARED || w.a.shared_len == 0;
   if (first) pdl_wait();
+  else __threadfence();
   pdl_trigger();
   int64_t total;
   if (SHARED) {
@@ -590,6 +593,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   const PagedAttnArgs& a = w.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_trigger();
+  __threadfence();  // the batch is in memory, as for the own part; the pieces only after the wait
   const int hpg = a.p.n_q / a.p.n_kv, items = a.p.n_rows * a.p.n_q;
   const int part = warp % parts, stride = gridDim.x * (4 / parts);
   const Line own = make_line(a.p, a.shared_len, true, w.own_mt, w.own_keys, kSetup, w.starts);
