@@ -145,6 +145,11 @@ int create_ctx(const char* what, int device, bool own_stream, cudaStream_t strea
   if (prop.major != 10) return fail(EMX_ERR_CUDA, "%s: device %d is sm_%d%d; libemx is built for sm_100a", what, device,
                                     prop.major, prop.minor);
   EMX_CHECK_CUDA(cudaSetDevice(device), "cudaSetDevice");
+  if (!own_stream) {  // what the context sets up on it has to run now
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    EMX_CHECK_CUDA(cudaStreamIsCapturing(stream, &cap), what);
+    if (cap != cudaStreamCaptureStatusNone) return fail(EMX_ERR_STATE, "%s: the stream is being captured", what);
+  }
   emx_ctx* c = new emx_ctx();
   c->device = device;
   c->num_sms = prop.multiProcessorCount;

@@ -64,8 +64,8 @@ typedef struct emx_ctx emx_ctx;
  * (crates/mlx-ffi/src/ops/real/mod.rs:19-33, crates/serve/src/engine.rs:69-80). */
 int emx_ctx_create(int device, emx_ctx** out);
 /* No reference counterpart: a context that runs on a stream of the caller's
- * (of this device; null: the legacy default stream), in order with the
- * caller's other work on it.  The stream outlives the context.  An engine
+ * (of this device, not being captured; null: the legacy default stream), in
+ * order with the caller's other work on it.  The stream outlives the context.  An engine
  * whose steps are replayed as a graph needs a stream that can be captured,
  * which the default one cannot. */
 int emx_ctx_create_on_stream(int device, void* cuda_stream, emx_ctx** out);

@@ -875,6 +875,24 @@ def test_a_context_on_a_torch_stream_is_captured_with_it(ctx):
     on.close()
 
 
+def test_a_context_is_not_made_on_a_stream_that_is_captured(ctx):
+    torch = pytest.importorskip("torch")
+    st, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    x = torch.ones(4, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=st, capture_error_mode="thread_local"):
+        y = x + 1
+        with pytest.raises(emx.EmxError, match="captured") as e:
+            emx.Ctx(0, stream=st)
+        assert e.value.code == emx.ERR_STATE
+    g.replay()
+    torch.cuda.synchronize()
+    assert (y == 2).all()
+    on = emx.Ctx(0, stream=st)
+    assert on.device_status() == 0
+    on.close()
+
+
 def test_tensors_of_other_types_and_places_are_refused(ctx):
     """Before anything is launched."""
     torch = pytest.importorskip("torch")
