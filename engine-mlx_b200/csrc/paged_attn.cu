@@ -814,8 +814,10 @@ cudaError_t launch(PagedWork& w, int num_sms, cudaStream_t st) {
       if (segments <= workers) {
         // A worker that goes from one segment to the next stores one's rows and
         // loads the other's Q with nothing to compute meanwhile: about four
-        // tiles' time.  Whole workers to a segment where the tiles that costs are
-        // fewer (64 rows a head on 32768: 15 tiles against 14 and a change).
+        // tiles' time.  Whole workers to a segment where that is not fewer tiles
+        // than it costs (40 and 60 segments of 64 to 256 rows: 3 tiles more than even
+        // shares have take 0.90 to 1.00 of their time, 4 tiles 0.97 to 1.03, 6 tiles
+        // 1.01 to 1.07).
         const int split = (int)(workers / segments), per = ceil_div(kt, split);
         if (per <= w.shared_per + 4) {
           w.shared_split = split;

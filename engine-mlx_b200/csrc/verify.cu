@@ -10,7 +10,8 @@
 //   as the first index whose running sum of r exceeds u_last * sum r,
 // which leaves every token distributed as p.  Comparisons and sums are in
 // fp64: u q is exact there (24 + 24 bits), and a running sum over 10^5 fp32
-// values keeps a border's place to ~1e-11 of the mass.
+// values keeps a border's place to ~1e-11 of the mass.  (Of p - q, its rounding to
+// fp32 is summed in fp64 and what that leaves, below 2^-24 of it, in fp32 beside.)
 //
 // Only the row that the next token is drawn from is read whole: V values of p
 // and, after a refusal, V of q, once; that stream bounds a batch, and one
@@ -21,7 +22,7 @@
 // remote is touched behind it; the CTA whose slice holds the token then walks
 // the run of the warp that does, all its threads together, out of L2.
 //
-// 64 sequences over 151936 fp32 values, p and q (78 MB): 23.5 us, 3.3 TB/s, half of
+// 64 sequences over 151936 fp32 values, p and q (78 MB): 23.4 us, 3.3 TB/s, half of
 // which are the chain's other links (7.0 us for one sequence: the drafts' two
 // dependent loads, the row, two reductions, the walk).
 #include <cooperative_groups.h>
@@ -320,12 +321,12 @@ template <typename T, int VEC>
 cudaError_t run(const VerifyArgs& a, int num_sms, cudaStream_t st) {
   // As many threads as there is room for, so that a thread's share of the row is a
   // load or two: sixteen CTAs of 512 a sequence while each has an SM of its own (one
-  // sequence of 151936: 7.2 us, with eight 9.3), then eight, of 512 threads where
+  // sequence of 151936: 7.0 us, with eight 9.3), then eight, of 512 threads where
   // 256 would take more than one round of loads (24 and 32 sequences of 151936: 14.7
   // and 16.0 us, of 256 17.8 and 18.1; of 32000 8.4 and 8.9 against 7.8).  Beyond seven
-  // quarters of an SM's worth each eight of 256, four on an SM, so that one's
-  // chain of latencies passes under the others' streams (37 sequences: 22.5 us, of
-  // 512 threads 23.2; 64: 23.5 and 28.4).
+  // quarters of an SM's worth each eight of 256, four on an SM, as all then begin
+  // at once (37 sequences: 22.5 us, of 512 threads 23.2; 64: 23.4 and 28.4); they go
+  // through the chain's links in step, so little of one's hides another's.
   if (a.n_seqs * 16 <= num_sms) return run<T, VEC, 512>(a, 16, st);
   const bool rounds = a.vocab > 8 * 256 * VEC * kLoads;
   if (rounds && a.n_seqs * 8 <= num_sms * 7 / 4) return run<T, VEC, 512>(a, 8, st);

@@ -283,8 +283,9 @@ int emx_sdpa_paged(emx_ctx* ctx, const void* q, const emx_paged_kv* kv, const em
  * itself where that has no mass), or from the row behind the last draft — the
  * first index whose running sum exceeds u times the total.  out int32[n_seqs,
  * n_draft + 1]: the accepted drafts, that token, then -1; accepted
- * int32[n_seqs]: how many drafts.  Comparisons and sums are in fp64; the rows
- * need not sum to 1, and entries that are negative or not finite carry no
+ * int32[n_seqs]: how many drafts.  Comparisons are exact and sums in fp64, but
+ * for what rounding p - q to fp32 leaves of it (below 2^-24), which is summed in
+ * fp32; the rows need not sum to 1, and entries that are negative or not finite carry no
  * mass.  No mass at all: -1 in the token's place.  counts[i] < 0: an empty
  * slot, all -1 and 0 accepted.  A draft outside [0, vocab) is refused
  * and reports EMX_DEV_BAD_TOKEN. */
