@@ -251,10 +251,15 @@ def _ptr(x, kind: _Kind, device: Optional[int] = None) -> Optional[int]:
 
 def _device(*xs) -> Optional[int]:
     """The GPU that Buffers and tensors are on (None: not known)."""
-    at = {x.ctx.device if isinstance(x, Buffer) else x.get_device() for x in xs if isinstance(x, Buffer) or hasattr(x, "get_device")}
-    if len(at) > 1:
-        raise EmxError(ERR_INVALID, "arrays on several GPUs: %s" % sorted(at))
-    return at.pop() if at else None
+    at = None
+    for x in xs:
+        d = x.ctx.device if x.__class__ is Buffer else x.get_device() if hasattr(x, "get_device") else at
+        if d is not None and d < 0:
+            raise EmxError(ERR_INVALID, "arrays on a GPU are wanted, not on the host")
+        if at is not None and d != at:
+            raise EmxError(ERR_INVALID, "arrays on several GPUs: %d and %d" % (at, d))
+        at = d
+    return at
 
 
 class PagedKV:
@@ -263,8 +268,8 @@ class PagedKV:
 
     def __init__(self, k, v, n_pages: int, page_size: int, n_kv: int, head_dim: int):
         self.k, self.v = k, v
-        self.c = PagedKVStruct(_ptr(k, _BF16), _ptr(v, _BF16), n_pages, page_size, n_kv, head_dim)
-        self.device = _device(k, v)
+        at = self.device = _device(k, v)
+        self.c = PagedKVStruct(_ptr(k, _BF16, at), _ptr(v, _BF16, at), n_pages, page_size, n_kv, head_dim)
 
 
 class PagedBatch:
@@ -274,8 +279,8 @@ class PagedBatch:
 
     def __init__(self, indptr, lengths, table, n_seqs: int, n_rows: int, max_pages: int):
         self.indptr, self.lengths, self.table = indptr, lengths, table
-        self.c = PagedBatchStruct(n_seqs, n_rows, max_pages, *(_ptr(x, _I32) for x in (indptr, lengths, table)))
-        self.device = _device(indptr, lengths, table)
+        at = self.device = _device(indptr, lengths, table)
+        self.c = PagedBatchStruct(n_seqs, n_rows, max_pages, _ptr(indptr, _I32, at), _ptr(lengths, _I32, at), _ptr(table, _I32, at))
         self._workspace = {}  # sdpa_paged's bytes, by what else they depend on
 
 
