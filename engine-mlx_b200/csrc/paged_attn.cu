@@ -23,7 +23,7 @@
 // alone, 5.4 TB/s; 54.3 us with the join), and a warp's own chain of latencies
 // elsewhere: a 16-key tile takes it 1.3 to 1.45 us, whether or not the SM's other
 // warps want memory.  Twelve warps an SM with two tiles each (against eight with
-// three) took 55.3 us, fewer instructions for the copies nothing off.  A short
+// three) took 55.3 us where these took 53.5, fewer instructions for the copies nothing off.  A short
 // sequence alone (132 positions) takes 8.7 us: three dependent loads (rows,
 // page, keys) and two kernels.
 #include "paged_attn.cuh"

@@ -236,7 +236,7 @@ def _ptr(x, kind: _Kind, device: Optional[int] = None) -> Optional[int]:
         return x.ptr
     t = getattr(x, "dtype", None)
     if t is None:
-        return x.data_ptr()
+        return x.ptr if isinstance(x, Buffer) else x.data_ptr()
     # first what a tensor in order is: a small call's time is the host's
     if t is kind.dtype and x.get_device() == device and x.is_contiguous():
         return x.data_ptr()
@@ -253,7 +253,7 @@ def _device(*xs) -> Optional[int]:
     """The GPU that Buffers and tensors are on (None: not known)."""
     at = None
     for x in xs:
-        d = x.ctx.device if x.__class__ is Buffer else x.get_device() if hasattr(x, "get_device") else at
+        d = x.ctx.device if isinstance(x, Buffer) else x.get_device() if hasattr(x, "get_device") else at
         if d is not None and d < 0:
             raise EmxError(ERR_INVALID, "arrays on a GPU are wanted, not on the host")
         if at is not None and d != at:
@@ -297,7 +297,7 @@ class Ctx:
             _check(lib().emx_ctx_create_on_stream(int(device), int(getattr(stream, "cuda_stream", stream)), C.byref(h)))
         self.stream = stream  # kept alive
         self.h = h.value
-        self.device = device
+        self.device = int(device)
         self._workspace = None  # sdpa_paged's, where the caller brings none
         self._num_sms = None
 
@@ -504,8 +504,9 @@ class Ctx:
 
     def sdpa_paged(self, q, kv, batch, n_q, scale, shared_len=0, shared_pages=None, out=None, workspace=None):
         """Attention of the batch's rows, the first shared_len positions read once for all; `workspace` is a
-        Buffer of sdpa_paged_workspace bytes (by default one that the context keeps and grows).  Graphs that can
-        run at the same time as another call take one of their own."""
+        Buffer of sdpa_paged_workspace bytes (by default one that the context keeps and grows; a capture, which cannot
+        allocate, wants `out`, and a workspace or an earlier call as large).  Graphs that can run at the same time as
+        another call take one of their own."""
         if kv.device != self.device or batch.device != self.device:
             self._elsewhere(kv, batch)
         if out is None:

@@ -65,9 +65,9 @@ typedef struct emx_ctx emx_ctx;
 int emx_ctx_create(int device, emx_ctx** out);
 /* No reference counterpart: a context that runs on a stream of the caller's
  * (of this device, not being captured; null: the legacy default stream), in
- * order with the caller's other work on it.  The stream outlives the context.  An engine
- * whose steps are replayed as a graph needs a stream that can be captured,
- * which the default one cannot. */
+ * order with the caller's other work on it.  The stream outlives the context.
+ * An engine whose steps are replayed as a graph needs a stream that can be
+ * captured, which the default one cannot. */
 int emx_ctx_create_on_stream(int device, void* cuda_stream, emx_ctx** out);
 int emx_ctx_destroy(emx_ctx* ctx);
 int emx_ctx_stream(emx_ctx* ctx, void** cuda_stream);
@@ -268,8 +268,9 @@ int emx_sdpa_paged_workspace(emx_ctx* ctx, const emx_paged_kv* kv, const emx_pag
  * zeros, as do rows that see no page inside the cache (such a page's positions
  * are left out).  Scores, maxima and sums are fp32; a weight enters the
  * product with v as two bf16 whose sum is off by at most 2^-14 of it, and the
- * output is rounded to bf16 once.  The workspace (256-byte aligned) belongs to this call until
- * it has run: calls that can overlap, or graphs that do, take one each. */
+ * output is rounded to bf16 once.  The workspace (256-byte aligned) belongs to
+ * this call until it has run: calls that can overlap, or graphs that do, take
+ * one each. */
 int emx_sdpa_paged(emx_ctx* ctx, const void* q, const emx_paged_kv* kv, const emx_paged_batch* batch, int n_q, float scale,
                    int shared_len, const int32_t* shared_pages, void* out, void* workspace, size_t workspace_bytes);
 /* Speculative sampling's acceptance for a batch of sequences, from given
@@ -285,10 +286,10 @@ int emx_sdpa_paged(emx_ctx* ctx, const void* q, const emx_paged_kv* kv, const em
  * n_draft + 1]: the accepted drafts, that token, then -1; accepted
  * int32[n_seqs]: how many drafts.  Comparisons are exact and sums in fp64, but
  * for what rounding p - q to fp32 leaves of it (below 2^-24), which is summed in
- * fp32; the rows need not sum to 1, and entries that are negative or not finite carry no
- * mass.  No mass at all: -1 in the token's place.  counts[i] < 0: an empty
- * slot, all -1 and 0 accepted.  A draft outside [0, vocab) is refused
- * and reports EMX_DEV_BAD_TOKEN. */
+ * fp32; the rows need not sum to 1, and entries that are negative or not
+ * finite carry no mass.  No mass at all: -1 in the token's place.
+ * counts[i] < 0: an empty slot, all -1 and 0 accepted.  A draft outside
+ * [0, vocab) is refused and reports EMX_DEV_BAD_TOKEN. */
 int emx_verify_draft(emx_ctx* ctx, const void* target, const void* draft, emx_dtype dtype, const int32_t* tokens,
                      const int32_t* counts, const float* uniforms, int n_seqs, int n_draft, int vocab, int32_t* out,
                      int32_t* accepted);
