@@ -981,19 +981,18 @@ def takes_tensor_memory(ctx, c):
 
 
 def attend_64(c):
-    """Case.attend on the device."""
+    """Case.attend on the device; the pages are looked up on the host."""
     torch = pytest.importorskip("torch")
-    t = lambda x: torch.from_numpy(emx.f32(x)).cuda().double()  # noqa: E731
-    k, v, q = t(c.k), t(c.v), t(c.q)
     out, size = (np.zeros((c.n, c.n_q, c.hd)) for _ in range(2))
     for i in range(c.n_seqs):
-        p = torch.arange(c.lens[i], device="cuda")
-        pages, off = torch.from_numpy(c.table[i]).cuda().long()[p // c.page], p % c.page
-        ks, vs = k[pages, :, off], v[pages, :, off]
+        if not c.rows[i]:
+            continue
+        ks, vs = (torch.from_numpy(c.keys(i, x)).cuda() for x in (c.k, c.v))
+        q = torch.from_numpy(emx.f32(c.q[c.indptr[i]:c.indptr[i + 1]])).cuda().double()
         for j, pos in enumerate(c.positions(i)):
-            row = c.indptr[i] + j
-            s = torch.einsum("hgd,shd->hgs", q[row].view(c.n_kv, -1, c.hd), ks[:pos + 1]) * c.scale
+            s = torch.einsum("hgd,shd->hgs", q[j].view(c.n_kv, -1, c.hd), ks[:pos + 1]) * c.scale
             w = torch.softmax(s, -1)
+            row = c.indptr[i] + j
             out[row] = torch.einsum("hgs,shd->hgd", w, vs[:pos + 1]).reshape(c.n_q, c.hd).cpu().numpy()
             size[row] = torch.einsum("hgs,shd->hgd", w, vs[:pos + 1].abs()).reshape(c.n_q, c.hd).cpu().numpy()
     return out, size
